@@ -31,6 +31,10 @@ FV_HASH_RAW = 2
 FV_HASH_NO_UNK = 4
 FV_HASH_EXACT = 8
 
+#: element types and activations of the dense operators
+DTYPES = {"float32": 0, "bfloat16": 1, "float16": 2}
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+
 STATUS_NAMES = {1: "FV_ERR_INVALID", 2: "FV_ERR_CUDA", 3: "FV_ERR_COMM", 4: "FV_ERR_STATE", 5: "FV_ERR_DATA",
                 6: "FV_ERR_TIMEOUT"}
 
@@ -64,6 +68,7 @@ class FvRunStats(C.Structure):
 
 
 _P = C.c_void_p
+_I = C.c_int64
 _PROTOTYPES = {
     "fv_version": ([], C.c_int),
     "fv_last_error": ([], C.c_char_p),
@@ -113,6 +118,18 @@ _PROTOTYPES = {
     "fv_hash_windows_device": ([_P, _P, C.c_uint64, C.c_uint32, C.c_int, C.c_uint32, C.c_uint32, _P,
                                 C.POINTER(C.c_double)], C.c_int),
     "fv_hasher_set_inverse_frequency": ([_P, _P, C.c_uint32], C.c_int),
+    "fv_layer_norm": ([C.c_int, _P, _P, _I, _I, _I, C.c_int, _P, _P, C.c_float, _P, C.c_int, _P, _P], C.c_int),
+    "fv_layer_norm_backward_workspace": ([C.c_int, _I, _I, C.c_int, C.POINTER(C.c_size_t)], C.c_int),
+    "fv_layer_norm_backward": ([C.c_int, _P, _P, _I, _P, _I, _I, _I, C.c_int, _P, _P, _P, _P, _P, _P, _P, C.c_size_t], C.c_int),
+    "fv_linear_workspace": ([_I, _I, _I, _P, _I, _I, _P, _I, _I, C.POINTER(C.c_size_t)], C.c_int),
+    "fv_linear": ([C.c_int, _P, _P, _I, _I, _P, _I, _I, _I, _I, _I, C.c_int, _P, C.c_int, _P, _I, _P, C.c_int, _P, _P, C.c_size_t],
+                  C.c_int),
+    "fv_linear_backward_workspace": ([C.c_int, _I, _I, _I, _P, _I, _P, _I, _I, _P, _I, _I, C.c_int, C.POINTER(C.c_size_t)], C.c_int),
+    "fv_linear_backward": ([C.c_int, _P, _P, _I, _P, _I, _I, _P, _I, _I, _I, _I, _I, C.c_int, _P, _I, C.c_int, _P, _P, _P, _P,
+                            C.c_size_t], C.c_int),
+    "fv_token_log_probs": ([C.c_int, _P, _P, _I, _I, _I, C.c_int, _P, C.c_int, C.c_float, C.c_int, _P, _P, _P, _P, _P, _P], C.c_int),
+    "fv_token_log_probs_backward": ([C.c_int, _P, _P, _P, _P, _I, _I, _I, C.c_int, _P, C.c_int, _P, _P, _P, C.c_float, _P], C.c_int),
+    "fv_ops_status": ([C.c_int, C.POINTER(C.c_uint32)], C.c_int),
     "fv_device_alloc": ([C.c_int, C.c_size_t, C.POINTER(_P)], C.c_int),
     "fv_device_free": ([C.c_int, _P], C.c_int),
     "fv_host_alloc_pinned": ([C.c_size_t, C.POINTER(_P)], C.c_int),

@@ -1,0 +1,1036 @@
+// Matrix product with bias, activation and residual in its epilogue, and its gradients.
+//
+//   forward    z = x w^T + b     y = act(z) + residual           x [rows][inner], w [outer][inner]
+//   backward   dz = dy act'(z)   dx = dz w     dw = dz^T x     db = sum_rows dz     (the residual's gradient is dy)
+//
+// All three products are one kernel, k_gemm: D[m][n] = sum_k A[m][k] B[n][k] in 16-bit operands with float accumulators.
+// An operand may be stored with k contiguous ("k-major") or with its row index contiguous ("mn-major"), so the
+// gradients and transposed weights need no transposition: only the shape of the TMA boxes, the strides in the
+// shared-memory descriptor and two bits of the instruction descriptor differ.
+//
+// k_gemm: one persistent block per SM.  One thread issues TMA loads into a ring of 64-deep k-blocks (192 KB of
+// shared memory, 128-byte swizzle), one thread issues tcgen05.mma on them (128 x BN tile, BN = 64, 128 or 256; the
+// accumulator sits in TMEM twice, so that the next tile's products run under the previous tile's epilogue), eight
+// warps take the accumulator through bias, activation and residual and out by way of shared memory, so that rows
+// leave in full 32-byte sectors.  Edges cost nothing extra: TMA fills zeros beyond the tensor, stores are guarded.
+// When there are fewer tiles than SMs, 2 to 8 blocks of a cluster share a tile's k range and add their partial
+// tiles over distributed shared memory, in rank order (no atomics, no workspace: the same bits every time).
+//
+// With at most 64 rows (serving) the product is bound by reading w.  Up to 4 rows it is done by plain loads and float
+// FMAs (k_gemv), above that by k_gemm with the roles exchanged: w's rows fill the 128-row side of the tile and the few
+// rows of x its narrow side.
+//
+// TMA needs 16-byte aligned rows.  Operands without them are copied once into rows of a multiple of 8 elements
+// (k_pack) in the caller's workspace; everything else is read where it lies.
+//
+// Roundings to 16 bits: the outputs, and dz before it enters the two products (as tensor-core operands have to be; db
+// is formed from the unrounded dz).
+//
+// Every wait is bounded: a wait that runs out raises a flag (fv_ops_status), the block drains what it has in
+// flight, frees its TMEM and returns.
+#include <cuda.h>
+
+#include <algorithm>
+
+#include "fv_ops.h"
+
+namespace fvo {
+namespace {
+
+// ---- activations ------------------------------------------------------------------------------------
+__device__ __forceinline__ float act_value(float z, int act) {
+  switch (act) {
+    case FV_ACT_RELU: return z < 0.f ? 0.f : z;  // keeps a NaN
+    case FV_ACT_GELU: return 0.5f * z * erfcf(-0.70710678f * z);  // erfc: no cancellation for z < 0
+    case FV_ACT_GELU_TANH: {
+      const float u = 0.7978845608f * fmaf(0.044715f * z * z, z, z);
+      return __fdividef(z, 1.0f + __expf(-2.0f * u));  // (1 + tanh u) / 2 = 1 / (1 + exp(-2 u))
+    }
+    case FV_ACT_SILU: return __fdividef(z, 1.0f + __expf(-z));
+    default: return z;
+  }
+}
+__device__ __forceinline__ float act_slope(float z, int act) {
+  switch (act) {
+    case FV_ACT_RELU: return z > 0.f ? 1.f : z <= 0.f ? 0.f : z;
+    case FV_ACT_GELU: return fmaf(z, 0.3989422804f * __expf(-0.5f * z * z), 0.5f * erfcf(-0.70710678f * z));
+    case FV_ACT_GELU_TANH: {
+      if (fabsf(z) > 16.f) return z > 0.f ? 1.f : 0.f;  // to float's last bit; beyond, z * z may overflow
+      const float z2 = z * z, u = 0.7978845608f * fmaf(0.044715f * z2, z, z);
+      const float s = __fdividef(1.0f, 1.0f + __expf(-2.0f * u));
+      return s + z * (2.0f * s * (1.0f - s)) * 0.7978845608f * fmaf(3.0f * 0.044715f, z2, 1.0f);
+    }
+    case FV_ACT_SILU: {
+      const float s = __fdividef(1.0f, 1.0f + __expf(-z));
+      return s * fmaf(z, 1.0f - s, 1.0f);
+    }
+    default: return 1.f;
+  }
+}
+
+// ---- device-side status -----------------------------------------------------------------------------
+__device__ unsigned g_status = 0;
+
+// ---- PTX --------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+constexpr long long WAIT_CYCLES = 4000000000ll;  // about two seconds
+// Waits for the phase of the given parity; false when the limit ran out here or elsewhere in the block.
+__device__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* stop) {
+  if (mbar_try(bar, parity)) return true;
+  const long long t0 = clock64();
+  for (;;) {
+    if (mbar_try(bar, parity)) return true;
+    if (*stop) return false;
+    if (clock64() - t0 > WAIT_CYCLES) {
+      *stop = 1;
+      atomicOr(&g_status, 1u);
+      return false;
+    }
+  }
+}
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+               "l"(map), "r"(x), "r"(y), "r"(bar)
+               : "memory");
+}
+// Shared-memory matrix descriptor, 128-byte swizzle; byte offsets in units of 16.
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead, uint32_t stride) {
+  return (uint64_t)((addr & 0x3ffff) >> 4) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(stride >> 4) << 32 | (uint64_t)1 << 46 |
+         (uint64_t)2 << 61;
+}
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// 32 lanes (the warp's quarter) x 32 columns
+__device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+        "=r"(r[31])
+      : "r"(addr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr, uint32_t rank) {
+  uint32_t far;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(far) : "r"(addr), "r"(rank));
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(far) : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// ---- the product ------------------------------------------------------------------------------------
+constexpr int BM = 128, BK = 64;                 // tile rows, depth of a k-block
+constexpr int RING_BYTES = 192 << 10;            // operand ring
+constexpr int EPI_WARPS = 8;
+constexpr int GEMM_THREADS = 64 + 32 * EPI_WARPS;
+constexpr int STAGE_OUT = 32 * 128;              // an epilogue warp's staging: 32 rows of 128 bytes
+constexpr int GEMM_SMEM = 1024 + RING_BYTES + EPI_WARPS * STAGE_OUT + 256;
+
+struct GemmParams {
+  int64_t m, n;        // rows of A, rows of B
+  int kblocks, tiles_m, tiles_n, splits;
+  int a_mn, b_mn;      // operand stored with its row index contiguous
+  uint32_t idesc;
+  int act, out_f32, swap;  // swap: D is stored transposed, out[n][m]; bias runs along m
+  int vec_y, vec_z, vec_r; // rows of y, z, residual start on 16-byte boundaries
+  const void *bias, *residual;
+  void *y, *z;
+  int64_t ldr, ldy, ldz;
+};
+
+// Where a tile lies.  Tiles are taken in bands of 16 row tiles, column by column within a band, so that the blocks
+// at work at one time share operand tiles in L2.
+__device__ __forceinline__ void tile_at(const GemmParams& p, int t, int& tm, int& tn) {
+  constexpr int BAND = 16;
+  const int per = BAND * p.tiles_n, band = t / per, in = t - band * per;
+  const int rows = min(BAND, p.tiles_m - band * BAND);
+  tn = in / rows;
+  tm = band * BAND + in - tn * rows;
+}
+
+template <typename T>
+__device__ __forceinline__ void stage_row(uint8_t* stage, int row, const float (&v)[32], bool f32) {
+  uint8_t* base = stage + row * 128;
+  if (f32) {
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      *reinterpret_cast<float4*>(base + ((c ^ (row & 7)) << 4)) = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+  } else {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      Pack<T, 8> o;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o.e[i] = from_f<T>(v[8 * c + i]);
+      *reinterpret_cast<uint4*>(base + ((c ^ (row & 7)) << 4)) = o.w;
+    }
+  }
+}
+// The staged 32 x 32 elements (of `es` bytes) to rows [r0, ...) and columns [c0, ...) of an array, guarded.
+__device__ __forceinline__ void stage_out(const uint8_t* stage, void* out, int64_t ld, int es, bool vec, int64_t r0, int64_t c0,
+                                          int64_t rows, int64_t cols) {
+  const int lane = threadIdx.x & 31;
+  uint8_t* base = static_cast<uint8_t*>(out);
+  if (vec && c0 + 32 <= cols) {
+    const int per = es == 4 ? 8 : 4;  // 16-byte words in a row
+    const int c = lane & (per - 1);
+#pragma unroll 4
+    for (int r = lane / per; r < 32; r += 32 / per)
+      if (r0 + r < rows)
+        *reinterpret_cast<uint4*>(base + ((r0 + r) * ld + c0) * es + c * 16) =
+            *reinterpret_cast<const uint4*>(stage + r * 128 + ((c ^ (r & 7)) << 4));
+  } else if (c0 + lane < cols) {
+#pragma unroll 4
+    for (int r = 0; r < 32; ++r)
+      if (r0 + r < rows) {
+        const uint8_t* s = stage + r * 128 + (((lane * es >> 4) ^ (r & 7)) << 4) + (lane * es & 15);
+        uint8_t* d = base + ((r0 + r) * ld + c0 + lane) * es;
+        if (es == 4)
+          *reinterpret_cast<uint32_t*>(d) = *reinterpret_cast<const uint32_t*>(s);
+        else
+          *reinterpret_cast<uint16_t*>(d) = *reinterpret_cast<const uint16_t*>(s);
+      }
+  }
+}
+// 32 x 32 16-bit elements of an array into the staging rows; what lies outside reads as 0.
+__device__ __forceinline__ void stage_in(uint8_t* stage, const void* in, int64_t ld, bool vec, int64_t r0, int64_t c0, int64_t rows,
+                                         int64_t cols) {
+  const int lane = threadIdx.x & 31;
+  const uint8_t* base = static_cast<const uint8_t*>(in);
+  if (vec && c0 + 32 <= cols) {
+    const int c = lane & 3;
+    uint4 w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int r = lane / 4 + 8 * k;
+      w[k] = make_uint4(0, 0, 0, 0);
+      if (r0 + r < rows) w[k] = __ldg(reinterpret_cast<const uint4*>(base + ((r0 + r) * ld + c0) * 2 + c * 16));
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int r = lane / 4 + 8 * k;
+      *reinterpret_cast<uint4*>(stage + r * 128 + ((c ^ (r & 7)) << 4)) = w[k];
+    }
+  } else {
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r) {
+      uint16_t v = 0;
+      if (r0 + r < rows && c0 + lane < cols) v = __ldg(reinterpret_cast<const uint16_t*>(base + ((r0 + r) * ld + c0 + lane) * 2));
+      *reinterpret_cast<uint16_t*>(stage + r * 128 + (((lane >> 3) ^ (r & 7)) << 4) + (lane & 7) * 2) = v;
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store_one(const GemmParams& p, int64_t r, int64_t c, float v) {  // r, c: row and column of y
+  if (p.z) static_cast<T*>(p.z)[r * p.ldz + c] = from_f<T>(v);
+  v = act_value(v, p.act);
+  if (p.residual) v += to_f<T>(static_cast<const T*>(p.residual)[r * p.ldr + c]);
+  if (p.out_f32)
+    static_cast<float*>(p.y)[r * p.ldy + c] = v;
+  else
+    static_cast<T*>(p.y)[r * p.ldy + c] = from_f<T>(v);
+}
+
+template <typename T, int BN>
+__global__ void __launch_bounds__(GEMM_THREADS, 1)
+    k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ GemmParams p) {
+  constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2, STAGE = A_BYTES + B_BYTES, STAGES = RING_BYTES / STAGE;
+  constexpr int TMEM_COLS = 2 * BN;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* staging = smem + RING_BYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(staging + EPI_WARPS * STAGE_OUT);
+  volatile int* stop = reinterpret_cast<volatile int*>(bars + 2 * STAGES + 5);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 6);
+  const uint32_t ring = smem_u32(smem), bar0 = smem_u32(bars);
+  auto full = [&](int s) { return bar0 + 8 * s; };
+  auto empty = [&](int s) { return bar0 + 8 * (STAGES + s); };
+  auto acc_full = [&](int a) { return bar0 + 8 * (2 * STAGES + a); };
+  auto acc_empty = [&](int a) { return bar0 + 8 * (2 * STAGES + 2 + a); };
+  const uint32_t drained = bar0 + 8 * (2 * STAGES + 4);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(acc_full(a), 1);
+      mbar_init(acc_empty(a), EPI_WARPS);
+    }
+    mbar_init(drained, 1);
+    *stop = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "n"(TMEM_COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  // blocks of one cluster (splits > 1) share a tile and divide its k-blocks; otherwise a block walks over its tiles
+  const int rank = p.splits > 1 ? blockIdx.x % p.splits : 0;
+  const int kb0 = (int)((int64_t)p.kblocks * rank / p.splits), kb1 = (int)((int64_t)p.kblocks * (rank + 1) / p.splits);
+  const int first = blockIdx.x / p.splits, step = gridDim.x / p.splits, tiles = p.tiles_m * p.tiles_n;
+
+  if (warp == 0) {
+    if (lane == 0) {  // loads
+      int s = 0, phase = 0, issued = 0;
+      bool ok = true;
+      for (int t = first; t < tiles && ok; t += step) {
+        int tm, tn;
+        tile_at(p, t, tm, tn);
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!(ok = mbar_wait(empty(s), phase ^ 1, stop))) break;
+          const uint32_t a = ring + s * STAGE, b = a + A_BYTES;
+          mbar_expect(full(s), STAGE);
+          if (p.a_mn) {
+#pragma unroll
+            for (int j = 0; j < BM / 64; ++j) tma_load(a + j * 8192, &map_a, tm * BM + j * 64, kb * BK, full(s));
+          } else {
+            tma_load(a, &map_a, kb * BK, tm * BM, full(s));
+          }
+          if (p.b_mn) {
+#pragma unroll
+            for (int j = 0; j < BN / 64; ++j) tma_load(b + j * 8192, &map_b, tn * BN + j * 64, kb * BK, full(s));
+          } else {
+            tma_load(b, &map_b, kb * BK, tn * BN, full(s));
+          }
+          ++issued;
+          if (++s == STAGES) {
+            s = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      if (!ok) {  // the copies in flight must land before the block ends
+        volatile int never = 0;
+        for (int i = 0; i < STAGES && i < issued; ++i) {
+          if (--s < 0) {
+            s = STAGES - 1;
+            phase ^= 1;
+          }
+          if (!mbar_wait(full(s), phase, &never)) break;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {  // products
+      // one 16-deep step inside a 64-deep k-block: 32 bytes along k-major rows, 16 rows of 128 bytes otherwise
+      const uint32_t a_step = p.a_mn ? 2048 : 32, b_step = p.b_mn ? 2048 : 32;
+      const uint32_t a_lead = p.a_mn ? 8192 : 16, b_lead = p.b_mn ? 8192 : 16;
+      int s = 0, phase = 0, acc = 0, acc_phase = 0;
+      bool ok = true;
+      for (int t = first; t < tiles && ok; t += step) {
+        if (!(ok = mbar_wait(acc_empty(acc), acc_phase ^ 1, stop))) break;
+        tc_fence_after();
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!(ok = mbar_wait(full(s), phase, stop))) break;
+          tc_fence_after();
+          const uint32_t a = ring + s * STAGE, b = a + A_BYTES;
+#pragma unroll
+          for (int k = 0; k < BK / 16; ++k)
+            mma_f16(tmem + acc * BN, smem_desc(a + k * a_step, a_lead, 1024), smem_desc(b + k * b_step, b_lead, 1024), p.idesc,
+                    kb != kb0 || k != 0);
+          mma_commit(empty(s));
+          if (++s == STAGES) {
+            s = 0;
+            phase ^= 1;
+          }
+        }
+        if (!ok) break;
+        mma_commit(acc_full(acc));
+        if (++acc == 2) {
+          acc = 0;
+          acc_phase ^= 1;
+        }
+      }
+      if (!ok) {  // products in flight must end before TMEM is freed
+        volatile int never = 0;
+        mma_commit(drained);
+        mbar_wait(drained, 0, &never);
+      }
+    }
+  } else {
+    // epilogue: warp w reads the TMEM lanes of its quarter; two warps share a quarter and take 32-column slices in turn
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    uint8_t* stage = staging + (warp - 2) * STAGE_OUT;
+    const T* bias = static_cast<const T*>(p.bias);
+    int acc = 0, acc_phase = 0;
+    for (int t = first; t < tiles; t += step) {
+      int tm, tn;
+      tile_at(p, t, tm, tn);
+      if (!mbar_wait(acc_full(acc), acc_phase, stop)) break;
+      tc_fence_after();
+      const int64_t r0 = (int64_t)tm * BM + quarter * 32;
+      const uint32_t src = tmem + acc * BN + ((uint32_t)(quarter * 32) << 16);
+      if (p.splits > 1) {  // to shared memory (the ring is free: every load was consumed before acc_full)
+        float* part = reinterpret_cast<float*>(smem);
+        for (int c = half * 32; c < BN; c += 64) {
+          float v[32];
+          tmem_load32(src + c, v);
+          float4* d = reinterpret_cast<float4*>(part + (quarter * 32 + lane) * (BN + 4) + c);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) d[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        }
+        break;  // one tile per cluster
+      }
+      for (int c = half * 32; c < BN; c += 64) {
+        const int64_t c0 = (int64_t)tn * BN + c;
+        float v[32];
+        if (c0 >= p.n || r0 >= p.m) continue;  // nothing of this slice exists (uniform over the warp)
+        if (p.swap) {
+          tmem_load32(src + c, v);
+          const int64_t o = r0 + lane;
+          if (o < p.m) {
+            const float bv = bias ? to_f<T>(bias[o]) : 0.f;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (c0 + i < p.n) store_one<T>(p, c0 + i, o, v[i] + bv);
+          }
+          continue;
+        }
+        float bv = 0.f;
+        if (bias && c0 + lane < p.n) bv = to_f<T>(bias[c0 + lane]);
+        float res[32];
+        if (p.residual) {
+          stage_in(stage, p.residual, p.ldr, p.vec_r, r0, c0, p.m, p.n);
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            Pack<T, 8> w;
+            w.w = *reinterpret_cast<const uint4*>(stage + lane * 128 + ((k ^ (lane & 7)) << 4));
+#pragma unroll
+            for (int i = 0; i < 8; ++i) res[8 * k + i] = to_f<T>(w.e[i]);
+          }
+          __syncwarp();
+        }
+        tmem_load32(src + c, v);
+        if (bias) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] += __shfl_sync(FULL, bv, i);
+        }
+        if (p.z) {
+          stage_row<T>(stage, lane, v, false);
+          __syncwarp();
+          stage_out(stage, p.z, p.ldz, 2, p.vec_z, r0, c0, p.m, p.n);
+          __syncwarp();
+        }
+        if (p.act != FV_ACT_NONE) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = act_value(v[i], p.act);
+        }
+        if (p.residual) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] += res[i];
+        }
+        stage_row<T>(stage, lane, v, p.out_f32);
+        __syncwarp();
+        stage_out(stage, p.y, p.ldy, p.out_f32 ? 4 : 2, p.vec_y, r0, c0, p.m, p.n);
+        __syncwarp();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(acc_empty(acc));
+      if (++acc == 2) {
+        acc = 0;
+        acc_phase ^= 1;
+      }
+    }
+  }
+  __syncwarp();
+  if (p.splits > 1) {
+    __syncthreads();
+    __syncwarp();
+    cluster_barrier();
+    // this block finishes 128 / splits rows of the tile from all blocks' partial tiles
+    if (!*stop && first < tiles) {
+      int tm, tn;
+      tile_at(p, first, tm, tn);
+      const int rows = BM / p.splits, row0 = rank * rows;
+      const T* bias = static_cast<const T*>(p.bias);
+      constexpr int QUADS = BN / 4;
+      for (int i = threadIdx.x; i < rows * QUADS; i += GEMM_THREADS) {
+        // consecutive threads along the output's contiguous axis
+        const int r = row0 + (p.swap ? i % rows : i / QUADS), c = 4 * (p.swap ? i / rows : i % QUADS);
+        const int64_t m = (int64_t)tm * BM + r, n = (int64_t)tn * BN + c;
+        if (m >= p.m || n >= p.n) continue;
+        const uint32_t at = ring + (r * (BN + 4) + c) * 4;
+        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k = 0; k < p.splits; ++k) {
+          const float4 q = ld_cluster4(at, k);
+          s.x += q.x;
+          s.y += q.y;
+          s.z += q.z;
+          s.w += q.w;
+        }
+        const float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n + j < p.n) {
+            if (p.swap)
+              store_one<T>(p, n + j, m, v[j] + (bias ? to_f<T>(bias[m]) : 0.f));
+            else
+              store_one<T>(p, m, n + j, v[j] + (bias ? to_f<T>(bias[n + j]) : 0.f));
+          }
+      }
+    }
+    __syncwarp();
+    cluster_barrier();  // nobody leaves while others read its shared memory
+  }
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(TMEM_COLS) : "memory");
+  }
+}
+
+// ---- up to four rows --------------------------------------------------------------------------------
+// G lanes share an output column: each reads 16 bytes of the weight's row at a time and multiplies them with the rows
+// of x, which lie in shared memory as floats.  Bound by reading w once.
+constexpr int GEMV_THREADS = 256, GEMV_CHUNK = 4096;
+template <typename T, int VEC, int G, int MT>
+__global__ void __launch_bounds__(GEMV_THREADS)
+    k_gemv(const T* __restrict__ x, int64_t ldx, const T* __restrict__ w, int64_t ldw, int64_t inner, int64_t outer, GemmParams p) {
+  extern __shared__ float xs[];  // [MT][chunk]
+  const int lane = threadIdx.x & (G - 1);
+  const int64_t o = ((int64_t)blockIdx.x * GEMV_THREADS + threadIdx.x) / G;
+  const bool live = o < outer;
+  const T* wr = w + (live ? o : 0) * ldw;
+  const int chunk = (int)min(inner, (int64_t)GEMV_CHUNK), pitch = (chunk + VEC - 1) / VEC * VEC;
+  float acc[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) acc[m] = 0.f;
+  for (int64_t k0 = 0; k0 < inner; k0 += chunk) {
+    const int n = (int)min((int64_t)chunk, inner - k0);
+    if (k0) __syncthreads();
+    for (int i = threadIdx.x; i < MT * n; i += GEMV_THREADS) {
+      const int m = i / n, k = i - m * n;
+      xs[m * pitch + k] = to_f<T>(x[m * ldx + k0 + k]);
+    }
+    __syncthreads();
+    if (live) {
+#pragma unroll 4
+      for (int k = lane * VEC; k < n; k += G * VEC) {
+        const Pack<T, VEC> q = load_pack_stream<T, VEC>(wr + k0 + k);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const float f = to_f<T>(q.e[i]);
+#pragma unroll
+          for (int m = 0; m < MT; ++m) acc[m] = fmaf(f, xs[m * pitch + k + i], acc[m]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int s = G / 2; s; s >>= 1) acc[m] += __shfl_xor_sync(FULL, acc[m], s);
+  if (live && lane == 0) {
+    const float bv = p.bias ? to_f<T>(static_cast<const T*>(p.bias)[o]) : 0.f;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) store_one<T>(p, m, o, acc[m] + bv);
+  }
+}
+
+// ---- copies, gradients' first step ------------------------------------------------------------------
+// src [rows][cols] with any row stride to dst with rows of `pitch` (a multiple of 8) elements.
+__global__ void __launch_bounds__(256) k_pack(const uint16_t* __restrict__ src, int64_t ld, int64_t rows, int64_t cols, uint16_t* __restrict__ dst,
+                                              int64_t pitch) {
+  const int64_t c0 = ((int64_t)blockIdx.x * 32 + (threadIdx.x & 31)) * 8;
+  if (c0 >= cols) return;
+  for (int64_t r = (int64_t)blockIdx.y * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.y * 8) {
+    Pack<__half, 8> o;
+    uint16_t v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = c0 + i < cols ? __ldg(src + r * ld + c0 + i) : (uint16_t)0;
+    o.w = make_uint4(v[0] | (uint32_t)v[1] << 16, v[2] | (uint32_t)v[3] << 16, v[4] | (uint32_t)v[5] << 16, v[6] | (uint32_t)v[7] << 16);
+    *reinterpret_cast<uint4*>(dst + r * pitch + c0) = o.w;
+  }
+}
+
+// dz = dy act'(z) (if dz) and the partial column sums part[blockIdx.y][outer]; a warp takes every eighth row of the
+// block's range, a lane VEC columns.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256)
+    k_act_grad(const T* __restrict__ dy, int64_t ldg, const T* __restrict__ z, int64_t ldz, int64_t rows, int64_t outer, int act,
+               T* __restrict__ dz, int64_t pitch, float* __restrict__ part) {
+  __shared__ float sum[8][32 * VEC];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t c = ((int64_t)blockIdx.x * 32 + lane) * VEC;
+  const int64_t r0 = rows * blockIdx.y / gridDim.y, r1 = rows * (blockIdx.y + 1) / gridDim.y;
+  float s[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) s[i] = 0.f;
+  if (c < outer) {
+#pragma unroll 2
+    for (int64_t r = r0 + warp; r < r1; r += 8) {
+      Pack<T, VEC> g = load_pack_stream<T, VEC>(dy + r * ldg + c);
+      if (act != FV_ACT_NONE) {
+        const Pack<T, VEC> q = load_pack_stream<T, VEC>(z + r * ldz + c);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const float v = to_f<T>(g.e[i]) * act_slope(to_f<T>(q.e[i]), act);
+          s[i] += v;
+          g.e[i] = from_f<T>(v);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) s[i] += to_f<T>(g.e[i]);
+      }
+      if (dz) store_pack<T, VEC>(dz + r * pitch + c, g);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) sum[warp][lane * VEC + i] = s[i];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 32 * VEC; i += 256) {
+    const int64_t col = (int64_t)blockIdx.x * 32 * VEC + i;
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) v += sum[w][i];
+    if (col < outer) part[(int64_t)blockIdx.y * outer + col] = v;
+  }
+}
+template <typename T>
+__global__ void __launch_bounds__(512) k_col_sum(const float* __restrict__ part, int64_t P, int64_t n, T* __restrict__ out) {
+  __shared__ float sum[16][33];
+  const int64_t c = (int64_t)blockIdx.x * 32 + threadIdx.x;
+  float s = 0.f;
+  if (c < n)
+    for (int64_t q = threadIdx.y; q < P; q += 16) s += part[q * n + c];
+  sum[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.y == 0 && c < n) {
+#pragma unroll
+    for (int k = 1; k < 16; ++k) s += sum[k][threadIdx.x];
+    out[c] = from_f<T>(s);
+  }
+}
+
+// ---- host side --------------------------------------------------------------------------------------
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                              const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                              CUtensorMapFloatOOBfill);
+EncodeFn encode_fn() {
+  static EncodeFn fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<EncodeFn>(f);
+  }();
+  return fn;
+}
+
+// A matrix as the product sees it: `rows` x `depth`; element (r, k) at p[r * ld + k], or p[k * ld + r] when mn.
+struct Operand {
+  const void* p;
+  int64_t rows, depth, ld;
+  bool mn;
+  int64_t inner() const { return mn ? rows : depth; }
+  int64_t outer() const { return mn ? depth : rows; }
+  // TMA: 16-byte aligned rows.  A single row has no stride that matters.
+  // Rows that overlap (a broadcast) are copied too.
+  bool tma_ok() const { return (uintptr_t)p % 16 == 0 && (outer() == 1 || (ld % 8 == 0 && ld >= inner())); }
+};
+constexpr size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
+int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
+size_t packed_bytes(const Operand& o) { return align256((size_t)o.outer() * (size_t)pad8(o.inner()) * 2); }
+
+struct Workspace {
+  uint8_t* base;
+  size_t size, used = 0;
+  void* take(size_t n) {
+    void* r = base + used;
+    used += align256(n);
+    return r;
+  }
+};
+
+int pack_operand(Operand& o, Workspace& ws, cudaStream_t st) {
+  if (o.tma_ok()) return FV_OK;
+  const int64_t pitch = pad8(o.inner());
+  uint16_t* dst = static_cast<uint16_t*>(ws.take((size_t)o.outer() * (size_t)pitch * 2));
+  FV_REQUIRE(ws.used <= ws.size, FV_ERR_INVALID, "workspace too small: %llu bytes needed so far, got %llu", (unsigned long long)ws.used,
+             (unsigned long long)ws.size);
+  const unsigned gx = (unsigned)((o.inner() + 255) / 256);
+  const unsigned gy = (unsigned)std::min<int64_t>((o.outer() + 7) / 8, 4096);
+  k_pack<<<dim3(gx, gy), 256, 0, st>>>(static_cast<const uint16_t*>(o.p), o.ld, o.outer(), o.inner(), dst, pitch);
+  FV_CUDA(cudaGetLastError());
+  o.p = dst;
+  o.ld = pitch;
+  return FV_OK;
+}
+
+int make_map(CUtensorMap* map, const Operand& o, int dtype, int box_rows) {
+  const EncodeFn enc = encode_fn();
+  FV_REQUIRE(enc, FV_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
+  const cuuint64_t dims[2] = {(cuuint64_t)o.inner(), (cuuint64_t)o.outer()};
+  const cuuint64_t strides[1] = {(cuuint64_t)(o.outer() == 1 ? pad8(o.inner()) : o.ld) * 2};
+  const cuuint32_t box[2] = {64, (cuuint32_t)(o.mn ? 64 : box_rows)};
+  const cuuint32_t one[2] = {1, 1};
+  const CUresult r = enc(map, dtype == FV_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(o.p),
+                         dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  FV_REQUIRE(r == CUDA_SUCCESS, FV_ERR_CUDA, "cuTensorMapEncodeTiled failed with %d ([%lld][%lld], stride %lld)", (int)r, (long long)o.outer(),
+             (long long)o.inner(), (long long)o.ld);
+  return FV_OK;
+}
+
+struct Shape {
+  int bn, splits;
+};
+// Tile width and split of k: the combination with the least estimated time, in units of one 128 x 64 x 64 product.  A
+// block pays for its k-blocks, about six units to fill the pipeline and drain the tile, and with a split two more
+// for the exchange.
+Shape choose_shape(int64_t m, int64_t n, int64_t kblocks, int sms, bool narrow) {
+  Shape best{64, 1};
+  double least = 1e300;
+  for (int bn : {256, 128, 64}) {
+    if (narrow && bn > 64) continue;
+    const double tiles = (double)((m + BM - 1) / BM) * (double)((n + bn - 1) / bn);
+    for (int s : {1, 2, 4, 8}) {
+      if (s > 1 && (s > kblocks || tiles * s > sms)) break;
+      const double waves = (double)((int64_t)(tiles * s + sms - 1) / sms);
+      const double width = bn / 64.0;
+      const double t = waves * ((double)((kblocks + s - 1) / s) * std::max(width, 1.5) + width) + 6.0 + (s > 1 ? 2.0 + width : 0.0);
+      if (t < least) {
+        least = t;
+        best = {bn, s};
+      }
+    }
+  }
+  return best;
+}
+
+template <typename T, int BN>
+int launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const GemmParams& p, unsigned grid, int splits, cudaStream_t st) {
+  static bool ready[64] = {false};  // per device; setting it twice does no harm
+  int device = 0;
+  FV_CUDA(cudaGetDevice(&device));
+  if (device >= 64 || !ready[device]) {
+    FV_CUDA(cudaFuncSetAttribute(k_gemm<T, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, GEMM_SMEM));
+    if (device < 64) ready[device] = true;
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(GEMM_THREADS);
+  cfg.dynamicSmemBytes = GEMM_SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)splits;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = splits > 1 ? 1 : 0;
+  FV_CUDA(cudaLaunchKernelEx(&cfg, k_gemm<T, BN>, a, b, p));
+  return FV_OK;
+}
+
+// D = A B^T with the epilogue that `p` describes (its output side is filled in by the caller).
+int gemm(Operand a, Operand b, int dtype, GemmParams p, Workspace& ws, int sms, bool narrow, cudaStream_t st) {
+  if (int rc = pack_operand(a, ws, st)) return rc;
+  if (int rc = pack_operand(b, ws, st)) return rc;
+  p.m = a.rows;
+  p.n = b.rows;
+  p.kblocks = (int)((a.depth + BK - 1) / BK);
+  const Shape s = choose_shape(p.m, p.n, p.kblocks, sms, narrow);
+  p.splits = s.splits;
+  p.tiles_m = (int)((p.m + BM - 1) / BM);
+  p.tiles_n = (int)((p.n + s.bn - 1) / s.bn);
+  FV_REQUIRE((int64_t)p.tiles_m * p.tiles_n < (1ll << 30), FV_ERR_INVALID, "the product is too large");
+  p.a_mn = a.mn;
+  p.b_mn = b.mn;
+  const uint32_t type = dtype == FV_BF16 ? 1u : 0u;
+  p.idesc = 1u << 4 | type << 7 | type << 10 | (uint32_t)a.mn << 15 | (uint32_t)b.mn << 16 | (uint32_t)(s.bn / 8) << 17 | (uint32_t)(BM / 16) << 24;
+  CUtensorMap ma, mb;
+  if (int rc = make_map(&ma, a, dtype, BM)) return rc;
+  if (int rc = make_map(&mb, b, dtype, s.bn)) return rc;
+  const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
+  const unsigned grid = (unsigned)(s.splits > 1 ? tiles * s.splits : std::min<int64_t>(tiles, sms));
+  if (dtype == FV_BF16) {
+    using T = __nv_bfloat16;
+    return s.bn == 256 ? launch_gemm<T, 256>(ma, mb, p, grid, s.splits, st)
+           : s.bn == 128 ? launch_gemm<T, 128>(ma, mb, p, grid, s.splits, st)
+                         : launch_gemm<T, 64>(ma, mb, p, grid, s.splits, st);
+  }
+  using T = __half;
+  return s.bn == 256 ? launch_gemm<T, 256>(ma, mb, p, grid, s.splits, st)
+         : s.bn == 128 ? launch_gemm<T, 128>(ma, mb, p, grid, s.splits, st)
+                       : launch_gemm<T, 64>(ma, mb, p, grid, s.splits, st);
+}
+
+template <typename T, int VEC, int G>
+void launch_gemv(const T* x, int64_t ldx, const T* w, int64_t ldw, int64_t rows, int64_t inner, int64_t outer, const GemmParams& p,
+                 cudaStream_t st) {
+  const unsigned grid = (unsigned)((outer * G + GEMV_THREADS - 1) / GEMV_THREADS);
+  const size_t smem = (size_t)rows * (std::min<int64_t>(inner, GEMV_CHUNK) + VEC) * sizeof(float);
+  auto go = [&](auto kernel) {
+    if (smem > 48 << 10) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    kernel<<<grid, GEMV_THREADS, smem, st>>>(x, ldx, w, ldw, inner, outer, p);
+  };
+  switch (rows) {
+    case 1: go(k_gemv<T, VEC, G, 1>); break;
+    case 2: go(k_gemv<T, VEC, G, 2>); break;
+    case 3: go(k_gemv<T, VEC, G, 3>); break;
+    default: go(k_gemv<T, VEC, G, 4>);
+  }
+}
+
+constexpr int64_t GEMV_ROWS = 4, NARROW_ROWS = 64;
+
+// w's layout: k-major rows for k_gemv
+bool use_gemv(int64_t rows, const Operand& w) { return rows <= GEMV_ROWS && !w.mn; }
+
+// A matrix given by both strides: k-major when its second axis is contiguous, else its first must be.
+bool operand_of(const void* p, int64_t rows, int64_t depth, int64_t rs, int64_t cs, Operand* o) {
+  if (cs == 1 || depth == 1) {
+    *o = Operand{p, rows, depth, rs, false};
+    return rs >= 0;
+  }
+  if (rs == 1 || rows == 1) {
+    *o = Operand{p, rows, depth, cs, true};
+    return cs >= 0;
+  }
+  return false;
+}
+Operand transposed(const Operand& o) { return Operand{o.p, o.depth, o.rows, o.ld, !o.mn}; }
+
+bool sizes_ok(int64_t rows, int64_t inner, int64_t outer) {
+  return rows >= 0 && inner >= 1 && outer >= 1 && rows < (1ll << 31) - 256 && inner < (1ll << 31) - 256 && outer < (1ll << 31) - 256;
+}
+// Strides past these would not fit a tensor map.
+bool stride_ok(int64_t s) { return s >= 0 && s < (1ll << 38); }
+
+int64_t act_grad_chunks(int64_t rows, int64_t outer, int vec, int sms) {
+  const int64_t blocks = (outer + 32 * vec - 1) / (32 * vec);
+  return std::max<int64_t>(1, std::min<int64_t>((rows + 15) / 16, (int64_t)sms * 8 / blocks));
+}
+
+}  // namespace
+}  // namespace fvo
+
+using namespace fvo;
+
+extern "C" {
+
+int fv_ops_status(int device, uint32_t* word) {
+  FV_REQUIRE(word, FV_ERR_INVALID, "fv_ops_status: NULL argument");
+  fv::DeviceGuard guard(device);
+  FV_REQUIRE(guard.ok, FV_ERR_CUDA, "cannot select device %d", device);
+  FV_CUDA(cudaMemcpyFromSymbol(word, g_status, sizeof(uint32_t)));
+  if (*word) {
+    const uint32_t zero = 0;
+    FV_CUDA(cudaMemcpyToSymbol(g_status, &zero, sizeof(zero)));
+  }
+  return FV_OK;
+}
+
+int fv_linear_workspace(int64_t rows, int64_t inner, int64_t outer, const void* x, int64_t x_rs, int64_t x_cs, const void* w, int64_t w_rs,
+                        int64_t w_cs, size_t* bytes) {
+  FV_REQUIRE(bytes && sizes_ok(rows, inner, outer), FV_ERR_INVALID, "fv_linear_workspace: bad argument");
+  Operand ox, ow;
+  FV_REQUIRE(operand_of(x, rows, inner, x_rs, x_cs, &ox) && operand_of(w, outer, inner, w_rs, w_cs, &ow), FV_ERR_INVALID,
+             "fv_linear: one axis of x and of the weight must be contiguous");
+  *bytes = 0;
+  if (rows == 0 || (use_gemv(rows, ow) && !ox.mn)) return FV_OK;
+  if (!ox.tma_ok()) *bytes += packed_bytes(ox);
+  if (!ow.tma_ok()) *bytes += packed_bytes(ow);
+  return FV_OK;
+}
+
+int fv_linear(int device, void* stream, const void* x, int64_t x_rs, int64_t x_cs, const void* w, int64_t w_rs, int64_t w_cs, int64_t rows,
+              int64_t inner, int64_t outer, int dtype, const void* bias, int act, const void* residual, int64_t residual_stride, void* y,
+              int y_dtype, void* z, void* workspace, size_t workspace_bytes) {
+  FV_REQUIRE(dtype == FV_BF16 || dtype == FV_F16, FV_ERR_INVALID, "fv_linear: operands must be bfloat16 or float16");
+  FV_REQUIRE(y_dtype == dtype || y_dtype == FV_F32, FV_ERR_INVALID, "fv_linear: the output has the operands' type or is float32");
+  FV_REQUIRE(sizes_ok(rows, inner, outer), FV_ERR_INVALID, "fv_linear: bad shape [%lld][%lld] x [%lld][%lld]", (long long)rows,
+             (long long)inner, (long long)outer, (long long)inner);
+  FV_REQUIRE(act >= FV_ACT_NONE && act <= FV_ACT_SILU, FV_ERR_INVALID, "fv_linear: unknown activation %d", act);
+  FV_REQUIRE(stride_ok(x_rs) && stride_ok(x_cs) && stride_ok(w_rs) && stride_ok(w_cs) && stride_ok(residual_stride), FV_ERR_INVALID,
+             "fv_linear: bad stride");
+  if (rows == 0) return FV_OK;
+  FV_REQUIRE(x && w && y, FV_ERR_INVALID, "fv_linear: NULL argument");
+  Operand ox, ow;
+  FV_REQUIRE(operand_of(x, rows, inner, x_rs, x_cs, &ox) && operand_of(w, outer, inner, w_rs, w_cs, &ow), FV_ERR_INVALID,
+             "fv_linear: one axis of x and of the weight must be contiguous");
+  FV_REQUIRE(workspace_bytes == 0 || (workspace && (uintptr_t)workspace % 256 == 0), FV_ERR_INVALID,
+             "fv_linear: the workspace must be 256-byte aligned");
+  fv::DeviceGuard guard(device);
+  const int sms = sm_count(device);
+  FV_REQUIRE(guard.ok && sms > 0, FV_ERR_CUDA, "cannot select device %d", device);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  GemmParams p{};
+  p.act = act;
+  p.out_f32 = y_dtype == FV_F32;
+  p.bias = bias;
+  p.residual = residual;
+  p.ldr = residual_stride;
+  p.y = y;
+  p.z = z;
+  p.ldy = p.ldz = outer;
+  const size_t ys = p.out_f32 ? 4 : 2;
+  p.vec_y = vec_ok(y, outer, ys, 16);
+  p.vec_z = z && vec_ok(z, outer, 2, 16);
+  p.vec_r = residual && vec_ok(residual, residual_stride, 2, 16);
+  if (use_gemv(rows, ow) && !ox.mn) {
+    // eight lanes to a column when that fills the GPU, else a warp; 16-byte loads where the rows allow them
+    const bool wide = vec_ok(w, outer > 1 ? ow.ld : 0, 2, 16) && inner % 8 == 0;
+    const bool few = outer * 8 < (int64_t)sms * 1024;
+    auto run = [&](auto tag) {
+      using T = decltype(tag);
+      const T *px = static_cast<const T*>(x), *pw = static_cast<const T*>(w);
+      if (wide && !few) launch_gemv<T, 8, 8>(px, ox.ld, pw, ow.ld, rows, inner, outer, p, st);
+      else if (wide) launch_gemv<T, 8, 32>(px, ox.ld, pw, ow.ld, rows, inner, outer, p, st);
+      else launch_gemv<T, 1, 32>(px, ox.ld, pw, ow.ld, rows, inner, outer, p, st);
+    };
+    if (dtype == FV_BF16) run(__nv_bfloat16{});
+    else run(__half{});
+    FV_CUDA(cudaGetLastError());
+    return FV_OK;
+  }
+  Workspace ws{static_cast<uint8_t*>(workspace), workspace_bytes};
+  if (rows <= NARROW_ROWS) {
+    p.swap = 1;
+    return gemm(ow, ox, dtype, p, ws, sms, true, st);
+  }
+  return gemm(ox, ow, dtype, p, ws, sms, false, st);
+}
+
+// dz is written when there is an activation, or when dy cannot be read by TMA.
+static bool needs_dz(const void* dy, int64_t dy_stride, int64_t rows, int64_t outer, int act) {
+  return act != FV_ACT_NONE || !Operand{dy, rows, outer, dy_stride, false}.tma_ok();
+}
+
+int fv_linear_backward_workspace(int device, int64_t rows, int64_t inner, int64_t outer, const void* dy, int64_t dy_stride, const void* x,
+                                 int64_t x_rs, int64_t x_cs, const void* w, int64_t w_rs, int64_t w_cs, int act, size_t* bytes) {
+  FV_REQUIRE(bytes && sizes_ok(rows, inner, outer), FV_ERR_INVALID, "fv_linear_backward_workspace: bad argument");
+  Operand ox, ow;
+  FV_REQUIRE(operand_of(x, rows, inner, x_rs, x_cs, &ox) && operand_of(w, outer, inner, w_rs, w_cs, &ow), FV_ERR_INVALID,
+             "fv_linear_backward: one axis of x and of the weight must be contiguous");
+  const int sms = sm_count(device);
+  FV_REQUIRE(sms > 0, FV_ERR_CUDA, "cannot select device %d", device);
+  *bytes = 0;
+  if (rows == 0) return FV_OK;
+  if (needs_dz(dy, dy_stride, rows, outer, act)) *bytes += align256((size_t)rows * (size_t)pad8(outer) * 2);
+  *bytes += align256((size_t)act_grad_chunks(rows, outer, 1, sms) * (size_t)outer * sizeof(float)) +
+            align256((size_t)act_grad_chunks(rows, outer, 8, sms) * (size_t)outer * sizeof(float));
+  if (!ox.tma_ok()) *bytes += packed_bytes(ox);
+  if (!ow.tma_ok()) *bytes += packed_bytes(ow);
+  return FV_OK;
+}
+
+int fv_linear_backward(int device, void* stream, const void* dy, int64_t dy_stride, const void* x, int64_t x_rs, int64_t x_cs, const void* w,
+                       int64_t w_rs, int64_t w_cs, int64_t rows, int64_t inner, int64_t outer, int dtype, const void* z, int64_t z_stride,
+                       int act, void* dx, void* dw, void* db, void* workspace, size_t workspace_bytes) {
+  FV_REQUIRE(dtype == FV_BF16 || dtype == FV_F16, FV_ERR_INVALID, "fv_linear_backward: operands must be bfloat16 or float16");
+  FV_REQUIRE(sizes_ok(rows, inner, outer), FV_ERR_INVALID, "fv_linear_backward: bad shape [%lld][%lld] x [%lld][%lld]", (long long)rows,
+             (long long)inner, (long long)outer, (long long)inner);
+  FV_REQUIRE(act >= FV_ACT_NONE && act <= FV_ACT_SILU, FV_ERR_INVALID, "fv_linear_backward: unknown activation %d", act);
+  FV_REQUIRE(stride_ok(dy_stride) && stride_ok(z_stride) && stride_ok(x_rs) && stride_ok(x_cs) && stride_ok(w_rs) && stride_ok(w_cs),
+             FV_ERR_INVALID, "fv_linear_backward: bad stride");
+  FV_REQUIRE(dw && db, FV_ERR_INVALID, "fv_linear_backward: NULL argument");
+  fv::DeviceGuard guard(device);
+  const int sms = sm_count(device);
+  FV_REQUIRE(guard.ok && sms > 0, FV_ERR_CUDA, "cannot select device %d", device);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (rows == 0) {  // a sum over nothing
+    FV_CUDA(cudaMemsetAsync(dw, 0, (size_t)outer * (size_t)inner * 2, st));
+    FV_CUDA(cudaMemsetAsync(db, 0, (size_t)outer * 2, st));
+    return FV_OK;
+  }
+  FV_REQUIRE(dy && x && w && dx && (act == FV_ACT_NONE || z), FV_ERR_INVALID,
+             "fv_linear_backward: NULL argument (an activation's gradient needs the pre-activation)");
+  Operand ox, ow;
+  FV_REQUIRE(operand_of(x, rows, inner, x_rs, x_cs, &ox) && operand_of(w, outer, inner, w_rs, w_cs, &ow), FV_ERR_INVALID,
+             "fv_linear_backward: one axis of x and of the weight must be contiguous");
+  size_t need = 0;
+  if (int rc = fv_linear_backward_workspace(device, rows, inner, outer, dy, dy_stride, x, x_rs, x_cs, w, w_rs, w_cs, act, &need)) return rc;
+  FV_REQUIRE(workspace && workspace_bytes >= need && (uintptr_t)workspace % 256 == 0, FV_ERR_INVALID,
+             "fv_linear_backward: the workspace must be 256-byte aligned and hold %llu bytes, got %llu", (unsigned long long)need,
+             (unsigned long long)workspace_bytes);
+  Workspace ws{static_cast<uint8_t*>(workspace), workspace_bytes};
+  Operand od{dy, rows, outer, dy_stride, false};
+  void* dz = nullptr;
+  const int64_t pitch = pad8(outer);
+  if (needs_dz(dy, dy_stride, rows, outer, act)) {
+    dz = ws.take((size_t)rows * (size_t)pitch * 2);
+    od = Operand{dz, rows, outer, pitch, false};
+  }
+  const bool vec = outer % 8 == 0 && vec_ok(dy, dy_stride, 2, 16) && (act == FV_ACT_NONE || vec_ok(z, z_stride, 2, 16));
+  const int64_t chunks = act_grad_chunks(rows, outer, vec ? 8 : 1, sms);
+  float* part = static_cast<float*>(ws.take((size_t)chunks * (size_t)outer * sizeof(float)));
+  auto first = [&](auto tag) {
+    using T = decltype(tag);
+    const T *pg = static_cast<const T*>(dy), *pz = static_cast<const T*>(z);
+    if (vec)
+      k_act_grad<T, 8><<<dim3((unsigned)((outer + 255) / 256), (unsigned)chunks), 256, 0, st>>>(pg, dy_stride, pz, z_stride, rows, outer, act,
+                                                                                               static_cast<T*>(dz), pitch, part);
+    else
+      k_act_grad<T, 1><<<dim3((unsigned)((outer + 31) / 32), (unsigned)chunks), 256, 0, st>>>(pg, dy_stride, pz, z_stride, rows, outer, act,
+                                                                                             static_cast<T*>(dz), pitch, part);
+    k_col_sum<T><<<(unsigned)((outer + 31) / 32), dim3(32, 16), 0, st>>>(part, chunks, outer, static_cast<T*>(db));
+  };
+  if (dtype == FV_BF16) first(__nv_bfloat16{});
+  else first(__half{});
+  FV_CUDA(cudaGetLastError());
+  if (int rc = pack_operand(ox, ws, st)) return rc;
+  if (int rc = pack_operand(ow, ws, st)) return rc;
+  GemmParams p{};
+  p.y = dx;
+  p.ldy = inner;
+  p.vec_y = vec_ok(dx, inner, 2, 16);
+  if (int rc = gemm(od, transposed(ow), dtype, p, ws, sms, false, st)) return rc;
+  p.y = dw;
+  p.vec_y = vec_ok(dw, inner, 2, 16);
+  return gemm(transposed(od), transposed(ox), dtype, p, ws, sms, false, st);
+}
+
+}  // extern "C"

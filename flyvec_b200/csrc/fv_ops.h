@@ -1,0 +1,108 @@
+// Helpers shared by the dense operators (fv_norm.cu, fv_logprob.cu, fv_linear.cu): element types, 16-byte
+// vectors of them, reductions.  Nothing here allocates or synchronises.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <math_constants.h>
+
+#include "fv_common.h"
+
+namespace fvo {
+
+constexpr unsigned FULL = 0xffffffffu;
+
+template <typename T>
+__device__ __forceinline__ float to_f(T v);
+template <>
+__device__ __forceinline__ float to_f<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <>
+__device__ __forceinline__ float to_f<__half>(__half v) { return __half2float(v); }
+
+template <typename T>
+__device__ __forceinline__ T from_f(float v);
+template <>
+__device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+
+// VEC consecutive elements moved by one access.  VEC * sizeof(T) is 16, 8, 4 or 2 bytes and the address a
+// multiple of it.
+template <int BYTES>
+struct Word;
+template <>
+struct Word<16> { using type = uint4; };
+template <>
+struct Word<8> { using type = uint2; };
+template <>
+struct Word<4> { using type = unsigned; };
+template <>
+struct Word<2> { using type = unsigned short; };
+
+template <typename T, int VEC>
+union Pack {
+  typename Word<(int)sizeof(T) * VEC>::type w;
+  T e[VEC];
+  __device__ __forceinline__ Pack() {}
+};
+
+template <typename T, int VEC>
+__device__ __forceinline__ Pack<T, VEC> load_pack(const T* p) {
+  Pack<T, VEC> r;
+  r.w = *reinterpret_cast<const decltype(r.w)*>(p);
+  return r;
+}
+// read once: keep it out of L1
+template <typename T, int VEC>
+__device__ __forceinline__ Pack<T, VEC> load_pack_stream(const T* p) {
+  Pack<T, VEC> r;
+  r.w = __ldcs(reinterpret_cast<const decltype(r.w)*>(p));
+  return r;
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void store_pack(T* p, const Pack<T, VEC>& v) {
+  *reinterpret_cast<decltype(v.w)*>(p) = v.w;
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
+  return v;
+}
+
+// Bytes that divide an address and a stride: which vector width a row-major array admits.
+inline unsigned common_alignment(uintptr_t a) { return a == 0 ? 4096u : (unsigned)(a & (~a + 1)); }
+inline bool vec_ok(const void* p, int64_t stride_elems, size_t elem, unsigned bytes) {
+  return (uintptr_t)p % bytes == 0 && ((uint64_t)stride_elems * elem) % bytes == 0;
+}
+inline size_t elem_size(int dtype) { return dtype == FV_F32 ? 4 : 2; }
+
+int sm_count(int device);  // cached per device; 0 after an error
+
+}  // namespace fvo
+
+#define FV_DTYPE_SWITCH(code, T, ...)         \
+  switch (code) {                             \
+    case FV_F32: {                            \
+      using T = float;                        \
+      __VA_ARGS__;                            \
+      break;                                  \
+    }                                         \
+    case FV_BF16: {                           \
+      using T = __nv_bfloat16;                \
+      __VA_ARGS__;                            \
+      break;                                  \
+    }                                         \
+    default: {                                \
+      using T = __half;                       \
+      __VA_ARGS__;                            \
+    }                                         \
+  }
+
+#define FV_CHECK_DTYPE(code, what) \
+  FV_REQUIRE((code) == FV_F32 || (code) == FV_BF16 || (code) == FV_F16, FV_ERR_INVALID, what ": unknown element type %d", (int)(code))

@@ -425,6 +425,66 @@ class DeviceBuffer:
             pass
 
 
+class DeviceArray(DeviceBuffer):
+    """Dense row-major array in device memory, the operand of :mod:`flyvec_b200.ops` where no PyTorch is at hand.
+    ``dtype`` is a name ("float32", "bfloat16", "float16", "int32", "int64", "uint8")."""
+
+    is_cuda = True
+    _NUMPY = {"float32": np.float32, "float16": np.float16, "int32": np.int32, "int64": np.int64, "uint8": np.uint8,
+              "bfloat16": np.uint16}
+
+    def __init__(self, shape, dtype: str, device: int = 0):
+        if dtype not in self._NUMPY:
+            raise TypeError(f"dtype must be one of {', '.join(self._NUMPY)}, got {dtype!r}")
+        self.ptr = None
+        self.shape = tuple(int(n) for n in (shape if hasattr(shape, "__iter__") else (shape,)))
+        if any(n < 0 for n in self.shape):
+            raise ValueError(f"bad shape {self.shape}")
+        self.dtype = dtype
+        self.size = int(np.prod(self.shape, dtype=np.int64))
+        # never empty: a pointer is needed even for no elements
+        super().__init__(max(self.size, 1) * np.dtype(self._NUMPY[dtype]).itemsize, device)
+
+    @classmethod
+    def from_numpy(cls, a, dtype: str | None = None, device: int = 0) -> "DeviceArray":
+        """Copy of a host array, converted to ``dtype`` (bfloat16: rounded to nearest even)."""
+        a = np.ascontiguousarray(a) if np.ndim(a) else np.asarray(a)
+        dtype = a.dtype.name if dtype is None else dtype
+        out = cls(a.shape, dtype, device)
+        if dtype == "bfloat16":
+            bits = np.asarray(a, np.float32).view(np.uint32)
+            even = ((bits >> 16) & 1) + np.uint32(0x7fff)
+            host = np.where(np.isnan(a), np.uint32(0x7fc0), (bits + even) >> 16).astype(np.uint16)
+        else:
+            host = np.asarray(a, cls._NUMPY[dtype])
+        if out.size:
+            out.upload(host)
+        return out
+
+    def numpy(self) -> np.ndarray:
+        """Copy on the host (bfloat16 as float32); waits for the work enqueued before it."""
+        if not self.size:
+            return np.empty(self.shape, np.float32 if self.dtype == "bfloat16" else self._NUMPY[self.dtype])
+        a = self.download(self.shape, self._NUMPY[self.dtype])
+        return (a.astype(np.uint32) << 16).view(np.float32) if self.dtype == "bfloat16" else a
+
+    def new_empty(self, shape, dtype: str) -> "DeviceArray":
+        return DeviceArray(shape, dtype, self.device)
+
+    def data_ptr(self) -> int:
+        return self.ptr
+
+    def get_device(self) -> int:
+        return self.device
+
+    def stride(self):
+        out, step = [], 1
+        for n in reversed(self.shape):
+            out.append(step)
+            step *= max(n, 1)
+        return tuple(reversed(out))
+
+
 def flush_l2(device: int = 0, nbytes: int = 256 << 20):
     check(_lib.lib().fv_flush_l2(device, nbytes))
 

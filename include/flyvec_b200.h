@@ -286,6 +286,71 @@ int fv_hash_windows_device(fv_hasher* h, const int32_t* d_idx, uint64_t nwin, ui
                            uint32_t hash_length, uint32_t flags, uint8_t* d_out, double* kernel_seconds);
 int fv_hasher_set_inverse_frequency(fv_hasher* h, const float* inv_freq, uint32_t vocab);
 
+/* ---- dense operators -------------------------------------------------------
+ * No counterpart in the reference.  What a model on top of the embeddings learns and answers with: layer norm
+ * (beside the row normalisation of fv_hasher_create), matrix products with an epilogue, and the log
+ * probabilities of given tokens (the softmax of flyvec/core.py:17-20 over a vocabulary), with their gradients.
+ *
+ * All arrays are device memory of `device`, row-major with the given strides in elements; outputs are dense.  Calls
+ * enqueue on `stream` (a cudaStream_t; NULL is the legacy default stream), allocate nothing, keep nothing and
+ * return at once; they may be captured into a graph.  Where a call needs scratch memory the caller passes a
+ * workspace of at least the size that the ..._workspace function answers for the same arguments; a workspace must not be
+ * used by two calls that can run at the same time.  Sums, statistics and accumulators are float. */
+#define FV_F32 0
+#define FV_BF16 1
+#define FV_F16 2
+
+#define FV_ACT_NONE 0
+#define FV_ACT_RELU 1
+#define FV_ACT_GELU 2      /* z Phi(z)                     */
+#define FV_ACT_GELU_TANH 3 /* its tanh approximation       */
+#define FV_ACT_SILU 4      /* z / (1 + exp(-z))            */
+
+/* y = (x - mean) * rstd * weight + bias over the last axis; x, weight and bias of type `dtype`, y dense in `y_dtype`.
+ * weight and bias may be NULL (a bias needs a weight), mean and rstd (float [rows]) too. */
+int fv_layer_norm(int device, void* stream, const void* x, int64_t x_stride, int64_t rows, int64_t cols, int dtype, const void* weight,
+                  const void* bias, float eps, void* y, int y_dtype, float* mean, float* rstd);
+/* dx, and with a weight dweight and dbias (else both NULL; no workspace is needed then).  The sums over the rows
+ * are formed in a fixed order. */
+int fv_layer_norm_backward_workspace(int device, int64_t rows, int64_t cols, int dtype, size_t* bytes);
+int fv_layer_norm_backward(int device, void* stream, const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, int64_t rows,
+                           int64_t cols, int dtype, const float* mean, const float* rstd, const void* weight, void* dx, void* dweight,
+                           void* dbias, void* workspace, size_t workspace_bytes);
+
+/* z = x w^T + bias, y = act(z) + residual.  x [rows][inner] and w [outer][inner] in bfloat16 or float16, each given by a row and a
+ * column stride of which one is 1 (so a transposed weight needs no copy); bias [outer] and residual [rows][outer] of
+ * the same type or NULL; y in that type or float; z (may be NULL) receives the pre-activation for the backward pass.
+ * The workspace is empty unless x or w has rows that do not start on 16-byte boundaries. */
+int fv_linear_workspace(int64_t rows, int64_t inner, int64_t outer, const void* x, int64_t x_rs, int64_t x_cs, const void* w, int64_t w_rs,
+                        int64_t w_cs, size_t* bytes);
+int fv_linear(int device, void* stream, const void* x, int64_t x_rs, int64_t x_cs, const void* w, int64_t w_rs, int64_t w_cs, int64_t rows,
+              int64_t inner, int64_t outer, int dtype, const void* bias, int act, const void* residual, int64_t residual_stride, void* y,
+              int y_dtype, void* z, void* workspace, size_t workspace_bytes);
+/* dz = dy act'(z), dx = dz w, dw = dz^T x (dense [outer][inner]), db = column sums of dz; the residual's gradient is dy. */
+int fv_linear_backward_workspace(int device, int64_t rows, int64_t inner, int64_t outer, const void* dy, int64_t dy_stride, const void* x,
+                                 int64_t x_rs, int64_t x_cs, const void* w, int64_t w_rs, int64_t w_cs, int act, size_t* bytes);
+int fv_linear_backward(int device, void* stream, const void* dy, int64_t dy_stride, const void* x, int64_t x_rs, int64_t x_cs, const void* w,
+                       int64_t w_rs, int64_t w_cs, int64_t rows, int64_t inner, int64_t outer, int dtype, const void* z, int64_t z_stride,
+                       int act, void* dx, void* dw, void* db, void* workspace, size_t workspace_bytes);
+
+/* Of every row of logits: log probability of its target under softmax(beta * logits), entropy, maximum logit, log of the
+ * sum of exp(beta * (logit - maximum)), and the `top` (0..64) most probable tokens (larger logit first, then the lower id)
+ * with their log probabilities.  targets are int32 or int64; -1 marks padding (log probability 0, no gradient), any other
+ * id outside [0, vocab) gives NaN.  A row of -inf only: log probabilities -inf, entropy 0, log_z -inf, gradient 0.  A row
+ * with a NaN or +inf: NaN everywhere but in top_ids (NaN first). */
+int fv_token_log_probs(int device, void* stream, const void* logits, int64_t stride, int64_t rows, int64_t vocab, int dtype,
+                       const void* targets, int targets_int64, float beta, int top, float* log_prob, float* entropy, float* row_max,
+                       float* log_z, int32_t* top_ids, float* top_log_prob);
+/* Gradient of sum(grad_log_prob * log_prob) + sum(grad_entropy * entropy) by the logits; row_max, log_z and entropy
+ * as the forward call left them.  grad_entropy may be NULL, entropy then too. */
+int fv_token_log_probs_backward(int device, void* stream, const float* grad_log_prob, const float* grad_entropy, const void* logits,
+                                int64_t stride, int64_t rows, int64_t vocab, int dtype, const void* targets, int targets_int64,
+                                const float* row_max, const float* log_z, const float* entropy, float beta, void* dlogits);
+
+/* Error bits of this device's dense operators since the last call (bit 0: a bounded wait inside a kernel ran out and that
+ * call's outputs are invalid); waits for the device and clears them. */
+int fv_ops_status(int device, uint32_t* word);
+
 /* ---- raw buffers (cuda_helpers.cu:8-29 do_gpu_cudaHostAlloc & co.) ------- */
 int fv_device_alloc(int device, size_t bytes, void** ptr);
 int fv_device_free(int device, void* ptr);
