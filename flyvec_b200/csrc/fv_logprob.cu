@@ -10,17 +10,19 @@
 // gradient; a row with a NaN or +inf has NaN everywhere but in top_ids, whose order takes NaN as the largest.
 //
 // Forward: bound by reading the logits once.  A block (for few rows a cluster of 2 to 8 blocks that meet in the
-// first one's shared memory) streams a row with 16-byte loads and keeps, per thread, the running maximum, R and
-// A = sum e d of the elements it saw, d = log2(e) beta (x - m).  The branch that moves the maximum is rare, so an
-// element costs a widening, a compare, a subtraction, a product, ex2 and two accumulations.  The best `top`
-// alternatives cost no second pass over the row: the `top`-th largest of the threads' maxima is a lower bound of the
-// row's `top`-th largest element, and only the threads above it (about `top` of them) have anything to offer; their
-// elements are read again by whole warps.  The few candidates are ranked by counting (value first, then the
-// lower index).  Rows of at most 1024 elements go to one warp each.
+// first one's shared memory) streams a row with 16-byte loads, four in flight per thread.  A thread takes the maximum of
+// the four words first and rescales its sums once for all their elements, without a branch; an element then costs a
+// widening, half a compare, half a subtraction and product (packed), a clamp, ex2 and half of each accumulation.  The
+// largest element's 1 is taken out afterwards: one warp reads the words of the thread that saw it once more.  The best
+// `top` alternatives cost no second pass over the row either: the threads' maxima give a lower bound of the row's
+// top-th largest element, only the threads whose maximum reaches it (about 2 top of 256) have anything to offer, and
+// their words are read again (L2).  The few candidates are ranked by counting (value first, then the lower index).
+// Rows of at most 1024 elements go to one warp each.
 #include <cooperative_groups.h>
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "fv_ops.h"
 
@@ -82,59 +84,93 @@ __device__ __forceinline__ Part merge(Part p, Part q, float bl2) {
   if (e > 0.f) p.a += e * fmaf(delta, t, q.a);
   return p;
 }
-__device__ __forceinline__ Part warp_merge(Part p, float bl2) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    Part q;
-    q.m = __shfl_xor_sync(FULL, p.m, o);
-    q.r = __shfl_xor_sync(FULL, p.r, o);
-    q.a = __shfl_xor_sync(FULL, p.a, o);
-    // both sides take the same operand first, so that all lanes end with the same bits
-    p = (threadIdx.x & o) ? merge(q, p, bl2) : merge(p, q, bl2);
-  }
-  return p;
-}
 
-// One access's elements into a thread's part.
-template <int N>
-__device__ __forceinline__ void take(Part& p, const float (&x)[N], float bl2) {
-  float big = x[0];
+// A thread's running sums while it streams its elements: m their maximum (NaN once there was one), s the sum of
+// exp(beta (x - m)) and a the sum of exp(.) times the exponent, both over ALL elements including the largest.  The
+// accumulators are pairs, so that the packed float instructions do two elements at a time.
+struct Stream {
+  float m;
+  float2 s, a;
+};
+__device__ __forceinline__ u64 pack2(float2 v) { return *reinterpret_cast<u64*>(&v); }
+__device__ __forceinline__ float2 unpack2(u64 v) { return *reinterpret_cast<float2*>(&v); }
+__device__ __forceinline__ float2 add2(float2 x, float2 y) {
+  u64 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pack2(x)), "l"(pack2(y)));
+  return unpack2(r);
+}
+__device__ __forceinline__ float2 mul2(float2 x, float2 y) {
+  u64 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pack2(x)), "l"(pack2(y)));
+  return unpack2(r);
+}
+__device__ __forceinline__ float2 fma2(float2 x, float2 y, float2 z) {
+  u64 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pack2(x)), "l"(pack2(y)), "l"(pack2(z)));
+  return unpack2(r);
+}
+// two elements of a 32-bit word (one element for float: the caller passes two words)
+template <typename T>
+__device__ __forceinline__ float2 widen2(unsigned w);
+template <>
+__device__ __forceinline__ float2 widen2<__nv_bfloat16>(unsigned w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ float2 widen2<__half>(unsigned w) {
+  return __half22float2(*reinterpret_cast<__half2*>(&w));
+}
+template <typename T>
+__device__ __forceinline__ float2 pair_of(const uint4& q, int i) {  // i-th pair of a 16-byte word
+  const unsigned w[4] = {q.x, q.y, q.z, q.w};
+  if constexpr (sizeof(T) == 4)
+    return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+  else
+    return widen2<T>(w[i]);
+}
+// largest element (NaN if there is one) of N 16-byte words
+template <typename T, int N>
+__device__ __forceinline__ float words_max(const uint4 (&q)[N]) {
+  if constexpr (sizeof(T) == 4) {
+    float m = -CUDART_INF_F;
 #pragma unroll
-  for (int i = 1; i < N; ++i) big = max_nan(big, x[i]);
-  if (!(big <= p.m) || big == -CUDART_INF_F) {
-    if (big == -CUDART_INF_F) return;
-    if (p.m != p.m) return;
-    if (!(big < CUDART_INF_F)) {  // NaN or +inf: the row has no probabilities
-      p.m = big;
-      p.r = CUDART_NAN_F;
-      return;
-    }
-    // the maximum moves: what was seen so far, its old maximum included, is scaled to the new one
-    if (p.m != -CUDART_INF_F) {
-      const float delta = (p.m - big) * bl2, e = ex2(delta), t = 1.0f + p.r;
-      p.a = e > 0.f ? e * fmaf(delta, t, p.a) : 0.f;
-      p.r = e * t;
-    }
-    p.m = big;
-    bool own = true;
+    for (int u = 0; u < N; ++u)
+      m = max_nan(m, max_nan(max_nan(__uint_as_float(q[u].x), __uint_as_float(q[u].y)), max_nan(__uint_as_float(q[u].z), __uint_as_float(q[u].w))));
+    return m;
+  } else {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    auto two = [](unsigned w) { return *reinterpret_cast<T2*>(&w); };
+    T2 m = two(q[0].x);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      if (own && x[i] == big) {
-        own = false;
-      } else {
-        const float d = max_nan((x[i] - big) * bl2, -200.f), e = ex2(d);
-        p.r += e;
-        p.a = fmaf(e, d, p.a);
-      }
-    }
-    return;
+    for (int u = 0; u < N; ++u) m = __hmax2_nan(m, __hmax2_nan(__hmax2_nan(two(q[u].x), two(q[u].y)), __hmax2_nan(two(q[u].z), two(q[u].w))));
+    const float2 f = widen2<T>(*reinterpret_cast<unsigned*>(&m));
+    return max_nan(f.x, f.y);
   }
+}
+// log2(e) beta (x - m) of a pair, kept finite: below -200 its exp is 0, and 0 times it has to stay 0
+__device__ __forceinline__ float2 exponents(float2 x, float minus_m, float bl2) {
+  float2 d = mul2(add2(x, make_float2(minus_m, minus_m)), make_float2(bl2, bl2));
+  d.x = max_nan(d.x, -200.f);
+  d.y = max_nan(d.y, -200.f);
+  return d;
+}
+// N words of elements: one rescaling for all of them, without a branch, then two elements per step.
+template <typename T, int N>
+__device__ __forceinline__ void take(Stream& t, const uint4 (&q)[N], float bl2) {
+  const float m = max_nan(t.m, words_max<T, N>(q)), m0 = m == -CUDART_INF_F ? 0.f : m;
+  const float delta = max_nan((t.m - m0) * bl2, -200.f), e = ex2(delta);
+  const float2 e2 = make_float2(e, e);
+  t.a = mul2(fma2(make_float2(delta, delta), t.s, t.a), e2);
+  t.s = mul2(t.s, e2);
+  t.m = m;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float d = max_nan((x[i] - p.m) * bl2, -200.f), e = ex2(d);  // below 2^-126 e is 0 and d stays finite
-    p.r += e;
-    p.a = fmaf(e, d, p.a);
-  }
+  for (int u = 0; u < N; ++u)
+#pragma unroll
+    for (int i = 0; i < 8 / (int)sizeof(T); ++i) {
+      const float2 d = exponents(pair_of<T>(q[u], i), -m0, bl2), z = make_float2(ex2(d.x), ex2(d.y));
+      t.s = add2(t.s, z);
+      t.a = fma2(z, d, t.a);
+    }
 }
 
 struct RowOut {
@@ -194,151 +230,218 @@ struct Row {
 };
 
 // ---- forward, one block or one cluster per row ------------------------------------------------------
+// A warp's r-th largest of its lanes' keys (0 if fewer lanes hold anything).
+__device__ __forceinline__ unsigned warp_rth(unsigned key, int r) {
+  unsigned best = 0;
+  for (int k = 0; k < r; ++k) {
+    best = __reduce_max_sync(FULL, key);
+    if ((threadIdx.x & 31) == __ffs(__ballot_sync(FULL, key == best)) - 1) key = 0;
+  }
+  return best;
+}
+
 template <typename T, int THREADS>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS)
     k_log_probs(const T* __restrict__ logits, int64_t xs, int64_t V, const void* __restrict__ targets, int t64, float beta, int top,
                 int parts, RowOut out) {
-  constexpr int VEC = Row<T>::VEC, WARPS = THREADS / 32, PER = THREADS / 32;
-  __shared__ Part warp_part[WARPS];
+  constexpr int VEC = Row<T>::VEC, WARPS = THREADS / 32;
+  __shared__ unsigned warp_key[WARPS], warp_tau[WARPS];
+  __shared__ float2 warp_sum2[WARPS];
   __shared__ Part all_part[8];
-  __shared__ unsigned keys[THREADS];
   __shared__ u64 cand[LP_CAND];
   __shared__ u64 best[LP_MAX_TOP];
   __shared__ u64 gathered[8 * LP_MAX_TOP];
+  __shared__ unsigned short holder[THREADS];
   __shared__ unsigned count, tau_s, warp_n[WARPS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t row = blockIdx.x / parts;
+  const int64_t row = parts == 1 ? (int64_t)blockIdx.x : blockIdx.x / parts;
   const int rank = (int)(blockIdx.x - row * parts);
   const Row<T> rw(logits + row * xs, V);
   const float bl2 = beta * LOG2E;
-  // this block's vectors [v0, v1); the first block of a cluster also has the single elements
-  const int64_t v0 = rw.nvec * rank / parts, v1 = rw.nvec * (rank + 1) / parts;
+  // this block's vectors [v0, v0 + nv); the first block of a cluster also has the single elements
+  const int64_t v0 = parts == 1 ? 0 : rw.nvec * rank / parts;
+  const int nv = (int)((parts == 1 ? rw.nvec : rw.nvec * (rank + 1) / parts) - v0);
+  const uint4* __restrict__ vecs = reinterpret_cast<const uint4*>(rw.x + rw.vec_at(v0));
   const int ends = rank == 0 ? rw.ends : 0;
   cg::cluster_group cluster = cg::this_cluster();
   if (parts > 1) cluster.barrier_arrive();
   long long t = -1;
   float xt = 0.f;
-  if (tid == 0 && rank == 0) {
-    t = target_of(targets, t64, row);
-    xt = value_at(rw.x, V, t);
-  }
-  Part p{-CUDART_INF_F, 0.f, 0.f};
-  if (tid < ends) {
-    const float x[1] = {to_f<T>(rw.x[rw.end_at(tid)])};
-    take<1>(p, x, bl2);
-  }
-  constexpr int U = 4;  // loads in flight per thread
-  int64_t i = v0 + tid;
-  for (; i + (U - 1) * THREADS < v1; i += U * THREADS) {
-    Pack<T, VEC> w[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) w[u] = load_pack<T, VEC>(rw.x + rw.vec_at(i + u * THREADS));
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float x[VEC];
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) x[k] = to_f<T>(w[u].e[k]);
-      take<VEC>(p, x, bl2);
+  if (tid == 0) {
+    count = 0;
+    if (rank == 0) {
+      t = target_of(targets, t64, row);
+      xt = value_at(rw.x, V, t);
     }
   }
-  for (; i < v1; i += THREADS) {
-    const Pack<T, VEC> w = load_pack<T, VEC>(rw.x + rw.vec_at(i));
-    float x[VEC];
+  Stream st{-CUDART_INF_F, make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+  constexpr int U = 4;  // loads in flight per thread
+  int i = tid;
+  for (; i + (U - 1) * THREADS < nv; i += U * THREADS) {
+    uint4 q[U];
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) x[k] = to_f<T>(w.e[k]);
-    take<VEC>(p, x, bl2);
+    for (int u = 0; u < U; ++u) q[u] = vecs[i + u * THREADS];
+    take<T, U>(st, q, bl2);
+  }
+  {
+    uint4 q[1];
+    for (; i < nv; i += THREADS) {
+      q[0] = vecs[i];
+      take<T, 1>(st, q, bl2);
+    }
+  }
+  if (tid < ends) {  // a single element, as if the others of its word were masked
+    const float x = to_f<T>(rw.x[rw.end_at(tid)]);
+    const float m = max_nan(st.m, x), m0 = m == -CUDART_INF_F ? 0.f : m;
+    const float delta = max_nan((st.m - m0) * bl2, -200.f), e = ex2(delta);
+    const float d = max_nan((x - m0) * bl2, -200.f), z = ex2(d);
+    st.a = make_float2(fmaf(z, d, fmaf(delta, st.s.x, st.a.x) * e), fmaf(delta, st.s.y, st.a.y) * e);
+    st.s = make_float2(fmaf(st.s.x, e, z), st.s.y * e);
+    st.m = m;
   }
   // largest key this thread saw; 0 if it saw nothing
-  const bool saw = tid < ends || v0 + tid < v1;
-  const unsigned my_key = saw ? key_of(p.m) : 0u;
-  keys[tid] = my_key;
-  p = warp_merge(p, bl2);
-  if (lane == 0) warp_part[warp] = p;
-  if (tid == 0) count = 0;
-  __syncthreads();
-  if (warp == 0) {
-    Part q{-CUDART_INF_F, 0.f, 0.f};
-    if (lane < WARPS) q = warp_part[lane];
-    q = warp_merge(q, bl2);
-    if (lane == 0) warp_part[0] = q;
-    if (top > 0) {  // a lower bound of the top-th largest of the threads' maxima, exact in its leading bits
-      unsigned k[PER];
-#pragma unroll
-      for (int j = 0; j < PER; ++j) k[j] = keys[lane + 32 * j];
-      unsigned tau = 0;
-      constexpr int LOW = sizeof(T) == 2 ? 13 : 8;
-      for (int b = 31; b >= LOW; --b) {
-        const unsigned c = tau | 1u << b;
-        unsigned n = 0;
-#pragma unroll
-        for (int j = 0; j < PER; ++j) n += k[j] >= c;
-        if (__reduce_add_sync(FULL, n) >= (unsigned)top) tau = c;
-      }
-      if (lane == 0) tau_s = max(tau, 1u);
-    }
+  const unsigned my_key = tid < ends || tid < nv ? key_of(st.m) : 0u;
+  const unsigned wk = __reduce_max_sync(FULL, my_key);
+  if (lane == 0) warp_key[warp] = wk;
+  if (top > 0) {
+    // A lower bound of the top-th largest element: the warps whose lanes all hold elements have, between them, `top`
+    // lanes whose maxima reach the smallest of the warps' r-th largest, r = top / warps.
+    const int full = min(WARPS, nv >> 5);
+    const int r = full ? (top + full - 1) / full : 33;
+    unsigned rth = 0;
+    if (r <= 32) rth = warp_rth(my_key, r);
+    if (lane == 0) warp_tau[warp] = warp < full ? rth : r <= 32 ? 0xffffffffu : 0u;
   }
   __syncthreads();
-  p = warp_part[0];
-  int mine = 0;  // how many of the row's best this block has to offer, in best[]
-  if (top > 0) {
-    const int64_t have = (v1 - v0) * VEC + ends;
-    mine = (int)min((int64_t)top, have);
-    unsigned tau = tau_s;
-    bool strict = false, ties = false;
-    for (;;) {
-      // offer: elements with key >= tau (strict: > tau); whole warps read the elements of one thread after another
-      const u64 floor_key = (u64)tau + (strict ? 1 : 0);
-      unsigned holders = __ballot_sync(FULL, my_key >= floor_key);
-      while (holders) {
-        const int owner = warp * 32 + __ffs(holders) - 1;
-        holders &= holders - 1;
-        auto offer = [&](float x, int64_t at) {
-          const unsigned k = key_of(x);
-          if (k >= floor_key) {
-            const unsigned slot = atomicAdd(&count, 1u);
-            if (slot < LP_CAND) cand[slot] = cand_of(k, (unsigned)at);
-          }
-        };
-        if (lane == 0 && owner < ends) offer(to_f<T>(rw.x[rw.end_at(owner)]), rw.end_at(owner));
-        for (int64_t v = v0 + owner + (int64_t)lane * THREADS; v < v1; v += 32 * THREADS) {
-          const Pack<T, VEC> w = load_pack<T, VEC>(rw.x + rw.vec_at(v));
+  unsigned block_key = 0, tau = 0xffffffffu;
 #pragma unroll
-          for (int k = 0; k < VEC; ++k) offer(to_f<T>(w.e[k]), rw.vec_at(v) + k);
+  for (int w = 0; w < WARPS; ++w) {
+    block_key = max(block_key, warp_key[w]);
+    if (top > 0) tau = min(tau, warp_tau[w]);
+  }
+  tau = max(tau, 1u);
+  // The sums relative to the block's maximum, without the largest element's own 1: its thread (the first of the first
+  // warp that holds it) leaves its sum out, and its warp reads that thread's elements again.
+  const float M = value_of(block_key), M0 = M == -CUDART_INF_F ? 0.f : M;
+  float r_sum, a_sum;
+  {
+    const float delta = max_nan((st.m - M0) * bl2, -200.f), e = ex2(delta), s = st.s.x + st.s.y;
+    r_sum = s * e;
+    a_sum = fmaf(delta, s, st.a.x + st.a.y) * e;
+  }
+  bool first = wk == block_key && block_key != 0u && M < CUDART_INF_F && M > -CUDART_INF_F;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w)
+    if (w < warp && warp_key[w] == block_key) first = false;
+  if (first) {
+    const int owner_lane = __ffs(__ballot_sync(FULL, my_key == block_key)) - 1, owner = warp * 32 + owner_lane;
+    if (lane == owner_lane) r_sum = 0.f;
+    bool taken = false;  // the largest element itself has been left out
+    if (owner < ends) {
+      const float x = to_f<T>(rw.x[rw.end_at(owner)]);
+      taken = x == M;
+      if (!taken && lane == 0) r_sum += ex2(max_nan((x - M0) * bl2, -200.f));
+    }
+    for (int base = owner; base < nv; base += 32 * THREADS) {
+      const int v = base + lane * THREADS;
+      uint4 q = make_uint4(0, 0, 0, 0);
+      const bool live = v < nv;
+      if (live) q = vecs[v];
+      bool has = false;
+#pragma unroll
+      for (int k = 0; k < VEC / 2; ++k) {
+        const float2 x = pair_of<T>(q, k);
+        has = has || (live && (x.x == M || x.y == M));
+      }
+      const unsigned who = __ballot_sync(FULL, has);
+      bool skip = !taken && who && lane == __ffs(who) - 1;
+      taken = taken || who;
+      if (live) {
+#pragma unroll
+        for (int k = 0; k < VEC / 2; ++k) {
+          const float2 x = pair_of<T>(q, k), d = exponents(x, -M0, bl2);
+          if (skip && x.x == M)
+            skip = false;
+          else
+            r_sum += ex2(d.x);
+          if (skip && x.y == M)
+            skip = false;
+          else
+            r_sum += ex2(d.y);
+        }
+      }
+    }
+  }
+  r_sum = warp_sum(r_sum);
+  a_sum = warp_sum(a_sum);
+  if (lane == 0) warp_sum2[warp] = make_float2(r_sum, a_sum);
+  int mine = 0;  // how many of the row's best this block has to offer
+  unsigned n_cand = 0;
+  bool ties = false;
+  if (top > 0) {
+    mine = (int)min((int64_t)top, (int64_t)nv * VEC + ends);
+    for (bool strict = false;;) {
+      // offer: elements with key >= tau (strict: > tau).  The threads that hold any are listed; their words are dealt to the
+      // warp's lanes.
+      const u64 floor_key = (u64)tau + (strict ? 1 : 0);
+      const unsigned holds = __ballot_sync(FULL, my_key >= floor_key);
+      const int n_hold = __popc(holds);
+      if (holds >> lane & 1) holder[warp * 32 + __popc(holds & ((1u << lane) - 1))] = (unsigned short)tid;
+      __syncwarp();
+      auto offer = [&](float x, int64_t at) {
+        const unsigned k = key_of(x);
+        if (k >= floor_key) {
+          const unsigned slot = atomicAdd(&count, 1u);
+          if (slot < LP_CAND) cand[slot] = cand_of(k, (unsigned)at);
+        }
+      };
+      if (tid < ends) offer(to_f<T>(rw.x[rw.end_at(tid)]), rw.end_at(tid));
+      const int iters = (nv + THREADS - 1) / THREADS;
+      for (int w = lane; w < n_hold * iters; w += 32) {
+        const int h = w / iters, v = holder[warp * 32 + h] + (w - h * iters) * THREADS;
+        if (v < nv) {
+          const uint4 q = vecs[v];
+#pragma unroll
+          for (int k = 0; k < VEC / 2; ++k) {
+            const float2 x = pair_of<T>(q, k);
+            const int64_t at = rw.vec_at(v0 + v) + 2 * k;
+            offer(x.x, at);
+            offer(x.y, at + 1);
+          }
         }
       }
       __syncthreads();
-      const unsigned n = count;
-      __syncthreads();
-      if (n <= LP_CAND) {
+      n_cand = count;
+      if (n_cand <= LP_CAND) {
         // ties at tau that did not fit are taken below in the order of their indices
-        ties = strict && n < (unsigned)mine;
+        ties = strict && n_cand < (unsigned)mine;
         break;
       }
+      __syncthreads();
       if (tid == 0) count = 0;
-      if (!strict) {
-        strict = true;
-      } else {  // more than fit lie above tau: the top-th largest of those held is a higher bound
+      if (strict) {  // more than fit lie above tau: the top-th largest of those held is a higher bound
         for (int c = tid; c < LP_CAND; c += THREADS) {
           const u64 me = cand[c];
           int above = 0;
           for (int j = 0; j < LP_CAND; ++j) above += cand[j] > me;
           if (above == mine - 1) tau_s = (unsigned)(me >> 32);
         }
-        strict = false;
       }
       __syncthreads();
-      tau = tau_s;
+      if (strict) tau = tau_s;
+      strict = !strict;
     }
-    const int n = (int)count;
-    for (int c = tid; c < n; c += THREADS) {
-      const u64 me = cand[c];
-      int above = 0;
-      for (int j = 0; j < n; ++j) above += cand[j] > me;
-      if (above < mine) best[above] = me;
+    if (ties || parts > 1) {
+      for (int c = tid; c < (int)n_cand; c += THREADS) {
+        const u64 me = cand[c];
+        int above = 0;
+        for (int j = 0; j < (int)n_cand; ++j) above += cand[j] > me;
+        if (above < mine) best[above] = me;
+      }
     }
     if (ties) {  // the first elements equal to tau, by index: the single ones at the front, the vectors', those at the end
-      int got = n;
-      const int64_t lo = rank == 0 ? 0 : rw.vec_at(v0), hi = rw.vec_at(v1);
+      int got = (int)n_cand;
+      const int64_t lo = rank == 0 ? 0 : rw.vec_at(v0), hi = rw.vec_at(v0 + nv);
       for (int phase = 0; phase < 2 && got < mine; ++phase) {
         const int64_t from = phase == 0 ? lo : rw.nvec * VEC + rw.head, to = phase == 0 ? hi : (rank == 0 ? V : 0);
         for (int64_t base = from; base < to && got < mine; base += THREADS) {
@@ -360,8 +463,17 @@ __global__ void __launch_bounds__(THREADS)
         }
       }
     }
+    if (ties || parts > 1) __syncthreads();
+  } else {
     __syncthreads();
   }
+  Part p{M, 0.f, 0.f};
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) {
+    p.r += warp_sum2[w].x;
+    p.a += warp_sum2[w].y;
+  }
+  if (!(M < CUDART_INF_F)) p.r = CUDART_NAN_F;
   if (parts > 1) {  // everything to the cluster's first block
     cluster.barrier_wait();  // the first block runs: its shared memory may be written
     if (tid == 0) cluster.map_shared_rank(all_part, 0)[rank] = p;
@@ -385,94 +497,128 @@ __global__ void __launch_bounds__(THREADS)
   }
   const RowScalars s = finish(p);
   if (tid == 0) write_row(out, row, p, s, xt, t, V, beta);
-  for (int c = tid; c < top; c += THREADS) {
-    const u64 me = best[c];
-    out.top_ids[row * top + c] = (int32_t)~(unsigned)me;
-    out.top_lp[row * top + c] = log_p(s, value_of((unsigned)(me >> 32)), beta);
+  auto write_top = [&](int place, u64 me) {
+    out.top_ids[row * top + place] = (int32_t)~(unsigned)me;
+    out.top_lp[row * top + place] = log_p(s, value_of((unsigned)(me >> 32)), beta);
+  };
+  if (ties || parts > 1) {
+    for (int c = tid; c < top; c += THREADS) write_top(c, best[c]);
+  } else {
+    for (int c = tid; c < (int)n_cand; c += THREADS) {
+      const u64 me = cand[c];
+      int above = 0;
+      for (int j = 0; j < (int)n_cand; ++j) above += cand[j] > me;
+      if (above < top) write_top(above, me);
+    }
   }
 }
 
 // ---- forward, one warp per row ----------------------------------------------------------------------
+// The row stays in registers, element lane + 32 e in x[e].  The top-th largest key is found bit by bit with warp
+// counts; what lies above it, and as many elements equal to it as are needed in the order of their indices, are the
+// candidates, exactly `top` of them.
 template <typename T, int E>  // V <= 32 * E
 __global__ void __launch_bounds__(128)
     k_log_probs_warp(const T* __restrict__ logits, int64_t xs, int64_t rows, int V, const void* __restrict__ targets, int t64,
                      float beta, int top, RowOut out) {
+  __shared__ u64 cand_all[4][LP_MAX_TOP];
   const int lane = threadIdx.x & 31;
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   if (row >= rows) return;
+  u64* cand = cand_all[threadIdx.x >> 5];
   const T* xr = logits + row * xs;
   const float bl2 = beta * LOG2E;
   const long long t = target_of(targets, t64, row);
   const float xt = value_at(xr, V, t);
   float x[E];
-  float m = -CUDART_INF_F, bad = 0.f;
-  unsigned big = 0;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int c = lane + 32 * e;
     x[e] = c < V ? to_f<T>(xr[c]) : -CUDART_INF_F;
+  }
+  float m = -CUDART_INF_F, bad = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
     m = fmaxf(m, x[e]);
     if (!(x[e] < CUDART_INF_F)) bad = CUDART_NAN_F;
-    if (c < V) big = max(big, key_of(x[e]));
   }
   float wm = m;
 #pragma unroll
   for (int o = 16; o; o >>= 1) wm = fmaxf(wm, __shfl_xor_sync(FULL, wm, o));
   // the first element equal to the maximum stays out of the sum
-  const unsigned at_max = __ballot_sync(FULL, m == wm);
-  bool own = lane == __ffs(at_max) - 1;
+  bool own = lane == __ffs(__ballot_sync(FULL, m == wm)) - 1;
   Part p{wm, bad, 0.f};
   if (wm != -CUDART_INF_F) {
 #pragma unroll
     for (int e = 0; e < E; ++e) {
+      const float d = max_nan((x[e] - wm) * bl2, -200.f);
+      float z = ex2(d);
       if (own && x[e] == wm) {
         own = false;
-      } else {
-        const float d = max_nan((x[e] - wm) * bl2, -200.f), z = ex2(d);
-        p.r += z;
-        p.a = fmaf(z, d, p.a);
+        z = 0.f;
       }
+      p.r += z;
+      p.a = fmaf(z, d, p.a);
     }
   }
   p.r = warp_sum(p.r);
   p.a = warp_sum(p.a);
   const RowScalars s = finish(p);
   if (lane == 0) write_row(out, row, p, s, xt, t, V, beta);
-  // the best `top`: each lane holds its best not yet taken
-  unsigned taken = 0;
-  for (int k = 0; k < top; ++k) {
-    const unsigned best = __reduce_max_sync(FULL, big);
-    int where = 0x7fffffff;
-    if (big == best) {
+  if (top == 0) return;
+  unsigned key[E];
 #pragma unroll
-      for (int e = E - 1; e >= 0; --e)
-        if (!(taken >> e & 1) && lane + 32 * e < V && key_of(x[e]) == best) where = lane + 32 * e;
-    }
-    const int at = __reduce_min_sync(FULL, where);
-    if (lane == 0) {
-      out.top_ids[row * top + k] = at;
-      out.top_lp[row * top + k] = log_p(s, value_of(best), beta);
-    }
-    if (at == where) {
-      taken |= 1u << (at >> 5);
-      big = 0;
+  for (int e = 0; e < E; ++e) key[e] = lane + 32 * e < V ? key_of(x[e]) : 0u;
+  unsigned tau = 0;
+  for (int b = 31; b >= 0; --b) {
+    const unsigned c = tau | 1u << b;
+    unsigned n = 0;
 #pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (!(taken >> e & 1) && lane + 32 * e < V) big = max(big, key_of(x[e]));
-    }
+    for (int e = 0; e < E; ++e) n += key[e] >= c;
+    n = __reduce_add_sync(FULL, n);
+    if (n >= (unsigned)top) tau = c;
+    if (n == (unsigned)top) break;  // exactly these
+  }
+  const unsigned below = (1u << lane) - 1;
+  int n = 0;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const bool take = key[e] > tau;
+    const unsigned v = __ballot_sync(FULL, take);
+    if (take) cand[n + __popc(v & below)] = cand_of(key[e], (unsigned)(lane + 32 * e));
+    n += __popc(v);
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const bool take = key[e] == tau;
+    const unsigned v = __ballot_sync(FULL, take);
+    const int slot = n + __popc(v & below);
+    if (take && slot < top) cand[slot] = cand_of(key[e], (unsigned)(lane + 32 * e));
+    n += __popc(v);
+  }
+  __syncwarp();
+  for (int c = lane; c < top; c += 32) {
+    const u64 me = cand[c];
+    int above = 0;
+    for (int j = 0; j < top; ++j) above += cand[j] > me;
+    out.top_ids[row * top + above] = (int32_t)~(unsigned)me;
+    out.top_lp[row * top + above] = log_p(s, value_of((unsigned)(me >> 32)), beta);
   }
 }
 
 // ---- backward ---------------------------------------------------------------------------------------
 struct GradRow {
-  float m, log_z, h, g, gh, beta;
-  bool empty;
+  float m, log_z, h, g, gh, beta, bl2, lz2, c0, c1;
+  bool empty;  // nothing but -inf: no gradient
 };
-// every element but the token's own
-__device__ __forceinline__ float grad_of(const GradRow& r, float x) {
-  if (r.empty) return 0.f;
-  const float lp = max_nan(fmaf(r.beta, x - r.m, -r.log_z), -200.f);  // below exp(-87) p is 0 and lp stays finite
-  return r.beta * -ex2(lp * LOG2E) * fmaf(r.gh, lp + r.h, r.g);
+// Every element but the token's own, two at a time, in powers of two: l = log2 p, d = p (c0 + c1 l) with
+// c0 = -beta (g + g_H H) and c1 = -beta g_H log(2).  Below 2^-200 p is 0 and l stays finite.
+__device__ __forceinline__ float2 grad_of(const GradRow& r, float2 x) {
+  float2 l = fma2(add2(x, make_float2(-r.m, -r.m)), make_float2(r.bl2, r.bl2), make_float2(-r.lz2, -r.lz2));
+  l.x = max_nan(l.x, -200.f);
+  l.y = max_nan(l.y, -200.f);
+  const float2 p = make_float2(ex2(l.x), ex2(l.y));
+  return mul2(p, fma2(make_float2(r.c1, r.c1), l, make_float2(r.c0, r.c0)));
 }
 // the token's: 1 - p by expm1, which keeps its digits where p is nearly 1
 __device__ __forceinline__ float grad_at_token(const GradRow& r, float x) {
@@ -490,6 +636,11 @@ __device__ __forceinline__ GradRow grad_row(int64_t row, long long t, int64_t V,
   r.gh = gh ? gh[row] : 0.f;
   r.beta = beta;
   r.empty = r.log_z == -CUDART_INF_F;
+  r.bl2 = beta * LOG2E;
+  r.lz2 = r.empty ? 0.f : r.log_z * LOG2E;
+  if (r.empty) r.m = 0.f;
+  r.c0 = r.empty ? 0.f : -beta * fmaf(r.gh, r.h, r.g);
+  r.c1 = r.empty ? 0.f : -beta * r.gh * LN2;
   return r;
 }
 // A block takes `chunk` columns of one row; the vectors are aligned to the gradient, which is dense.
@@ -511,7 +662,7 @@ __global__ void __launch_bounds__(256)
   if (part == 0 && (int)threadIdx.x < rw.ends) {
     const int64_t at = rw.end_at(threadIdx.x);
     const float x = to_f<T>(xr[at]);
-    dr[at] = from_f<T>(at == t ? grad_at_token(r, x) : grad_of(r, x));
+    dr[at] = from_f<T>(at == t ? grad_at_token(r, x) : grad_of(r, make_float2(x, x)).x);
   }
   for (int64_t i0 = v0 + threadIdx.x; i0 < v1; i0 += U * 256) {
     Pack<T, VEC> w[U];
@@ -536,7 +687,11 @@ __global__ void __launch_bounds__(256)
         const int64_t ahead = t - at;
         Pack<T, VEC> o;
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) o.e[k] = from_f<T>(grad_of(r, to_f<T>(w[u].e[k])));
+        for (int k = 0; k < VEC; k += 2) {
+          const float2 d = grad_of(r, make_float2(to_f<T>(w[u].e[k]), to_f<T>(w[u].e[k + 1])));
+          o.e[k] = from_f<T>(d.x);
+          o.e[k + 1] = from_f<T>(d.y);
+        }
         if (ahead >= 0 && ahead < VEC) {
 #pragma unroll
           for (int k = 0; k < VEC; ++k)
@@ -560,7 +715,7 @@ __global__ void __launch_bounds__(128)
 #pragma unroll 4
   for (int c = threadIdx.x & 31; c < V; c += 32) {
     const float x = to_f<T>(logits[row * xs + c]);
-    dx[row * V + c] = from_f<T>(c == t ? grad_at_token(r, x) : grad_of(r, x));
+    dx[row * V + c] = from_f<T>(c == t ? grad_at_token(r, x) : grad_of(r, make_float2(x, x)).x);
   }
 }
 
@@ -621,7 +776,8 @@ int fv_token_log_probs(int device, void* stream, const void* logits, int64_t str
       // few rows: a cluster per row, as long as every block keeps two vectors a thread
       int parts = 1;
       while (parts < 8 && rows * parts * 2 <= 2 * sms && vocab / (parts * 2) >= 2 * 256 * Row<T>::VEC) parts *= 2;
-      e = launch_rows<T, 256>(parts, rows, st, x, stride, vocab, targets, targets_int64, beta, top, out);
+      e = vocab / Row<T>::VEC <= 1024 ? launch_rows<T, 128>(parts, rows, st, x, stride, vocab, targets, targets_int64, beta, top, out)
+                                      : launch_rows<T, 256>(parts, rows, st, x, stride, vocab, targets, targets_int64, beta, top, out);
     }
   });
   FV_CUDA(e);
