@@ -38,10 +38,22 @@ namespace fvo {
 namespace {
 
 // ---- activations ------------------------------------------------------------------------------------
+// The normal distribution function, Phi(z) = erfc(-z / sqrt(2)) / 2, by Abramowitz and Stegun's formula 7.1.26
+// (|error of erf| <= 1.5e-7, and it shrinks with exp(-z^2 / 2) for z < 0): two special-function calls and ten
+// multiplications instead of the forty operations of erfcf.
+__device__ __forceinline__ float normal_cdf(float z) {
+  const float x = fabsf(z) * 0.70710678f, t = __fdividef(1.0f, fmaf(0.3275911f, x, 1.0f));
+  float q = fmaf(1.061405429f, t, -1.453152027f);
+  q = fmaf(q, t, 1.421413741f);
+  q = fmaf(q, t, -0.284496736f);
+  q = fmaf(q, t, 0.254829592f);
+  q *= 0.5f * t * __expf(-x * x);
+  return z < 0.f ? q : 1.0f - q;
+}
 __device__ __forceinline__ float act_value(float z, int act) {
   switch (act) {
     case FV_ACT_RELU: return z < 0.f ? 0.f : z;  // keeps a NaN
-    case FV_ACT_GELU: return 0.5f * z * erfcf(-0.70710678f * z);  // erfc: no cancellation for z < 0
+    case FV_ACT_GELU: return z * normal_cdf(z);
     case FV_ACT_GELU_TANH: {
       const float u = 0.7978845608f * fmaf(0.044715f * z * z, z, z);
       return __fdividef(z, 1.0f + __expf(-2.0f * u));  // (1 + tanh u) / 2 = 1 / (1 + exp(-2 u))
@@ -53,7 +65,7 @@ __device__ __forceinline__ float act_value(float z, int act) {
 __device__ __forceinline__ float act_slope(float z, int act) {
   switch (act) {
     case FV_ACT_RELU: return z > 0.f ? 1.f : z <= 0.f ? 0.f : z;
-    case FV_ACT_GELU: return fmaf(z, 0.3989422804f * __expf(-0.5f * z * z), 0.5f * erfcf(-0.70710678f * z));
+    case FV_ACT_GELU: return fmaf(z, 0.3989422804f * __expf(-0.5f * z * z), normal_cdf(z));
     case FV_ACT_GELU_TANH: {
       if (fabsf(z) > 16.f) return z > 0.f ? 1.f : 0.f;  // to float's last bit; beyond, z * z may overflow
       const float z2 = z * z, u = 0.7978845608f * fmaf(0.044715f * z2, z, z);

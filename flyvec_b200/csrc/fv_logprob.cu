@@ -34,6 +34,9 @@ namespace {
 constexpr int LP_MAX_TOP = 64;
 constexpr int LP_CAND = 1024;      // candidates a block can hold at once
 constexpr int LP_SMALL = 1024;     // rows up to here: one warp
+constexpr int LP_THREADS = 256;    // largest block, and that of every cluster
+constexpr int LP_SLOTS = 16;       // batches of a thread whose maxima are kept apart
+constexpr int LP_LIST = 256;       // batches that can be listed for their candidates
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 
@@ -154,10 +157,11 @@ __device__ __forceinline__ float2 exponents(float2 x, float minus_m, float bl2) 
   d.y = max_nan(d.y, -200.f);
   return d;
 }
-// N words of elements: one rescaling for all of them, without a branch, then two elements per step.
+// N words of elements: one rescaling for all of them, without a branch, then two elements per step.  Returns their
+// maximum.
 template <typename T, int N>
-__device__ __forceinline__ void take(Stream& t, const uint4 (&q)[N], float bl2) {
-  const float m = max_nan(t.m, words_max<T, N>(q)), m0 = m == -CUDART_INF_F ? 0.f : m;
+__device__ __forceinline__ float take(Stream& t, const uint4 (&q)[N], float bl2) {
+  const float big = words_max<T, N>(q), m = max_nan(t.m, big), m0 = m == -CUDART_INF_F ? 0.f : m;
   const float delta = max_nan((t.m - m0) * bl2, -200.f), e = ex2(delta);
   const float2 e2 = make_float2(e, e);
   t.a = mul2(fma2(make_float2(delta, delta), t.s, t.a), e2);
@@ -171,6 +175,7 @@ __device__ __forceinline__ void take(Stream& t, const uint4 (&q)[N], float bl2) 
       t.s = add2(t.s, z);
       t.a = fma2(z, d, t.a);
     }
+  return big;
 }
 
 struct RowOut {
@@ -241,7 +246,7 @@ __device__ __forceinline__ unsigned warp_rth(unsigned key, int r) {
 }
 
 template <typename T, int THREADS>
-__global__ void __launch_bounds__(THREADS, 1024 / THREADS)
+__global__ void __launch_bounds__(THREADS, 1280 / THREADS)
     k_log_probs(const T* __restrict__ logits, int64_t xs, int64_t V, const void* __restrict__ targets, int t64, float beta, int top,
                 int parts, RowOut out) {
   constexpr int VEC = Row<T>::VEC, WARPS = THREADS / 32;
@@ -250,9 +255,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
   __shared__ Part all_part[8];
   __shared__ u64 cand[LP_CAND];
   __shared__ u64 best[LP_MAX_TOP];
-  __shared__ u64 gathered[8 * LP_MAX_TOP];
-  __shared__ unsigned short holder[THREADS];
-  __shared__ unsigned count, tau_s, warp_n[WARPS];
+  __shared__ u64 gathered[THREADS == LP_THREADS ? 8 * LP_MAX_TOP : 1];  // clusters have blocks of LP_THREADS
+  __shared__ float slot_max[LP_SLOTS][THREADS];
+  __shared__ unsigned short listed[LP_LIST];
+  __shared__ unsigned count, n_listed, tau_s, warp_n[WARPS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t row = parts == 1 ? (int64_t)blockIdx.x : blockIdx.x / parts;
   const int rank = (int)(blockIdx.x - row * parts);
@@ -268,7 +274,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
   long long t = -1;
   float xt = 0.f;
   if (tid == 0) {
-    count = 0;
+    count = n_listed = 0;
     if (rank == 0) {
       t = target_of(targets, t64, row);
       xt = value_at(rw.x, V, t);
@@ -276,19 +282,27 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
   }
   Stream st{-CUDART_INF_F, make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
   constexpr int U = 4;  // loads in flight per thread
-  int i = tid;
+  int i = tid, batch = 0;
+  // the largest element of each batch of U words, for finding the candidates again
+  auto note = [&](float big) {
+    if (top > 0) {
+      float* at = &slot_max[batch % LP_SLOTS][tid];
+      *at = batch < LP_SLOTS ? big : max_nan(*at, big);
+      ++batch;
+    }
+  };
   for (; i + (U - 1) * THREADS < nv; i += U * THREADS) {
     uint4 q[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) q[u] = vecs[i + u * THREADS];
-    take<T, U>(st, q, bl2);
+    note(take<T, U>(st, q, bl2));
   }
-  {
-    uint4 q[1];
-    for (; i < nv; i += THREADS) {
-      q[0] = vecs[i];
-      take<T, 1>(st, q, bl2);
-    }
+  if (i < nv) {  // the last words together; what is missing reads as masked
+    uint4 q[U - 1];
+    const unsigned none = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+#pragma unroll
+    for (int u = 0; u < U - 1; ++u) q[u] = i + u * THREADS < nv ? vecs[i + u * THREADS] : make_uint4(none, none, none, none);
+    note(take<T, U - 1>(st, q, bl2));
   }
   if (tid < ends) {  // a single element, as if the others of its word were masked
     const float x = to_f<T>(rw.x[rw.end_at(tid)]);
@@ -310,7 +324,11 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
     const int r = full ? (top + full - 1) / full : 33;
     unsigned rth = 0;
     if (r <= 32) rth = warp_rth(my_key, r);
-    if (lane == 0) warp_tau[warp] = warp < full ? rth : r <= 32 ? 0xffffffffu : 0u;
+    const bool many = __popc(__ballot_sync(FULL, my_key == rth)) > 16;
+    if (lane == 0) {
+      warp_tau[warp] = warp < full ? rth : r <= 32 ? 0xffffffffu : 0u;
+      warp_n[warp] = many;
+    }
   }
   __syncthreads();
   unsigned block_key = 0, tau = 0xffffffffu;
@@ -318,6 +336,13 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
   for (int w = 0; w < WARPS; ++w) {
     block_key = max(block_key, warp_key[w]);
     if (top > 0) tau = min(tau, warp_tau[w]);
+  }
+  // Half a warp's maxima equal to the bound: a masked or constant row.  Only what lies above it is offered then, and
+  // its equals are taken in the order of their indices.
+  bool strict = false;
+  if (top > 0) {
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) strict = strict || (warp_tau[w] == tau && warp_n[w]);
   }
   tau = max(tau, 1u);
   // The sums relative to the block's maximum, without the largest element's own 1: its thread (the first of the first
@@ -380,14 +405,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
   bool ties = false;
   if (top > 0) {
     mine = (int)min((int64_t)top, (int64_t)nv * VEC + ends);
-    for (bool strict = false;;) {
-      // offer: elements with key >= tau (strict: > tau).  The threads that hold any are listed; their words are dealt to the
-      // warp's lanes.
+    for (bool again = false;; again = true) {
+      // offer: elements with key >= tau (strict: > tau)
       const u64 floor_key = (u64)tau + (strict ? 1 : 0);
-      const unsigned holds = __ballot_sync(FULL, my_key >= floor_key);
-      const int n_hold = __popc(holds);
-      if (holds >> lane & 1) holder[warp * 32 + __popc(holds & ((1u << lane) - 1))] = (unsigned short)tid;
-      __syncwarp();
+      const float floor_value = value_of(tau);
       auto offer = [&](float x, int64_t at) {
         const unsigned k = key_of(x);
         if (k >= floor_key) {
@@ -395,23 +416,51 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
           if (slot < LP_CAND) cand[slot] = cand_of(k, (unsigned)at);
         }
       };
-      if (tid < ends) offer(to_f<T>(rw.x[rw.end_at(tid)]), rw.end_at(tid));
-      const int iters = (nv + THREADS - 1) / THREADS;
-      for (int w = lane; w < n_hold * iters; w += 32) {
-        const int h = w / iters, v = holder[warp * 32 + h] + (w - h * iters) * THREADS;
-        if (v < nv) {
-          const uint4 q = vecs[v];
+      auto offer_word = [&](int v) {
+        const uint4 one[1] = {vecs[v]};
+        if (words_max<T, 1>(one) < floor_value) return;
+        unsigned hits = 0;
 #pragma unroll
-          for (int k = 0; k < VEC / 2; ++k) {
-            const float2 x = pair_of<T>(q, k);
-            const int64_t at = rw.vec_at(v0 + v) + 2 * k;
-            offer(x.x, at);
-            offer(x.y, at + 1);
+        for (int k = 0; k < VEC / 2; ++k) {
+          const float2 x = pair_of<T>(one[0], k);
+          hits |= (x.x < floor_value ? 0u : 1u << 2 * k) | (x.y < floor_value ? 0u : 2u << 2 * k);
+        }
+        for (; hits; hits &= hits - 1) {
+          const int k = __ffs(hits) - 1;
+          offer(to_f<T>(reinterpret_cast<const T*>(vecs + v)[k]), rw.vec_at(v0 + v) + k);
+        }
+      };
+      if (tid < ends) offer(to_f<T>(rw.x[rw.end_at(tid)]), rw.end_at(tid));
+      if (!again) {
+        // the batches that reach the bound are listed, then their words are dealt to all threads
+        if (my_key >= floor_key) {
+          for (int b = 0; b < min(batch, LP_SLOTS); ++b)
+            if (key_of(slot_max[b][tid]) >= floor_key) {
+              const unsigned place = atomicAdd(&n_listed, 1u);
+              if (place < LP_LIST) listed[place] = (unsigned short)(tid * LP_SLOTS + b);
+            }
+        }
+        __syncthreads();
+        const int n = (int)n_listed;
+        if (n <= LP_LIST) {
+          for (int w = tid; w < n * U; w += THREADS) {
+            const int e = listed[w / U];
+            for (int v = e / LP_SLOTS + (e % LP_SLOTS * U + w % U) * THREADS; v < nv; v += LP_SLOTS * U * THREADS) offer_word(v);
           }
         }
+      } else {
+        unsigned holds = __ballot_sync(FULL, my_key >= floor_key);
+        for (; holds; holds &= holds - 1)
+          for (int v = warp * 32 + __ffs(holds) - 1 + lane * THREADS; v < nv; v += 32 * THREADS) offer_word(v);
       }
       __syncthreads();
       n_cand = count;
+      if (!again && n_listed > LP_LIST) {  // not all were listed: again, all words of the threads that reach the bound
+        __syncthreads();
+        if (tid == 0) count = 0;
+        __syncthreads();
+        continue;
+      }
       if (n_cand <= LP_CAND) {
         // ties at tau that did not fit are taken below in the order of their indices
         ties = strict && n_cand < (unsigned)mine;
@@ -489,12 +538,22 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
       const u64 me = gathered[(c / top) * LP_MAX_TOP + c % top];
       if (!me) continue;
       int above = 0;
-      for (int k = 0; k < parts; ++k)
-        for (int j = 0; j < top; ++j) above += gathered[k * LP_MAX_TOP + j] > me;
+      for (int k = 0; k < parts; ++k) {  // how many of list k are larger: halving
+        int lo = 0, hi = top;
+        while (lo < hi) {
+          const int mid = (lo + hi) >> 1;
+          if (gathered[k * LP_MAX_TOP + mid] > me)
+            lo = mid + 1;
+          else
+            hi = mid;
+        }
+        above += lo;
+      }
       if (above < top) best[above] = me;
     }
     __syncthreads();
   }
+  if (tid != 0 && tid >= (ties || parts > 1 ? top : (int)n_cand)) return;
   const RowScalars s = finish(p);
   if (tid == 0) write_row(out, row, p, s, xt, t, V, beta);
   auto write_top = [&](int place, u64 me) {
@@ -776,8 +835,11 @@ int fv_token_log_probs(int device, void* stream, const void* logits, int64_t str
       // few rows: a cluster per row, as long as every block keeps two vectors a thread
       int parts = 1;
       while (parts < 8 && rows * parts * 2 <= 2 * sms && vocab / (parts * 2) >= 2 * 256 * Row<T>::VEC) parts *= 2;
-      e = vocab / Row<T>::VEC <= 1024 ? launch_rows<T, 128>(parts, rows, st, x, stride, vocab, targets, targets_int64, beta, top, out)
-                                      : launch_rows<T, 256>(parts, rows, st, x, stride, vocab, targets, targets_int64, beta, top, out);
+      // a warp's share of the fixed work per row (reductions, candidates) weighs more the shorter the row
+      const int64_t words = vocab / Row<T>::VEC;
+      e = parts > 1 || words > 4096      ? launch_rows<T, LP_THREADS>(parts, rows, st, x, stride, vocab, targets, targets_int64, beta, top, out)
+          : words <= 512 && top <= 16 ? launch_rows<T, 64>(1, rows, st, x, stride, vocab, targets, targets_int64, beta, top, out)
+                                      : launch_rows<T, 128>(1, rows, st, x, stride, vocab, targets, targets_int64, beta, top, out);
     }
   });
   FV_CUDA(e);
