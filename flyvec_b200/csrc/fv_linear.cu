@@ -120,8 +120,32 @@ __device__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* stop) {
     }
   }
 }
+// One thread of a converged warp, in a form that the compiler knows to be one thread: the loads and products below
+// take their operands from uniform registers, and under a plain lane == 0 each would be wrapped in a loop over lanes
+// (0.285 against 0.199 us per k-block).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
+}
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, uint32_t rank) {
+  uint32_t far;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(far) : "r"(addr), "r"(rank));
+  return far;
+}
+__device__ __forceinline__ void mbar_arrive_far(uint32_t far) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(far) : "memory");
+}
+// PAIR: the copy lands in this block and reports to a barrier of either block of the pair
+template <bool PAIR>
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-  asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+  if constexpr (PAIR)
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];" ::"r"(
+                     dst),
+                 "l"(map), "r"(x), "r"(y), "r"(bar)
+                 : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
                "l"(map), "r"(x), "r"(y), "r"(bar)
                : "memory");
 }
@@ -130,16 +154,32 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead, uint
   return (uint64_t)((addr & 0x3ffff) >> 4) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(stride >> 4) << 32 | (uint64_t)1 << 46 |
          (uint64_t)2 << 61;
 }
+template <bool PAIR>
 __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
-      : "memory");
+  if constexpr (PAIR)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+        : "memory");
 }
+// arrives at `bar` (of both blocks of a pair) when the products issued so far are done
+template <bool PAIR>
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  if constexpr (PAIR)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+                 "h"((uint16_t)3)
+                 : "memory");
+  else
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -176,7 +216,7 @@ constexpr int RING_BYTES = 192 << 10;            // operand ring
 constexpr int EPI_WARPS = 8;
 constexpr int GEMM_THREADS = 64 + 32 * EPI_WARPS;
 constexpr int STAGE_OUT = 32 * 128;              // an epilogue warp's staging: 32 rows of 128 bytes
-constexpr int GEMM_SMEM = 1024 + RING_BYTES + EPI_WARPS * STAGE_OUT + 256;
+constexpr int GEMM_SMEM = 1024 + RING_BYTES + EPI_WARPS * (STAGE_OUT + 128) + 256;  // + 32 floats of bias a warp
 
 struct GemmParams {
   int64_t m, n;        // rows of A, rows of B
@@ -243,26 +283,30 @@ __device__ __forceinline__ void stage_out(const uint8_t* stage, void* out, int64
       }
   }
 }
-// 32 x 32 16-bit elements of an array into the staging rows; what lies outside reads as 0.
-__device__ __forceinline__ void stage_in(uint8_t* stage, const void* in, int64_t ld, bool vec, int64_t r0, int64_t c0, int64_t rows,
+// 32 x 32 16-bit elements of an array: fetched early into registers (four 16-byte words a lane; rows that do not admit
+// them are fetched late, element by element), then put into the staging rows.  What lies outside reads as 0.
+__device__ __forceinline__ void fetch_in(uint4 (&w)[4], const void* in, int64_t ld, bool vec, int64_t r0, int64_t c0, int64_t rows,
                                          int64_t cols) {
   const int lane = threadIdx.x & 31;
-  const uint8_t* base = static_cast<const uint8_t*>(in);
+  if (!vec || c0 + 32 > cols) return;
+  const uint8_t* base = static_cast<const uint8_t*>(in) + ((r0 + lane / 4) * ld + c0) * 2 + (lane & 3) * 16;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    w[k] = make_uint4(0, 0, 0, 0);
+    if (r0 + lane / 4 + 8 * k < rows) w[k] = __ldcs(reinterpret_cast<const uint4*>(base + 16 * k * ld));
+  }
+}
+__device__ __forceinline__ void stage_in(uint8_t* stage, const uint4 (&w)[4], const void* in, int64_t ld, bool vec, int64_t r0, int64_t c0,
+                                         int64_t rows, int64_t cols) {
+  const int lane = threadIdx.x & 31;
   if (vec && c0 + 32 <= cols) {
-    const int c = lane & 3;
-    uint4 w[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int r = lane / 4 + 8 * k;
-      w[k] = make_uint4(0, 0, 0, 0);
-      if (r0 + r < rows) w[k] = __ldg(reinterpret_cast<const uint4*>(base + ((r0 + r) * ld + c0) * 2 + c * 16));
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int r = lane / 4 + 8 * k;
-      *reinterpret_cast<uint4*>(stage + r * 128 + ((c ^ (r & 7)) << 4)) = w[k];
+      *reinterpret_cast<uint4*>(stage + r * 128 + (((lane & 3) ^ (r & 7)) << 4)) = w[k];
     }
   } else {
+    const uint8_t* base = static_cast<const uint8_t*>(in);
 #pragma unroll 8
     for (int r = 0; r < 32; ++r) {
       uint16_t v = 0;
@@ -283,15 +327,20 @@ __device__ __forceinline__ void store_one(const GemmParams& p, int64_t r, int64_
     static_cast<T*>(p.y)[r * p.ldy + c] = from_f<T>(v);
 }
 
-template <typename T, int BN>
+// PAIR: two neighbouring blocks (a cluster) work on one 256 x BN tile: each loads its 128 rows of A and half of B's rows, the
+// first one's thread issues the products of both (they read both blocks' shared memory), and each takes its own 128 rows of
+// the accumulator through the epilogue.
+template <typename T, int BN, bool PAIR>
 __global__ void __launch_bounds__(GEMM_THREADS, 1)
     k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ GemmParams p) {
-  constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2, STAGE = A_BYTES + B_BYTES, STAGES = RING_BYTES / STAGE;
+  constexpr int BROWS = PAIR ? BN / 2 : BN;  // rows of B this block loads
+  constexpr int A_BYTES = BM * BK * 2, B_BYTES = BROWS * BK * 2, STAGE = A_BYTES + B_BYTES, STAGES = RING_BYTES / STAGE;
   constexpr int TMEM_COLS = 2 * BN;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* staging = smem + RING_BYTES;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(staging + EPI_WARPS * STAGE_OUT);
+  float* bias_slices = reinterpret_cast<float*>(staging + EPI_WARPS * STAGE_OUT);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(staging + EPI_WARPS * (STAGE_OUT + 128));
   volatile int* stop = reinterpret_cast<volatile int*>(bars + 2 * STAGES + 5);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 6);
   const uint32_t ring = smem_u32(smem), bar0 = smem_u32(bars);
@@ -301,6 +350,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
   auto acc_empty = [&](int a) { return bar0 + 8 * (2 * STAGES + 2 + a); };
   const uint32_t drained = bar0 + 8 * (2 * STAGES + 4);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int side = PAIR ? blockIdx.x & 1 : 0;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -309,7 +359,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(acc_full(a), 1);
-      mbar_init(acc_empty(a), EPI_WARPS);
+      mbar_init(acc_empty(a), PAIR ? 2 * EPI_WARPS : EPI_WARPS);
     }
     mbar_init(drained, 1);
     *stop = 0;
@@ -317,21 +367,28 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "n"(TMEM_COLS) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if constexpr (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "n"(TMEM_COLS) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "n"(TMEM_COLS) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
   }
   tc_fence_before();
   __syncthreads();
+  __syncwarp();
+  if constexpr (PAIR) cluster_barrier();  // the other block's barriers are ready
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
   // blocks of one cluster (splits > 1) share a tile and divide its k-blocks; otherwise a block walks over its tiles
-  const int rank = p.splits > 1 ? blockIdx.x % p.splits : 0;
+  const int rank = !PAIR && p.splits > 1 ? blockIdx.x % p.splits : 0;
   const int kb0 = (int)((int64_t)p.kblocks * rank / p.splits), kb1 = (int)((int64_t)p.kblocks * (rank + 1) / p.splits);
-  const int first = blockIdx.x / p.splits, step = gridDim.x / p.splits, tiles = p.tiles_m * p.tiles_n;
+  const int group = PAIR ? 2 : p.splits, first = blockIdx.x / group, step = gridDim.x / group, tiles = p.tiles_m * p.tiles_n;
 
   if (warp == 0) {
-    if (lane == 0) {  // loads
+    if (elect_one()) {  // loads
       int s = 0, phase = 0, issued = 0;
       bool ok = true;
       for (int t = first; t < tiles && ok; t += step) {
@@ -340,18 +397,20 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!(ok = mbar_wait(empty(s), phase ^ 1, stop))) break;
           const uint32_t a = ring + s * STAGE, b = a + A_BYTES;
-          mbar_expect(full(s), STAGE);
+          const int ra = PAIR ? tm * 2 * BM + side * BM : tm * BM, rb = tn * BN + side * BROWS;
+          const uint32_t bar = PAIR ? cluster_addr(full(s), 0) : full(s);  // a pair's loads report to its first block
+          if (side == 0) mbar_expect(full(s), PAIR ? 2 * STAGE : STAGE);
           if (p.a_mn) {
 #pragma unroll
-            for (int j = 0; j < BM / 64; ++j) tma_load(a + j * 8192, &map_a, tm * BM + j * 64, kb * BK, full(s));
+            for (int j = 0; j < BM / 64; ++j) tma_load<PAIR>(a + j * 8192, &map_a, ra + j * 64, kb * BK, bar);
           } else {
-            tma_load(a, &map_a, kb * BK, tm * BM, full(s));
+            tma_load<PAIR>(a, &map_a, kb * BK, ra, bar);
           }
           if (p.b_mn) {
 #pragma unroll
-            for (int j = 0; j < BN / 64; ++j) tma_load(b + j * 8192, &map_b, tn * BN + j * 64, kb * BK, full(s));
+            for (int j = 0; j < BROWS / 64; ++j) tma_load<PAIR>(b + j * 8192, &map_b, rb + j * 64, kb * BK, bar);
           } else {
-            tma_load(b, &map_b, kb * BK, tn * BN, full(s));
+            tma_load<PAIR>(b, &map_b, kb * BK, rb, bar);
           }
           ++issued;
           if (++s == STAGES) {
@@ -360,7 +419,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
           }
         }
       }
-      if (!ok) {  // the copies in flight must land before the block ends
+      if (!ok && side == 0) {  // the copies in flight must land before the block (the pair: both meet below) ends
         volatile int never = 0;
         for (int i = 0; i < STAGES && i < issued; ++i) {
           if (--s < 0) {
@@ -372,7 +431,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {  // products
+    if (side == 0 && elect_one()) {  // products
       // one 16-deep step inside a 64-deep k-block: 32 bytes along k-major rows, 16 rows of 128 bytes otherwise
       const uint32_t a_step = p.a_mn ? 2048 : 32, b_step = p.b_mn ? 2048 : 32;
       const uint32_t a_lead = p.a_mn ? 8192 : 16, b_lead = p.b_mn ? 8192 : 16;
@@ -387,16 +446,16 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
           const uint32_t a = ring + s * STAGE, b = a + A_BYTES;
 #pragma unroll
           for (int k = 0; k < BK / 16; ++k)
-            mma_f16(tmem + acc * BN, smem_desc(a + k * a_step, a_lead, 1024), smem_desc(b + k * b_step, b_lead, 1024), p.idesc,
+            mma_f16<PAIR>(tmem + acc * BN, smem_desc(a + k * a_step, a_lead, 1024), smem_desc(b + k * b_step, b_lead, 1024), p.idesc,
                     kb != kb0 || k != 0);
-          mma_commit(empty(s));
+          mma_commit<PAIR>(empty(s));
           if (++s == STAGES) {
             s = 0;
             phase ^= 1;
           }
         }
         if (!ok) break;
-        mma_commit(acc_full(acc));
+        mma_commit<PAIR>(acc_full(acc));
         if (++acc == 2) {
           acc = 0;
           acc_phase ^= 1;
@@ -404,7 +463,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
       }
       if (!ok) {  // products in flight must end before TMEM is freed
         volatile int never = 0;
-        mma_commit(drained);
+        mma_commit<PAIR>(drained);
         mbar_wait(drained, 0, &never);
       }
     }
@@ -412,16 +471,19 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
     // epilogue: warp w reads the TMEM lanes of its quarter; two warps share a quarter and take 32-column slices in turn
     const int quarter = warp & 3, half = (warp - 2) >> 2;
     uint8_t* stage = staging + (warp - 2) * STAGE_OUT;
+    float* bias_slice = bias_slices + (warp - 2) * 32;
     const T* bias = static_cast<const T*>(p.bias);
     int acc = 0, acc_phase = 0;
     for (int t = first; t < tiles; t += step) {
       int tm, tn;
       tile_at(p, t, tm, tn);
+      const int64_t r0 = (int64_t)(PAIR ? tm * 2 + side : tm) * BM + quarter * 32;
+      uint4 early[4];
+      if (p.residual && p.splits == 1 && !p.swap) fetch_in(early, p.residual, p.ldr, p.vec_r, r0, (int64_t)tn * BN + half * 32, p.m, p.n);
       if (!mbar_wait(acc_full(acc), acc_phase, stop)) break;
       tc_fence_after();
-      const int64_t r0 = (int64_t)tm * BM + quarter * 32;
       const uint32_t src = tmem + acc * BN + ((uint32_t)(quarter * 32) << 16);
-      if (p.splits > 1) {  // to shared memory (the ring is free: every load was consumed before acc_full)
+      if (!PAIR && p.splits > 1) {  // to shared memory (the ring is free: every load was consumed before acc_full)
         float* part = reinterpret_cast<float*>(smem);
         for (int c = half * 32; c < BN; c += 64) {
           float v[32];
@@ -447,11 +509,11 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
           }
           continue;
         }
-        float bv = 0.f;
-        if (bias && c0 + lane < p.n) bv = to_f<T>(bias[c0 + lane]);
+        if (bias) bias_slice[lane] = c0 + lane < p.n ? to_f<T>(bias[c0 + lane]) : 0.f;
         float res[32];
         if (p.residual) {
-          stage_in(stage, p.residual, p.ldr, p.vec_r, r0, c0, p.m, p.n);
+          stage_in(stage, early, p.residual, p.ldr, p.vec_r, r0, c0, p.m, p.n);
+          if (c + 64 < BN) fetch_in(early, p.residual, p.ldr, p.vec_r, r0, c0 + 64, p.m, p.n);
           __syncwarp();
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -464,8 +526,15 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
         }
         tmem_load32(src + c, v);
         if (bias) {
+          __syncwarp();
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] += __shfl_sync(FULL, bv, i);
+          for (int i = 0; i < 8; ++i) {
+            const float4 b4 = reinterpret_cast<const float4*>(bias_slice)[i];
+            v[4 * i] += b4.x;
+            v[4 * i + 1] += b4.y;
+            v[4 * i + 2] += b4.z;
+            v[4 * i + 3] += b4.w;
+          }
         }
         if (p.z) {
           stage_row<T>(stage, lane, v, false);
@@ -484,11 +553,16 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
         stage_row<T>(stage, lane, v, p.out_f32);
         __syncwarp();
         stage_out(stage, p.y, p.ldy, p.out_f32 ? 4 : 2, p.vec_y, r0, c0, p.m, p.n);
-        __syncwarp();
+        __syncwarp();  // the staging rows and the bias slice may be written again
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(acc_empty(acc));
+      if (lane == 0) {
+        if constexpr (PAIR)
+          mbar_arrive_far(cluster_addr(acc_empty(acc), 0));
+        else
+          mbar_arrive(acc_empty(acc));
+      }
       if (++acc == 2) {
         acc = 0;
         acc_phase ^= 1;
@@ -496,7 +570,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
     }
   }
   __syncwarp();
-  if (p.splits > 1) {
+  if (!PAIR && p.splits > 1) {
     __syncthreads();
     __syncwarp();
     cluster_barrier();
@@ -536,10 +610,15 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
     cluster_barrier();  // nobody leaves while others read its shared memory
   }
   __syncthreads();
+  __syncwarp();
+  if constexpr (PAIR) cluster_barrier();  // the pair's loads, products and arrivals are done on both sides
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(TMEM_COLS) : "memory");
+    if constexpr (PAIR)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(TMEM_COLS) : "memory");
+    else
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(TMEM_COLS) : "memory");
   }
 }
 
@@ -738,37 +817,40 @@ int make_map(CUtensorMap* map, const Operand& o, int dtype, int box_rows) {
 
 struct Shape {
   int bn, splits;
+  bool pair;
 };
-// Tile width and split of k: the combination with the least estimated time, in units of one 128 x 64 x 64 product.  A
-// block pays for its k-blocks, about six units to fill the pipeline and drain the tile, and with a split two more
-// for the exchange.
+// Tile and split of k: the combination with the least estimated time, in units of one 128 x 64 x 64 product.  A block
+// pays for its k-blocks (bound by the issue of loads below a width of 3 units), about six units to fill the pipeline
+// and drain the tile, and with a split two more for the exchange.
 Shape choose_shape(int64_t m, int64_t n, int64_t kblocks, int sms, bool narrow) {
-  Shape best{64, 1};
+  Shape best{64, 1, false};
   double least = 1e300;
-  for (int bn : {256, 128, 64}) {
+  for (int bn : {512, 256, 128, 64}) {  // 512: a pair on 256 x 256
     if (narrow && bn > 64) continue;
-    const double tiles = (double)((m + BM - 1) / BM) * (double)((n + bn - 1) / bn);
+    const bool pair = bn == 512;
+    const int64_t tm = (m + (pair ? 2 * BM : BM) - 1) / (pair ? 2 * BM : BM), tn = (n + (pair ? 256 : bn) - 1) / (pair ? 256 : bn);
+    const double tiles = (double)tm * (double)tn, places = pair ? sms / 2 : sms;
     for (int s : {1, 2, 4, 8}) {
-      if (s > 1 && (s > kblocks || tiles * s > sms)) break;
-      const double waves = (double)((int64_t)(tiles * s + sms - 1) / sms);
-      const double width = bn / 64.0;
-      const double t = waves * ((double)((kblocks + s - 1) / s) * std::max(width, 1.5) + width) + 6.0 + (s > 1 ? 2.0 + width : 0.0);
+      if (s > 1 && (pair || s > kblocks || tiles * s > sms)) break;
+      const double waves = (double)((int64_t)((tiles * s + places - 1) / places));
+      const double width = pair ? 4.0 : bn == 256 ? 4.6 : bn == 128 ? 3.2 : 2.9;
+      const double t = waves * ((double)((kblocks + s - 1) / s) * width + bn / 64.0) + 6.0 + (s > 1 ? 2.0 + width : 0.0);
       if (t < least) {
         least = t;
-        best = {bn, s};
+        best = {pair ? 256 : bn, s, pair};
       }
     }
   }
   return best;
 }
 
-template <typename T, int BN>
+template <typename T, int BN, bool PAIR>
 int launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const GemmParams& p, unsigned grid, int splits, cudaStream_t st) {
   static bool ready[64] = {false};  // per device; setting it twice does no harm
   int device = 0;
   FV_CUDA(cudaGetDevice(&device));
   if (device >= 64 || !ready[device]) {
-    FV_CUDA(cudaFuncSetAttribute(k_gemm<T, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, GEMM_SMEM));
+    FV_CUDA(cudaFuncSetAttribute(k_gemm<T, BN, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, GEMM_SMEM));
     if (device < 64) ready[device] = true;
   }
   cudaLaunchConfig_t cfg{};
@@ -778,11 +860,11 @@ int launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const GemmParams& p,
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)splits;
+  attr[0].val.clusterDim.x = PAIR ? 2u : (unsigned)splits;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = splits > 1 ? 1 : 0;
-  FV_CUDA(cudaLaunchKernelEx(&cfg, k_gemm<T, BN>, a, b, p));
+  cfg.numAttrs = PAIR || splits > 1 ? 1 : 0;
+  FV_CUDA(cudaLaunchKernelEx(&cfg, k_gemm<T, BN, PAIR>, a, b, p));
   return FV_OK;
 }
 
@@ -795,28 +877,27 @@ int gemm(Operand a, Operand b, int dtype, GemmParams p, Workspace& ws, int sms, 
   p.kblocks = (int)((a.depth + BK - 1) / BK);
   const Shape s = choose_shape(p.m, p.n, p.kblocks, sms, narrow);
   p.splits = s.splits;
-  p.tiles_m = (int)((p.m + BM - 1) / BM);
+  const int rows = s.pair ? 2 * BM : BM;
+  p.tiles_m = (int)((p.m + rows - 1) / rows);
   p.tiles_n = (int)((p.n + s.bn - 1) / s.bn);
   FV_REQUIRE((int64_t)p.tiles_m * p.tiles_n < (1ll << 30), FV_ERR_INVALID, "the product is too large");
   p.a_mn = a.mn;
   p.b_mn = b.mn;
   const uint32_t type = dtype == FV_BF16 ? 1u : 0u;
-  p.idesc = 1u << 4 | type << 7 | type << 10 | (uint32_t)a.mn << 15 | (uint32_t)b.mn << 16 | (uint32_t)(s.bn / 8) << 17 | (uint32_t)(BM / 16) << 24;
+  p.idesc = 1u << 4 | type << 7 | type << 10 | (uint32_t)a.mn << 15 | (uint32_t)b.mn << 16 | (uint32_t)(s.bn / 8) << 17 | (uint32_t)(rows / 16) << 24;
   CUtensorMap ma, mb;
   if (int rc = make_map(&ma, a, dtype, BM)) return rc;
-  if (int rc = make_map(&mb, b, dtype, s.bn)) return rc;
+  if (int rc = make_map(&mb, b, dtype, s.pair ? s.bn / 2 : s.bn)) return rc;
   const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
-  const unsigned grid = (unsigned)(s.splits > 1 ? tiles * s.splits : std::min<int64_t>(tiles, sms));
-  if (dtype == FV_BF16) {
-    using T = __nv_bfloat16;
-    return s.bn == 256 ? launch_gemm<T, 256>(ma, mb, p, grid, s.splits, st)
-           : s.bn == 128 ? launch_gemm<T, 128>(ma, mb, p, grid, s.splits, st)
-                         : launch_gemm<T, 64>(ma, mb, p, grid, s.splits, st);
-  }
-  using T = __half;
-  return s.bn == 256 ? launch_gemm<T, 256>(ma, mb, p, grid, s.splits, st)
-         : s.bn == 128 ? launch_gemm<T, 128>(ma, mb, p, grid, s.splits, st)
-                       : launch_gemm<T, 64>(ma, mb, p, grid, s.splits, st);
+  const unsigned grid = (unsigned)(s.splits > 1 ? tiles * s.splits : std::min<int64_t>(tiles, s.pair ? sms / 2 : sms) * (s.pair ? 2 : 1));
+  auto go = [&](auto tag) {
+    using T = decltype(tag);
+    return s.pair        ? launch_gemm<T, 256, true>(ma, mb, p, grid, 1, st)
+           : s.bn == 256 ? launch_gemm<T, 256, false>(ma, mb, p, grid, s.splits, st)
+           : s.bn == 128 ? launch_gemm<T, 128, false>(ma, mb, p, grid, s.splits, st)
+                         : launch_gemm<T, 64, false>(ma, mb, p, grid, s.splits, st);
+  };
+  return dtype == FV_BF16 ? go(__nv_bfloat16{}) : go(__half{});
 }
 
 template <typename T, int VEC, int G>

@@ -448,8 +448,9 @@ def test_linear(built_lib, rows, inner, outer, dtype):
             slack = slack + want.abs() * U
         close(z, want, rounded(want, dtype, slack))
         y = ACTS[act](want)
-        # slopes are below 1.13; the activation itself: erfc, exp and a quotient, 2^-20 of its value with arguments below 32
-        s = 1.13 * slack + y.abs() * 2.0 ** -20 * (act != "none")
+        # slopes are below 1.13; the activation itself: an exp and a quotient, 2^-20 of its value with arguments below 32, and
+        # for the gelu the published bound of its erf, 1.5e-7, times z / 2
+        s = 1.13 * slack + y.abs() * 2.0 ** -20 * (act != "none") + want.abs() * 7.5e-8 * (act == "gelu")
         if residual:
             y = y + r.double()
             s = s + y.abs() * U
@@ -496,7 +497,7 @@ def test_linear_backward(built_lib, rows, inner, outer, dtype):
         if act != "none":
             zz = z.double().requires_grad_()
             dz, = torch.autograd.grad(ACTS[act](zz), zz, dy.double())
-            # the slope: sums of terms up to 1.13 + |z| / 2 in magnitude, each good to 2^-20
+            # the slope: sums of terms up to 1.13 + |z| / 2 in magnitude, each good to 2^-20 (erf: 1.5e-7 / 2)
             off = dy.double().abs() * 2.0 ** -20 * (2 + z.double().abs())
         dz16 = off + dz.abs() * half_step(dtype) + floor_step(dtype) if act != "none" else off  # as the products see it
         want = dz @ w.double()
