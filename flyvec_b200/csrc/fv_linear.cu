@@ -38,46 +38,82 @@ namespace fvo {
 namespace {
 
 // ---- activations ------------------------------------------------------------------------------------
-// The normal distribution function, Phi(z) = erfc(-z / sqrt(2)) / 2, by Abramowitz and Stegun's formula 7.1.26
-// (|error of erf| <= 1.5e-7, and it shrinks with exp(-z^2 / 2) for z < 0): two special-function calls and ten
-// multiplications instead of the forty operations of erfcf.
-__device__ __forceinline__ float normal_cdf(float z) {
-  const float x = fabsf(z) * 0.70710678f, t = __fdividef(1.0f, fmaf(0.3275911f, x, 1.0f));
-  float q = fmaf(1.061405429f, t, -1.453152027f);
-  q = fmaf(q, t, 1.421413741f);
-  q = fmaf(q, t, -0.284496736f);
-  q = fmaf(q, t, 0.254829592f);
-  q *= 0.5f * t * __expf(-x * x);
-  return z < 0.f ? q : 1.0f - q;
+constexpr float LOG2E = 1.4426950408889634f;
+// exp(-z^2 / 2) and the tail Phi(-|z|) of the normal distribution, by Abramowitz and Stegun's formula 7.1.26 for erfc
+// (|error of erf| <= 1.5e-7, shrinking with exp(-z^2 / 2)): two special-function calls a value, the rest two values at a
+// time.  az = |z|.
+__device__ __forceinline__ float2 normal_tail(float2 z, float2 az, float2& e) {
+  const float2 d = fma2(both(0.3275911f * 0.70710678f), az, both(1.0f)), t = make_float2(rcp(d.x), rcp(d.y));
+  const float2 l = mul2(mul2(z, z), both(-0.5f * LOG2E));
+  e = make_float2(ex2(l.x), ex2(l.y));
+  float2 q = fma2(both(0.5f * 1.061405429f), t, both(0.5f * -1.453152027f));
+  q = fma2(q, t, both(0.5f * 1.421413741f));
+  q = fma2(q, t, both(0.5f * -0.284496736f));
+  q = fma2(q, t, both(0.5f * 0.254829592f));
+  return mul2(mul2(q, t), e);
 }
-__device__ __forceinline__ float act_value(float z, int act) {
-  switch (act) {
-    case FV_ACT_RELU: return z < 0.f ? 0.f : z;  // keeps a NaN
-    case FV_ACT_GELU: return z * normal_cdf(z);
-    case FV_ACT_GELU_TANH: {
-      const float u = 0.7978845608f * fmaf(0.044715f * z * z, z, z);
-      return __fdividef(z, 1.0f + __expf(-2.0f * u));  // (1 + tanh u) / 2 = 1 / (1 + exp(-2 u))
-    }
-    case FV_ACT_SILU: return __fdividef(z, 1.0f + __expf(-z));
-    default: return z;
+// |z|, kept finite so that 0 times it stays 0
+__device__ __forceinline__ float2 magnitude(float2 z) { return make_float2(min_nan(fabsf(z.x), 1e30f), min_nan(fabsf(z.y), 1e30f)); }
+// 1 / (1 + exp(-x))
+__device__ __forceinline__ float2 logistic(float2 x) {
+  const float2 l = mul2(x, both(-LOG2E)), d = add2(make_float2(ex2(l.x), ex2(l.y)), both(1.0f));
+  return make_float2(rcp(d.x), rcp(d.y));
+}
+constexpr float TANH_A = 0.7978845608f, TANH_B = 0.044715f;  // (1 + tanh u) / 2 = 1 / (1 + exp(-2 u)), u = A (z + B z^3)
+
+template <int ACT>
+__device__ __forceinline__ float2 act_value(float2 z) {
+  if constexpr (ACT == FV_ACT_RELU) return make_float2(max_nan(z.x, 0.f), max_nan(z.y, 0.f));
+  if constexpr (ACT == FV_ACT_GELU) {  // z Phi(z) = max(z, 0) - |z| Phi(-|z|)
+    const float2 az = magnitude(z);
+    float2 e;
+    const float2 q = normal_tail(z, az, e);
+    return fma2(make_float2(-az.x, -az.y), q, make_float2(max_nan(z.x, 0.f), max_nan(z.y, 0.f)));
+  }
+  if constexpr (ACT == FV_ACT_GELU_TANH)
+    return mul2(z, logistic(mul2(z, fma2(mul2(z, z), both(2.0f * TANH_A * TANH_B), both(2.0f * TANH_A)))));
+  if constexpr (ACT == FV_ACT_SILU) return mul2(z, logistic(z));
+  return z;
+}
+template <int ACT>
+__device__ __forceinline__ float2 act_slope(float2 z) {
+  if constexpr (ACT == FV_ACT_RELU)  // NaN for a NaN
+    return make_float2(z.x > 0.f ? 1.f : z.x <= 0.f ? 0.f : z.x, z.y > 0.f ? 1.f : z.y <= 0.f ? 0.f : z.y);
+  if constexpr (ACT == FV_ACT_GELU) {  // Phi(z) + z phi(z)
+    float2 e;
+    const float2 q = normal_tail(z, magnitude(z), e);
+    const float2 side = make_float2(copysignf(0.5f - q.x, z.x), copysignf(0.5f - q.y, z.y));
+    return add2(side, fma2(mul2(make_float2(max_nan(min_nan(z.x, 1e30f), -1e30f), max_nan(min_nan(z.y, 1e30f), -1e30f)), e),
+                           both(0.3989422804f), both(0.5f)));
+  }
+  if constexpr (ACT == FV_ACT_GELU_TANH) {
+    // beyond 16 the slope is 0 or 1 to the last bit, and z z would overflow at last
+    const float2 y = make_float2(max_nan(min_nan(z.x, 16.f), -16.f), max_nan(min_nan(z.y, 16.f), -16.f)), y2 = mul2(y, y);
+    const float2 s = logistic(mul2(y, fma2(y2, both(2.0f * TANH_A * TANH_B), both(2.0f * TANH_A))));
+    const float2 r = make_float2(1.0f - s.x, 1.0f - s.y);  // s + y s (1 - s) 2 A (1 + 3 B y^2)
+    return fma2(mul2(mul2(y, s), r), fma2(y2, both(6.0f * TANH_A * TANH_B), both(2.0f * TANH_A)), s);
+  }
+  if constexpr (ACT == FV_ACT_SILU) {
+    const float2 y = make_float2(max_nan(z.x, -1e30f), max_nan(z.y, -1e30f)), s = logistic(y);
+    return mul2(s, fma2(y, make_float2(1.0f - s.x, 1.0f - s.y), both(1.0f)));
+  }
+  return both(1.0f);
+}
+template <int ACT, int N>
+__device__ __forceinline__ void act_each(float (&v)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    const float2 y = act_value<ACT>(make_float2(v[i], v[i + 1]));
+    v[i] = y.x;
+    v[i + 1] = y.y;
   }
 }
-__device__ __forceinline__ float act_slope(float z, int act) {
-  switch (act) {
-    case FV_ACT_RELU: return z > 0.f ? 1.f : z <= 0.f ? 0.f : z;
-    case FV_ACT_GELU: return fmaf(z, 0.3989422804f * __expf(-0.5f * z * z), normal_cdf(z));
-    case FV_ACT_GELU_TANH: {
-      if (fabsf(z) > 16.f) return z > 0.f ? 1.f : 0.f;  // to float's last bit; beyond, z * z may overflow
-      const float z2 = z * z, u = 0.7978845608f * fmaf(0.044715f * z2, z, z);
-      const float s = __fdividef(1.0f, 1.0f + __expf(-2.0f * u));
-      return s + z * (2.0f * s * (1.0f - s)) * 0.7978845608f * fmaf(3.0f * 0.044715f, z2, 1.0f);
-    }
-    case FV_ACT_SILU: {
-      const float s = __fdividef(1.0f, 1.0f + __expf(-z));
-      return s * fmaf(z, 1.0f - s, 1.0f);
-    }
-    default: return 1.f;
-  }
+template <int N>
+__device__ __forceinline__ void act_values(float (&v)[N], int act) {
+  if (act == FV_ACT_RELU) act_each<FV_ACT_RELU>(v);
+  if (act == FV_ACT_GELU) act_each<FV_ACT_GELU>(v);
+  if (act == FV_ACT_GELU_TANH) act_each<FV_ACT_GELU_TANH>(v);
+  if (act == FV_ACT_SILU) act_each<FV_ACT_SILU>(v);
 }
 
 // ---- device-side status -----------------------------------------------------------------------------
@@ -240,86 +276,124 @@ __device__ __forceinline__ void tile_at(const GemmParams& p, int t, int& tm, int
   tm = band * BAND + in - tn * rows;
 }
 
+// An epilogue warp's staging: 32 rows of 128 bytes, the 16-byte words of row r swizzled with r % 8 as TMA's 128-byte
+// swizzle does (so that lanes writing one word of eight rows hit all banks).  A slice of the output is 128 bytes wide: 64
+// columns of 16 bits in two halves, or 32 of float.
 template <typename T>
-__device__ __forceinline__ void stage_row(uint8_t* stage, int row, const float (&v)[32], bool f32) {
+__device__ __forceinline__ void stage_row(uint8_t* stage, int row, const float (&v)[32], int half) {
   uint8_t* base = stage + row * 128;
-  if (f32) {
 #pragma unroll
-    for (int c = 0; c < 8; ++c)
-      *reinterpret_cast<float4*>(base + ((c ^ (row & 7)) << 4)) = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
-  } else {
+  for (int c = 0; c < 4; ++c) {
+    Pack<T, 8> o;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      Pack<T, 8> o;
+    for (int i = 0; i < 8; ++i) o.e[i] = from_f<T>(v[8 * c + i]);
+    *reinterpret_cast<uint4*>(base + (((c + 4 * half) ^ (row & 7)) << 4)) = o.w;
+  }
+}
+__device__ __forceinline__ void stage_row_f32(uint8_t* stage, int row, const float (&v)[32]) {
+  uint8_t* base = stage + row * 128;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) o.e[i] = from_f<T>(v[8 * c + i]);
-      *reinterpret_cast<uint4*>(base + ((c ^ (row & 7)) << 4)) = o.w;
+  for (int c = 0; c < 8; ++c)
+    *reinterpret_cast<float4*>(base + ((c ^ (row & 7)) << 4)) = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+}
+// The staged rows as a 128-byte wide box of the output; what lies outside the output is not written.
+__device__ __forceinline__ void stage_store(const uint8_t* stage, const CUtensorMap* map, int64_t r0, int64_t c0) {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"((int)c0), "r"((int)r0),
+                 "r"(smem_u32(stage))
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+  }
+}
+// before the staging rows are written again
+__device__ __forceinline__ void stage_free() {
+  if ((threadIdx.x & 31) == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+  __syncwarp();
+}
+// The same for outputs whose rows do not start on 16-byte boundaries: 32 columns, element by element.
+__device__ __forceinline__ void stage_out(const uint8_t* stage, void* out, int64_t ld, int es, int half, int64_t r0, int64_t c0, int64_t rows,
+                                          int64_t cols) {
+  const int lane = threadIdx.x & 31, at = lane * es + (es == 2 ? 64 * half : 0);
+  __syncwarp();
+  if (c0 + lane < cols) {
+    uint8_t* d = static_cast<uint8_t*>(out) + (r0 * ld + c0 + lane) * es;
+    const int n = (int)min((int64_t)32, rows - r0);
+#pragma unroll 4
+    for (int r = 0; r < n; ++r, d += ld * es) {
+      const uint8_t* s = stage + r * 128 + (((at >> 4) ^ (r & 7)) << 4) + (at & 15);
+      if (es == 4)
+        *reinterpret_cast<uint32_t*>(d) = *reinterpret_cast<const uint32_t*>(s);
+      else
+        *reinterpret_cast<uint16_t*>(d) = *reinterpret_cast<const uint16_t*>(s);
     }
   }
+  __syncwarp();
 }
-// The staged 32 x 32 elements (of `es` bytes) to rows [r0, ...) and columns [c0, ...) of an array, guarded.
-__device__ __forceinline__ void stage_out(const uint8_t* stage, void* out, int64_t ld, int es, bool vec, int64_t r0, int64_t c0,
-                                          int64_t rows, int64_t cols) {
-  const int lane = threadIdx.x & 31;
-  uint8_t* base = static_cast<uint8_t*>(out);
-  if (vec && c0 + 32 <= cols) {
-    const int per = es == 4 ? 8 : 4;  // 16-byte words in a row
-    const int c = lane & (per - 1);
-#pragma unroll 4
-    for (int r = lane / per; r < 32; r += 32 / per)
-      if (r0 + r < rows)
-        *reinterpret_cast<uint4*>(base + ((r0 + r) * ld + c0) * es + c * 16) =
-            *reinterpret_cast<const uint4*>(stage + r * 128 + ((c ^ (r & 7)) << 4));
-  } else if (c0 + lane < cols) {
-#pragma unroll 4
-    for (int r = 0; r < 32; ++r)
-      if (r0 + r < rows) {
-        const uint8_t* s = stage + r * 128 + (((lane * es >> 4) ^ (r & 7)) << 4) + (lane * es & 15);
-        uint8_t* d = base + ((r0 + r) * ld + c0 + lane) * es;
-        if (es == 4)
-          *reinterpret_cast<uint32_t*>(d) = *reinterpret_cast<const uint32_t*>(s);
-        else
-          *reinterpret_cast<uint16_t*>(d) = *reinterpret_cast<const uint16_t*>(s);
-      }
+// The staged 64 columns of 16 bits to an array by plain stores, whole lines where its rows admit 16-byte words; unlike
+// the asynchronous copy it is done with the staging rows when it returns.
+__device__ __forceinline__ void copy_out(const uint8_t* stage, void* out, int64_t ld, bool vec, int64_t r0, int64_t c0, int64_t rows,
+                                         int64_t cols) {
+  if (!vec || c0 + 64 > cols) {
+    stage_out(stage, out, ld, 2, 0, r0, c0, rows, cols);
+    if (c0 + 32 < cols) stage_out(stage, out, ld, 2, 1, r0, c0 + 32, rows, cols);
+    return;
   }
+  const int lane = threadIdx.x & 31;
+  __syncwarp();
+  uint8_t* base = static_cast<uint8_t*>(out) + ((r0 + lane / 8) * ld + c0) * 2 + (lane & 7) * 16;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const int r = lane / 8 + 4 * k;
+    if (r0 + r < rows)
+      *reinterpret_cast<uint4*>(base + 8 * k * ld) = *reinterpret_cast<const uint4*>(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+  }
+  __syncwarp();
 }
-// 32 x 32 16-bit elements of an array: fetched early into registers (four 16-byte words a lane; rows that do not admit
+// 32 x 64 16-bit elements of an array: fetched early into registers (eight 16-byte words a lane; rows that do not admit
 // them are fetched late, element by element), then put into the staging rows.  What lies outside reads as 0.
-__device__ __forceinline__ void fetch_in(uint4 (&w)[4], const void* in, int64_t ld, bool vec, int64_t r0, int64_t c0, int64_t rows,
+__device__ __forceinline__ void fetch_in(uint4 (&w)[8], const void* in, int64_t ld, bool vec, int64_t r0, int64_t c0, int64_t rows,
                                          int64_t cols) {
   const int lane = threadIdx.x & 31;
-  if (!vec || c0 + 32 > cols) return;
-  const uint8_t* base = static_cast<const uint8_t*>(in) + ((r0 + lane / 4) * ld + c0) * 2 + (lane & 3) * 16;
+  if (!vec || c0 + 64 > cols) return;
+  const uint8_t* base = static_cast<const uint8_t*>(in) + ((r0 + lane / 8) * ld + c0) * 2 + (lane & 7) * 16;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
+  for (int k = 0; k < 8; ++k) {
     w[k] = make_uint4(0, 0, 0, 0);
-    if (r0 + lane / 4 + 8 * k < rows) w[k] = __ldcs(reinterpret_cast<const uint4*>(base + 16 * k * ld));
+    if (r0 + lane / 8 + 4 * k < rows) w[k] = __ldcs(reinterpret_cast<const uint4*>(base + 8 * k * ld));
   }
 }
-__device__ __forceinline__ void stage_in(uint8_t* stage, const uint4 (&w)[4], const void* in, int64_t ld, bool vec, int64_t r0, int64_t c0,
+__device__ __forceinline__ void stage_in(uint8_t* stage, const uint4 (&w)[8], const void* in, int64_t ld, bool vec, int64_t r0, int64_t c0,
                                          int64_t rows, int64_t cols) {
   const int lane = threadIdx.x & 31;
-  if (vec && c0 + 32 <= cols) {
+  if (vec && c0 + 64 <= cols) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int r = lane / 4 + 8 * k;
-      *reinterpret_cast<uint4*>(stage + r * 128 + (((lane & 3) ^ (r & 7)) << 4)) = w[k];
+    for (int k = 0; k < 8; ++k) {
+      const int r = lane / 8 + 4 * k;
+      *reinterpret_cast<uint4*>(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4)) = w[k];
     }
   } else {
     const uint8_t* base = static_cast<const uint8_t*>(in);
-#pragma unroll 8
-    for (int r = 0; r < 32; ++r) {
-      uint16_t v = 0;
-      if (r0 + r < rows && c0 + lane < cols) v = __ldg(reinterpret_cast<const uint16_t*>(base + ((r0 + r) * ld + c0 + lane) * 2));
-      *reinterpret_cast<uint16_t*>(stage + r * 128 + (((lane >> 3) ^ (r & 7)) << 4) + (lane & 7) * 2) = v;
-    }
+#pragma unroll 4
+    for (int r = 0; r < 32; ++r)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int c = lane + 32 * h;
+        uint16_t v = 0;
+        if (r0 + r < rows && c0 + c < cols) v = __ldg(reinterpret_cast<const uint16_t*>(base + ((r0 + r) * ld + c0 + c) * 2));
+        *reinterpret_cast<uint16_t*>(stage + r * 128 + (((c >> 3) ^ (r & 7)) << 4) + (c & 7) * 2) = v;
+      }
   }
+  __syncwarp();
 }
 
 template <typename T>
 __device__ __forceinline__ void store_one(const GemmParams& p, int64_t r, int64_t c, float v) {  // r, c: row and column of y
   if (p.z) static_cast<T*>(p.z)[r * p.ldz + c] = from_f<T>(v);
-  v = act_value(v, p.act);
+  float one[2] = {v, v};
+  act_values(one, p.act);
+  v = one[0];
   if (p.residual) v += to_f<T>(static_cast<const T*>(p.residual)[r * p.ldr + c]);
   if (p.out_f32)
     static_cast<float*>(p.y)[r * p.ldy + c] = v;
@@ -332,7 +406,8 @@ __device__ __forceinline__ void store_one(const GemmParams& p, int64_t r, int64_
 // the accumulator through the epilogue.
 template <typename T, int BN, bool PAIR>
 __global__ void __launch_bounds__(GEMM_THREADS, 1)
-    k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ GemmParams p) {
+    k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_y,
+           const __grid_constant__ GemmParams p) {
   constexpr int BROWS = PAIR ? BN / 2 : BN;  // rows of B this block loads
   constexpr int A_BYTES = BM * BK * 2, B_BYTES = BROWS * BK * 2, STAGE = A_BYTES + B_BYTES, STAGES = RING_BYTES / STAGE;
   constexpr int TMEM_COLS = 2 * BN;
@@ -468,7 +543,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
       }
     }
   } else {
-    // epilogue: warp w reads the TMEM lanes of its quarter; two warps share a quarter and take 32-column slices in turn
+    // epilogue: warp w reads the TMEM lanes of its quarter; two warps share a quarter and take 64-column slices in turn
     const int quarter = warp & 3, half = (warp - 2) >> 2;
     uint8_t* stage = staging + (warp - 2) * STAGE_OUT;
     float* bias_slice = bias_slices + (warp - 2) * 32;
@@ -478,8 +553,17 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
       int tm, tn;
       tile_at(p, t, tm, tn);
       const int64_t r0 = (int64_t)(PAIR ? tm * 2 + side : tm) * BM + quarter * 32;
-      uint4 early[4];
-      if (p.residual && p.splits == 1 && !p.swap) fetch_in(early, p.residual, p.ldr, p.vec_r, r0, (int64_t)tn * BN + half * 32, p.m, p.n);
+      uint4 early[8];
+      if (p.residual && p.splits == 1 && !p.swap && half * 64 < BN)
+        fetch_in(early, p.residual, p.ldr, p.vec_r, r0, (int64_t)tn * BN + half * 64, p.m, p.n);
+      float bias_reg[4];  // this warp's two slices, a column a lane
+      if (bias && p.splits == 1 && !p.swap) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int64_t c = (int64_t)tn * BN + half * 64 + (j >> 1) * 128 + (j & 1) * 32 + lane;
+          bias_reg[j] = c < p.n ? to_f<T>(bias[c]) : 0.f;
+        }
+      }
       if (!mbar_wait(acc_full(acc), acc_phase, stop)) break;
       tc_fence_after();
       const uint32_t src = tmem + acc * BN + ((uint32_t)(quarter * 32) << 16);
@@ -494,66 +578,103 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
         }
         break;  // one tile per cluster
       }
-      for (int c = half * 32; c < BN; c += 64) {
-        const int64_t c0 = (int64_t)tn * BN + c;
-        float v[32];
-        if (c0 >= p.n || r0 >= p.m) continue;  // nothing of this slice exists (uniform over the warp)
-        if (p.swap) {
+      if (p.swap) {
+        const int64_t o = r0 + lane;
+        for (int c = half * 32; c < BN; c += 64) {
+          const int64_t c0 = (int64_t)tn * BN + c;
+          if (c0 >= p.n || r0 >= p.m) continue;  // nothing of this slice exists (uniform over the warp)
+          float v[32];
           tmem_load32(src + c, v);
-          const int64_t o = r0 + lane;
           if (o < p.m) {
             const float bv = bias ? to_f<T>(bias[o]) : 0.f;
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if (c0 + i < p.n) store_one<T>(p, c0 + i, o, v[i] + bv);
           }
-          continue;
         }
-        if (bias) bias_slice[lane] = c0 + lane < p.n ? to_f<T>(bias[c0 + lane]) : 0.f;
-        float res[32];
-        if (p.residual) {
-          stage_in(stage, early, p.residual, p.ldr, p.vec_r, r0, c0, p.m, p.n);
-          if (c + 64 < BN) fetch_in(early, p.residual, p.ldr, p.vec_r, r0, c0 + 64, p.m, p.n);
-          __syncwarp();
+      } else {
+        for (int c = half * 64; c < BN; c += 128) {
+          const int64_t c0 = (int64_t)tn * BN + c;
+          if (c0 >= p.n || r0 >= p.m) continue;
+          uint4 res[8];  // the residual's row, then the result's
+          if (p.residual) {
+            stage_free();
+            stage_in(stage, early, p.residual, p.ldr, p.vec_r, r0, c0, p.m, p.n);
+            if (c + 128 < BN) fetch_in(early, p.residual, p.ldr, p.vec_r, r0, c0 + 128, p.m, p.n);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            Pack<T, 8> w;
-            w.w = *reinterpret_cast<const uint4*>(stage + lane * 128 + ((k ^ (lane & 7)) << 4));
-#pragma unroll
-            for (int i = 0; i < 8; ++i) res[8 * k + i] = to_f<T>(w.e[i]);
+            for (int k = 0; k < 8; ++k) res[k] = *reinterpret_cast<const uint4*>(stage + lane * 128 + ((k ^ (lane & 7)) << 4));
+            __syncwarp();
+          } else if (p.z) {
+            stage_free();
           }
-          __syncwarp();
-        }
-        tmem_load32(src + c, v);
-        if (bias) {
-          __syncwarp();
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float4 b4 = reinterpret_cast<const float4*>(bias_slice)[i];
-            v[4 * i] += b4.x;
-            v[4 * i + 1] += b4.y;
-            v[4 * i + 2] += b4.z;
-            v[4 * i + 3] += b4.w;
+          for (int h = 0; h < 2; ++h) {
+            const int64_t ch = c0 + 32 * h;
+            if (ch >= p.n) break;
+            float v[32];
+            if (bias) bias_slice[lane] = bias_reg[c >= 128 ? 2 + h : h];
+            tmem_load32(src + c + 32 * h, v);
+            if (bias) {
+              __syncwarp();
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const float4 b4 = reinterpret_cast<const float4*>(bias_slice)[i];
+                const float2 lo = add2(make_float2(v[4 * i], v[4 * i + 1]), make_float2(b4.x, b4.y));
+                const float2 hi = add2(make_float2(v[4 * i + 2], v[4 * i + 3]), make_float2(b4.z, b4.w));
+                v[4 * i] = lo.x;
+                v[4 * i + 1] = lo.y;
+                v[4 * i + 2] = hi.x;
+                v[4 * i + 3] = hi.y;
+              }
+              __syncwarp();  // the slice may be written again
+            }
+            if (p.z) {
+              stage_row<T>(stage, lane, v, h);
+              if (p.out_f32) stage_out(stage, p.z, p.ldz, 2, h, r0, ch, p.m, p.n);
+            }
+            act_values(v, p.act);
+            if (p.residual) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                Pack<T, 8> w;
+                w.w = res[4 * h + k];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[8 * k + i] += to_f<T>(w.e[i]);
+              }
+            }
+            if (p.out_f32) {
+              if (!p.z) stage_free();
+              stage_row_f32(stage, lane, v);
+              if (p.vec_y)
+                stage_store(stage, &map_y, r0, ch);
+              else
+                stage_out(stage, p.y, p.ldy, 4, 0, r0, ch, p.m, p.n);
+              if (p.z) stage_free();
+            } else {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                Pack<T, 8> o;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o.e[i] = from_f<T>(v[8 * k + i]);
+                res[4 * h + k] = o.w;
+              }
+            }
+          }
+          if (!p.out_f32) {
+            if (p.z)
+              copy_out(stage, p.z, p.ldz, p.vec_z, r0, c0, p.m, p.n);
+            else if (!p.residual)
+              stage_free();
+#pragma unroll
+            for (int k = 0; k < 8; ++k) *reinterpret_cast<uint4*>(stage + lane * 128 + ((k ^ (lane & 7)) << 4)) = res[k];
+            if (p.vec_y) {
+              stage_store(stage, &map_y, r0, c0);
+            } else {
+              stage_out(stage, p.y, p.ldy, 2, 0, r0, c0, p.m, p.n);
+              if (c0 + 32 < p.n) stage_out(stage, p.y, p.ldy, 2, 1, r0, c0 + 32, p.m, p.n);
+            }
           }
         }
-        if (p.z) {
-          stage_row<T>(stage, lane, v, false);
-          __syncwarp();
-          stage_out(stage, p.z, p.ldz, 2, p.vec_z, r0, c0, p.m, p.n);
-          __syncwarp();
-        }
-        if (p.act != FV_ACT_NONE) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = act_value(v[i], p.act);
-        }
-        if (p.residual) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] += res[i];
-        }
-        stage_row<T>(stage, lane, v, p.out_f32);
-        __syncwarp();
-        stage_out(stage, p.y, p.ldy, p.out_f32 ? 4 : 2, p.vec_y, r0, c0, p.m, p.n);
-        __syncwarp();  // the staging rows and the bias slice may be written again
       }
       tc_fence_before();
       __syncwarp();
@@ -568,6 +689,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
         acc_phase ^= 1;
       }
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // shared memory outlives the stores that read it
   }
   __syncwarp();
   if (!PAIR && p.splits > 1) {
@@ -687,11 +809,12 @@ __global__ void __launch_bounds__(256) k_pack(const uint16_t* __restrict__ src, 
 }
 
 // dz = dy act'(z) (if dz) and the partial column sums part[blockIdx.y][outer]; a warp takes every eighth row of the
-// block's range, a lane VEC columns.
-template <typename T, int VEC>
+// block's range, a lane VEC columns, ROWS rows in flight.
+template <typename T, int VEC, int ACT>
 __global__ void __launch_bounds__(256)
-    k_act_grad(const T* __restrict__ dy, int64_t ldg, const T* __restrict__ z, int64_t ldz, int64_t rows, int64_t outer, int act,
+    k_act_grad(const T* __restrict__ dy, int64_t ldg, const T* __restrict__ z, int64_t ldz, int64_t rows, int64_t outer,
                T* __restrict__ dz, int64_t pitch, float* __restrict__ part) {
+  constexpr int ROWS = 4;
   __shared__ float sum[8][32 * VEC];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t c = ((int64_t)blockIdx.x * 32 + lane) * VEC;
@@ -700,22 +823,29 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
   for (int i = 0; i < VEC; ++i) s[i] = 0.f;
   if (c < outer) {
-#pragma unroll 2
-    for (int64_t r = r0 + warp; r < r1; r += 8) {
-      Pack<T, VEC> g = load_pack_stream<T, VEC>(dy + r * ldg + c);
-      if (act != FV_ACT_NONE) {
-        const Pack<T, VEC> q = load_pack_stream<T, VEC>(z + r * ldz + c);
+    for (int64_t r = r0 + warp; r < r1; r += 8 * ROWS) {
+      Pack<T, VEC> g[ROWS], q[ROWS];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float v = to_f<T>(g.e[i]) * act_slope(to_f<T>(q.e[i]), act);
-          s[i] += v;
-          g.e[i] = from_f<T>(v);
+      for (int k = 0; k < ROWS; ++k)
+        if (r + 8 * k < r1) {
+          g[k] = load_pack_stream<T, VEC>(dy + (r + 8 * k) * ldg + c);
+          if (ACT != FV_ACT_NONE) q[k] = load_pack_stream<T, VEC>(z + (r + 8 * k) * ldz + c);
         }
-      } else {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) s[i] += to_f<T>(g.e[i]);
-      }
-      if (dz) store_pack<T, VEC>(dz + r * pitch + c, g);
+      for (int k = 0; k < ROWS; ++k)
+        if (r + 8 * k < r1) {
+#pragma unroll
+          for (int i = 0; i < VEC; i += 2) {
+            constexpr int one = VEC > 1;
+            float2 v = make_float2(to_f<T>(g[k].e[i]), to_f<T>(g[k].e[i + one]));
+            if (ACT != FV_ACT_NONE) v = mul2(v, act_slope<ACT>(make_float2(to_f<T>(q[k].e[i]), to_f<T>(q[k].e[i + one]))));
+            s[i] += v.x;
+            if (one) s[i + one] += v.y;
+            g[k].e[i] = from_f<T>(v.x);
+            if (one) g[k].e[i + one] = from_f<T>(v.y);
+          }
+          if (dz) store_pack<T, VEC>(dz + (r + 8 * k) * pitch + c, g[k]);
+        }
     }
   }
 #pragma unroll
@@ -727,6 +857,18 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
     for (int w = 0; w < 8; ++w) v += sum[w][i];
     if (col < outer) part[(int64_t)blockIdx.y * outer + col] = v;
+  }
+}
+template <typename T, int VEC>
+void launch_act_grad(cudaStream_t st, const T* dy, int64_t ldg, const T* z, int64_t ldz, int64_t rows, int64_t outer, int act, T* dz,
+                     int64_t pitch, float* part, int64_t chunks) {
+  const dim3 grid((unsigned)((outer + 32 * VEC - 1) / (32 * VEC)), (unsigned)chunks);
+  switch (act) {
+    case FV_ACT_RELU: k_act_grad<T, VEC, FV_ACT_RELU><<<grid, 256, 0, st>>>(dy, ldg, z, ldz, rows, outer, dz, pitch, part); break;
+    case FV_ACT_GELU: k_act_grad<T, VEC, FV_ACT_GELU><<<grid, 256, 0, st>>>(dy, ldg, z, ldz, rows, outer, dz, pitch, part); break;
+    case FV_ACT_GELU_TANH: k_act_grad<T, VEC, FV_ACT_GELU_TANH><<<grid, 256, 0, st>>>(dy, ldg, z, ldz, rows, outer, dz, pitch, part); break;
+    case FV_ACT_SILU: k_act_grad<T, VEC, FV_ACT_SILU><<<grid, 256, 0, st>>>(dy, ldg, z, ldz, rows, outer, dz, pitch, part); break;
+    default: k_act_grad<T, VEC, FV_ACT_NONE><<<grid, 256, 0, st>>>(dy, ldg, z, ldz, rows, outer, dz, pitch, part);
   }
 }
 template <typename T>
@@ -815,6 +957,25 @@ int make_map(CUtensorMap* map, const Operand& o, int dtype, int box_rows) {
   return FV_OK;
 }
 
+// An output [rows][cols], dense, as 128-byte wide boxes of 32 rows.
+int make_out_map(CUtensorMap* map, void* out, int64_t rows, int64_t cols, int dtype) {
+  const EncodeFn enc = encode_fn();
+  FV_REQUIRE(enc, FV_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
+  const size_t es = elem_size(dtype);
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)(cols * es)};
+  const cuuint32_t box[2] = {(cuuint32_t)(128 / es), 32};
+  const cuuint32_t one[2] = {1, 1};
+  const CUresult r = enc(map, dtype == FV_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                              : dtype == FV_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                         2, out, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  FV_REQUIRE(r == CUDA_SUCCESS, FV_ERR_CUDA, "cuTensorMapEncodeTiled failed with %d for an output [%lld][%lld]", (int)r, (long long)rows,
+             (long long)cols);
+  return FV_OK;
+}
+
 struct Shape {
   int bn, splits;
   bool pair;
@@ -845,7 +1006,7 @@ Shape choose_shape(int64_t m, int64_t n, int64_t kblocks, int sms, bool narrow) 
 }
 
 template <typename T, int BN, bool PAIR>
-int launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const GemmParams& p, unsigned grid, int splits, cudaStream_t st) {
+int launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& y, const GemmParams& p, unsigned grid, int splits, cudaStream_t st) {
   static bool ready[64] = {false};  // per device; setting it twice does no harm
   int device = 0;
   FV_CUDA(cudaGetDevice(&device));
@@ -864,7 +1025,7 @@ int launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const GemmParams& p,
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = PAIR || splits > 1 ? 1 : 0;
-  FV_CUDA(cudaLaunchKernelEx(&cfg, k_gemm<T, BN, PAIR>, a, b, p));
+  FV_CUDA(cudaLaunchKernelEx(&cfg, k_gemm<T, BN, PAIR>, a, b, y, p));
   return FV_OK;
 }
 
@@ -885,17 +1046,19 @@ int gemm(Operand a, Operand b, int dtype, GemmParams p, Workspace& ws, int sms, 
   p.b_mn = b.mn;
   const uint32_t type = dtype == FV_BF16 ? 1u : 0u;
   p.idesc = 1u << 4 | type << 7 | type << 10 | (uint32_t)a.mn << 15 | (uint32_t)b.mn << 16 | (uint32_t)(s.bn / 8) << 17 | (uint32_t)(rows / 16) << 24;
-  CUtensorMap ma, mb;
+  CUtensorMap ma, mb, my{};
+  if (!p.swap && s.splits == 1 && p.vec_y)
+    if (int rc = make_out_map(&my, p.y, p.m, p.n, p.out_f32 ? FV_F32 : dtype)) return rc;
   if (int rc = make_map(&ma, a, dtype, BM)) return rc;
   if (int rc = make_map(&mb, b, dtype, s.pair ? s.bn / 2 : s.bn)) return rc;
   const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
   const unsigned grid = (unsigned)(s.splits > 1 ? tiles * s.splits : std::min<int64_t>(tiles, s.pair ? sms / 2 : sms) * (s.pair ? 2 : 1));
   auto go = [&](auto tag) {
     using T = decltype(tag);
-    return s.pair        ? launch_gemm<T, 256, true>(ma, mb, p, grid, 1, st)
-           : s.bn == 256 ? launch_gemm<T, 256, false>(ma, mb, p, grid, s.splits, st)
-           : s.bn == 128 ? launch_gemm<T, 128, false>(ma, mb, p, grid, s.splits, st)
-                         : launch_gemm<T, 64, false>(ma, mb, p, grid, s.splits, st);
+    return s.pair        ? launch_gemm<T, 256, true>(ma, mb, my, p, grid, 1, st)
+           : s.bn == 256 ? launch_gemm<T, 256, false>(ma, mb, my, p, grid, s.splits, st)
+           : s.bn == 128 ? launch_gemm<T, 128, false>(ma, mb, my, p, grid, s.splits, st)
+                         : launch_gemm<T, 64, false>(ma, mb, my, p, grid, s.splits, st);
   };
   return dtype == FV_BF16 ? go(__nv_bfloat16{}) : go(__half{});
 }
@@ -1104,11 +1267,9 @@ int fv_linear_backward(int device, void* stream, const void* dy, int64_t dy_stri
     using T = decltype(tag);
     const T *pg = static_cast<const T*>(dy), *pz = static_cast<const T*>(z);
     if (vec)
-      k_act_grad<T, 8><<<dim3((unsigned)((outer + 255) / 256), (unsigned)chunks), 256, 0, st>>>(pg, dy_stride, pz, z_stride, rows, outer, act,
-                                                                                               static_cast<T*>(dz), pitch, part);
+      launch_act_grad<T, 8>(st, pg, dy_stride, pz, z_stride, rows, outer, act, static_cast<T*>(dz), pitch, part, chunks);
     else
-      k_act_grad<T, 1><<<dim3((unsigned)((outer + 31) / 32), (unsigned)chunks), 256, 0, st>>>(pg, dy_stride, pz, z_stride, rows, outer, act,
-                                                                                             static_cast<T*>(dz), pitch, part);
+      launch_act_grad<T, 1>(st, pg, dy_stride, pz, z_stride, rows, outer, act, static_cast<T*>(dz), pitch, part, chunks);
     k_col_sum<T><<<(unsigned)((outer + 31) / 32), dim3(32, 16), 0, st>>>(part, chunks, outer, static_cast<T*>(db));
   };
   if (dtype == FV_BF16) first(__nv_bfloat16{});

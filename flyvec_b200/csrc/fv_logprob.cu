@@ -42,18 +42,6 @@ constexpr float LN2 = 0.6931471805599453f;
 
 typedef unsigned long long u64;
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-// maximum that keeps a NaN
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float y;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
-  return y;
-}
-
 // Order of the elements as unsigned integers: NaN above +inf, -0 equal to +0, 0 below everything.
 __device__ __forceinline__ unsigned key_of(float x) {
   if (x != x) return 0xffffffffu;
@@ -95,23 +83,6 @@ struct Stream {
   float m;
   float2 s, a;
 };
-__device__ __forceinline__ u64 pack2(float2 v) { return *reinterpret_cast<u64*>(&v); }
-__device__ __forceinline__ float2 unpack2(u64 v) { return *reinterpret_cast<float2*>(&v); }
-__device__ __forceinline__ float2 add2(float2 x, float2 y) {
-  u64 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pack2(x)), "l"(pack2(y)));
-  return unpack2(r);
-}
-__device__ __forceinline__ float2 mul2(float2 x, float2 y) {
-  u64 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pack2(x)), "l"(pack2(y)));
-  return unpack2(r);
-}
-__device__ __forceinline__ float2 fma2(float2 x, float2 y, float2 z) {
-  u64 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pack2(x)), "l"(pack2(y)), "l"(pack2(z)));
-  return unpack2(r);
-}
 // two elements of a 32-bit word (one element for float: the caller passes two words)
 template <typename T>
 __device__ __forceinline__ float2 widen2(unsigned w);

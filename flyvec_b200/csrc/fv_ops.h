@@ -75,6 +75,48 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
+// ---- single instructions ----
+__device__ __forceinline__ float ex2(float x) {  // 2^x, to 2^-22; results below 2^-126 are 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp(float x) {  // 1 / x, to 2^-23
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// larger and smaller of two, a NaN if either is one
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float y;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+// two float operations at a time
+__device__ __forceinline__ unsigned long long pack2(float2 v) { return *reinterpret_cast<unsigned long long*>(&v); }
+__device__ __forceinline__ float2 unpack2(unsigned long long v) { return *reinterpret_cast<float2*>(&v); }
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 add2(float2 x, float2 y) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pack2(x)), "l"(pack2(y)));
+  return unpack2(r);
+}
+__device__ __forceinline__ float2 mul2(float2 x, float2 y) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(pack2(x)), "l"(pack2(y)));
+  return unpack2(r);
+}
+__device__ __forceinline__ float2 fma2(float2 x, float2 y, float2 z) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(pack2(x)), "l"(pack2(y)), "l"(pack2(z)));
+  return unpack2(r);
+}
+
 // Bytes that divide an address and a stride: which vector width a row-major array admits.
 inline unsigned common_alignment(uintptr_t a) { return a == 0 ? 4096u : (unsigned)(a & (~a + 1)); }
 inline bool vec_ok(const void* p, int64_t stride_elems, size_t elem, unsigned bytes) {
