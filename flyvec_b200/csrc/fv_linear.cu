@@ -873,18 +873,7 @@ void launch_act_grad(cudaStream_t st, const T* dy, int64_t ldg, const T* z, int6
 }
 template <typename T>
 __global__ void __launch_bounds__(512) k_col_sum(const float* __restrict__ part, int64_t P, int64_t n, T* __restrict__ out) {
-  __shared__ float sum[16][33];
-  const int64_t c = (int64_t)blockIdx.x * 32 + threadIdx.x;
-  float s = 0.f;
-  if (c < n)
-    for (int64_t q = threadIdx.y; q < P; q += 16) s += part[q * n + c];
-  sum[threadIdx.y][threadIdx.x] = s;
-  __syncthreads();
-  if (threadIdx.y == 0 && c < n) {
-#pragma unroll
-    for (int k = 1; k < 16; ++k) s += sum[k][threadIdx.x];
-    out[c] = from_f<T>(s);
-  }
+  column_sums(part, P, n, [&](int64_t c, float v) { out[c] = from_f<T>(v); });
 }
 
 // ---- host side --------------------------------------------------------------------------------------
@@ -1126,6 +1115,9 @@ int fv_ops_status(int device, uint32_t* word) {
     const uint32_t zero = 0;
     FV_CUDA(cudaMemcpyToSymbol(g_status, &zero, sizeof(zero)));
   }
+  uint32_t more = 0;
+  FV_CUDA(norm_status(&more));
+  *word |= more;
   return FV_OK;
 }
 
@@ -1270,7 +1262,7 @@ int fv_linear_backward(int device, void* stream, const void* dy, int64_t dy_stri
       launch_act_grad<T, 8>(st, pg, dy_stride, pz, z_stride, rows, outer, act, static_cast<T*>(dz), pitch, part, chunks);
     else
       launch_act_grad<T, 1>(st, pg, dy_stride, pz, z_stride, rows, outer, act, static_cast<T*>(dz), pitch, part, chunks);
-    k_col_sum<T><<<(unsigned)((outer + 31) / 32), dim3(32, 16), 0, st>>>(part, chunks, outer, static_cast<T*>(db));
+    k_col_sum<T><<<(unsigned)((outer + 31) / 32), 512, 0, st>>>(part, chunks, outer, static_cast<T*>(db));
   };
   if (dtype == FV_BF16) first(__nv_bfloat16{});
   else first(__half{});

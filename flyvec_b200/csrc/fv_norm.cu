@@ -4,16 +4,22 @@
 //   backward  h = (x - mean) rstd, u = dy w:
 //             dx = rstd (u - sum u / D - h sum (u h) / D)      dw = sum_rows dy h      db = sum_rows dy
 //
-// Both passes are bound by memory: each row is read once, kept in registers while its sums are formed, and
-// written once.  A row of up to 1024 elements belongs to one warp (no barrier), a longer one to a block of up
-// to 512 threads with 8, 16 or 32 elements each; rows beyond 16384 elements (8192 for the float gradient,
-// whose accumulators would spill) are read again from L2 instead of being held.  All sums are float; the variance
-// is formed from the centred values, so a large common offset does not cancel it.
+// Both passes are bound by memory: a row is read once and written once.  A group of threads (a warp for short rows, a
+// block for longer ones) walks over rows; bulk asynchronous copies bring the next rows into a ring in shared memory
+// while it works on one, so that the loads never wait for the reductions.  All sums are float.  The variance is formed
+// together with the mean, in one pass about a pivot (the mean of eight of the row's elements), so that a large common
+// offset does not cancel it; should the pivot lie more than a standard deviation from the mean (where at most one bit is
+// lost) the row is summed again about the mean.
 //
-// The weight's and the bias's gradients are sums over rows.  Each thread of the backward kernel owns the same
-// columns in every row its block visits, so it keeps their running sums in registers; a block leaves one
-// partial row in the workspace and a second kernel adds the partials in a fixed order (no atomics: the same
-// inputs give the same bits).
+// Rows need not start on 16-byte boundaries: the copies take whole 16-byte words around a row, and a thread's columns
+// are aligned to the words, not to the row's start.  A group's rows are a multiple of 8 apart, so all of them start
+// at the same place in a word and a thread's columns, its weights and its gradient sums stay the same.  Only where dy
+// or the output starts at another place in a word than x is that array accessed element by element.
+//
+// The weight's and the bias's gradients are sums over rows.  A thread keeps the running sums of its columns in
+// registers; a block leaves one partial row in the workspace and a second kernel adds the partials in a fixed order (no
+// atomics: the same inputs give the same bits).  Rows of more than 32 KB (64 KB in the float forward pass) are read
+// again from L2 instead of being held.
 #include <algorithm>
 
 #include "fv_ops.h"
@@ -52,17 +58,25 @@ __device__ __forceinline__ float2 group_sum2(float a, float b, float (*red)[2], 
       red[threadIdx.x >> 5][1] = b;
     }
     __syncthreads();
-    a = lane < nwarps ? red[lane][0] : 0.f;
-    b = lane < nwarps ? red[lane][1] : 0.f;
-#pragma unroll
-    for (int o = 8; o; o >>= 1) {
-      a += __shfl_xor_sync(FULL, a, o);
-      b += __shfl_xor_sync(FULL, b, o);
+    // every thread adds the warps' sums in the same order: two per load, no shuffles
+    const float4* all = reinterpret_cast<const float4*>(red);
+    a = b = 0.f;
+    for (int k = 0; k < (nwarps + 1) / 2; ++k) {
+      const float4 f = all[k];
+      a += f.x;
+      b += f.y;
+      if (2 * k + 1 < nwarps) {
+        a += f.z;
+        b += f.w;
+      }
     }
-    a = __shfl_sync(FULL, a, 0);
-    b = __shfl_sync(FULL, b, 0);
   }
   return make_float2(a, b);
+}
+
+template <bool BLOCK>
+__device__ __forceinline__ float group_sum(float a, float (*red)[2], int nwarps) {
+  return group_sum2<BLOCK>(a, 0.f, red, nwarps).x;
 }
 
 template <int VEC>
@@ -88,67 +102,227 @@ __device__ __forceinline__ void store_as(void* p, int dtype, int64_t at, const f
     store_pack<__half, VEC>(static_cast<__half*>(p) + at, o);
   }
 }
+__device__ __forceinline__ void store_one(void* p, int dtype, int64_t at, float v) {
+  const float one[1] = {v};
+  store_as<1>(p, dtype, at, one);
+}
 
-// y in the type `ydt`; VEC elements per access, NV accesses per thread.
-template <typename T, int VEC, int NV, bool BLOCK>
+// ---- the ring -----------------------------------------------------------------------------------------
+__device__ unsigned g_norm_status = 0;
+
+constexpr int RING_MOST = 8;  // stages at most
+// Rows as they come into shared memory: `arrays` rows to a stage, each in `pitch` bytes, starting at the row's place in its
+// first 16-byte word.
+struct Ring {
+  unsigned char* base;
+  uint64_t* bars;
+  int stages, pitch;
+};
+__device__ __forceinline__ uint32_t shared_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void ring_copy(unsigned char* dst, const void* row, int bytes, uint64_t* bar) {
+  const uintptr_t from = (uintptr_t)row & ~(uintptr_t)15, to = ((uintptr_t)row + bytes + 15) & ~(uintptr_t)15;
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(shared_addr(dst)), "l"(from),
+               "r"((uint32_t)(to - from)), "r"(shared_addr(bar))
+               : "memory");
+}
+__device__ __forceinline__ uint32_t ring_bytes(const void* row, int bytes) {
+  return (uint32_t)((((uintptr_t)row + bytes + 15) & ~(uintptr_t)15) - ((uintptr_t)row & ~(uintptr_t)15));
+}
+__device__ __forceinline__ void ring_expect(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(shared_addr(bar)), "r"(bytes) : "memory");
+}
+// Bounded wait for a stage; false when the copies did not arrive (about two seconds).
+__device__ __forceinline__ bool ring_wait(uint64_t* bar, int parity) {
+  long long t0 = 0;
+  for (;;) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(shared_addr(bar)), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    const long long now = clock64();
+    if (t0 == 0) t0 = now;
+    if (now - t0 > 4000000000ll) {
+      atomicOr(&g_norm_status, 1u);
+      return false;
+    }
+  }
+}
+// A group's place: its threads, its first row and the distance to its next.
+template <bool BLOCK>
+struct Group {
+  int size, t, warps;
+  int64_t first, step;
+  __device__ Group() {
+    size = BLOCK ? blockDim.x : 32;
+    t = BLOCK ? threadIdx.x : threadIdx.x & 31;
+    warps = BLOCK ? blockDim.x >> 5 : 1;
+    first = BLOCK ? blockIdx.x : (int64_t)blockIdx.x * NORM_WARPS + (threadIdx.x >> 5);
+    step = (int64_t)gridDim.x * (BLOCK ? 1 : NORM_WARPS);
+  }
+};
+template <bool BLOCK>
+__device__ __forceinline__ Ring make_ring(unsigned char* smem, int stages, int pitch, int arrays, int t) {
+  Ring r;
+  const int w = BLOCK ? 0 : threadIdx.x >> 5;
+  r.bars = reinterpret_cast<uint64_t*>(smem) + w * RING_MOST;
+  r.base = smem + (BLOCK ? 1 : NORM_WARPS) * RING_MOST * 8 + (size_t)w * stages * pitch * arrays;
+  r.stages = stages;
+  r.pitch = pitch;
+  if (t == 0) {
+    for (int s = 0; s < stages; ++s) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_addr(r.bars + s)) : "memory");
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (BLOCK)
+    __syncthreads();
+  else
+    __syncwarp();
+  return r;
+}
+
+// A thread's columns: NV words of VEC elements, word t + j size of the row's words; `off` elements of the first word
+// precede the row.
+template <int VEC, int NV>
+struct Columns {
+  int off, D, t, size;
+  __device__ __forceinline__ int at(int j) const { return (t + j * size) * VEC - off; }  // column of the word's first element
+  __device__ __forceinline__ bool any(int j) const { return at(j) < D; }
+  __device__ __forceinline__ bool whole(int j) const { return at(j) >= 0 && at(j) + VEC <= D; }
+  __device__ __forceinline__ bool has(int j, int i) const { return (unsigned)(at(j) + i) < (unsigned)D; }
+};
+// a vector of D elements at a thread's columns, as pairs of floats; `none` outside or without a vector
+template <typename T, int VEC, int NV>
+__device__ __forceinline__ void load_columns(const Columns<VEC, NV>& c, const T* v, float none, float2 (&out)[NV][VEC / 2]) {
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) {
+      out[j][i].x = v && c.has(j, 2 * i) ? to_f<T>(v[c.at(j) + 2 * i]) : none;
+      out[j][i].y = v && c.has(j, 2 * i + 1) ? to_f<T>(v[c.at(j) + 2 * i + 1]) : none;
+    }
+}
+// the words a thread holds of a row in shared memory; `none` in place of what lies outside the row
+template <typename T, int VEC, int NV, bool EDGE>
+__device__ __forceinline__ void word_pairs(const Columns<VEC, NV>& c, int j, const Pack<T, VEC>& p, float none, float2 (&out)[VEC / 2]) {
+#pragma unroll
+  for (int i = 0; i < VEC / 2; ++i) {
+    out[i] = make_float2(to_f<T>(p.e[2 * i]), to_f<T>(p.e[2 * i + 1]));
+    if (EDGE) {
+      if (!c.has(j, 2 * i)) out[i].x = none;
+      if (!c.has(j, 2 * i + 1)) out[i].y = none;
+    }
+  }
+}
+
+// y in the type `ydt`; EDGE: a row's first or last word may be partial.
+template <typename T, int NV, bool BLOCK, bool EDGE>
 __global__ void __launch_bounds__(BLOCK ? NORM_MAX_THREADS : 32 * NORM_WARPS)
     k_norm(const T* __restrict__ x, int64_t xs, int64_t rows, int D, const T* __restrict__ w, const T* __restrict__ b, float eps,
-           void* __restrict__ y, int ydt, float* __restrict__ mean_out, float* __restrict__ rstd_out) {
-  __shared__ float red[2][16][2];
-  const int G = BLOCK ? blockDim.x : 32, t = BLOCK ? threadIdx.x : threadIdx.x & 31, nw = BLOCK ? blockDim.x >> 5 : 1;
-  const int64_t per = BLOCK ? 1 : NORM_WARPS, first = BLOCK ? blockIdx.x : (int64_t)blockIdx.x * NORM_WARPS + (threadIdx.x >> 5);
-  const float n = (float)D;
-  for (int64_t r = first; r < rows; r += (int64_t)gridDim.x * per) {
-    const T* xr = x + r * xs;
-    float v[NV][VEC];
-    float s = 0.f;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = (t + j * G) * VEC;
-      if (c < D) {
-        const Pack<T, VEC> p = load_pack_stream<T, VEC>(xr + c);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          v[j][i] = to_f<T>(p.e[i]);
-          s += v[j][i];
-        }
-      }
+           void* __restrict__ y, int ydt, float* __restrict__ mean_out, float* __restrict__ rstd_out, int stages, int pitch) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ __align__(16) float red[2][16][2];
+  const Group<BLOCK> g;
+  const Ring ring = make_ring<BLOCK>(smem, stages, pitch, 1, g.t);
+  const int bytes = D * (int)sizeof(T);
+  auto fetch = [&](int64_t r, int s) {
+    if (r < rows) {
+      const T* row = x + r * xs;
+      ring_expect(ring.bars + s, ring_bytes(row, bytes));
+      ring_copy(ring.base + (size_t)s * pitch, row, bytes, ring.bars + s);
     }
-    const float mean = group_sum2<BLOCK>(s, 0.f, red[0], nw).x / n;
-    float q = 0.f;
+  };
+  if (g.t == 0)
+    for (int s = 0; s < stages; ++s) fetch(g.first + s * g.step, s);
+  const int off = EDGE ? (int)(((uintptr_t)(x + g.first * xs) & 15) / sizeof(T)) : 0;
+  const Columns<VEC, NV> col{off, D, g.t, g.size};
+  int turn = 0;
+  float2 pw[NV][VEC / 2], pb[NV][VEC / 2];
+  load_columns(col, w, 1.f, pw);
+  load_columns(col, b, 0.f, pb);
+  const int yes = ydt == FV_F32 ? 4 : 2;
+  const float inv_n = 1.0f / (float)D;
+  // where the words of the group's first row go; the next row's are `hop` further
+  unsigned char* out = static_cast<unsigned char*>(y) + (g.first * D + col.at(0)) * yes;
+  const int64_t hop = g.step * D * yes;
+  const bool aligned = !EDGE || ((uintptr_t)y + (uintptr_t)(g.first * D - off) * yes) % (VEC * yes < 16 ? VEC * yes : 16) == 0;
+  // The pivot: mean of a word, or the first element of a row that has no whole word
+  const bool wide = !EDGE || D >= 2 * VEC;
+  const int pivot_at = EDGE ? (wide ? VEC : off) : 0;
+  int s = 0, parity = 0;
+  for (int64_t r = g.first; r < rows; r += g.step, out += hop) {
+    if (!ring_wait(ring.bars + s, parity)) break;
+    const T* stage = reinterpret_cast<const T*>(ring.base + (size_t)s * pitch);
+    float pivot;
+    if (wide) {
+      const Pack<T, VEC> p = load_pack<T, VEC>(stage + pivot_at);
+      float h[VEC];
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-      if ((t + j * G) * VEC < D) {
+      for (int i = 0; i < VEC; ++i) h[i] = to_f<T>(p.e[i]);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          v[j][i] -= mean;
-          q = fmaf(v[j][i], v[j][i], q);
+      for (int k = VEC / 2; k; k /= 2)
+#pragma unroll
+        for (int i = 0; i < k; ++i) h[i] += h[i + k];
+      pivot = h[0] * (1.0f / VEC);
+    } else {
+      pivot = to_f<T>(stage[pivot_at]);
+    }
+    float2 v[NV][VEC / 2];
+    float shift, var;
+    for (bool again = false;; again = true) {
+      float2 sum = both(0.f), q = both(0.f);
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (col.any(j)) {
+          word_pairs<T, VEC, NV, EDGE>(col, j, load_pack<T, VEC>(stage + (g.t + j * g.size) * VEC), pivot, v[j]);
+#pragma unroll
+          for (int i = 0; i < VEC / 2; ++i) {
+            v[j][i] = add2(v[j][i], both(-pivot));
+            sum = add2(sum, v[j][i]);
+            q = fma2(v[j][i], v[j][i], q);
+          }
         }
-      }
-    const float rstd = 1.0f / sqrtf(group_sum2<BLOCK>(q, 0.f, red[1], nw).x / n + eps);
-    if (t == 0) {
-      if (mean_out) mean_out[r] = mean;
+      const float2 sums = group_sum2<BLOCK>(sum.x + sum.y, q.x + q.y, red[turn], g.warps);
+      turn ^= 1;
+      shift = sums.x * inv_n;
+      var = fmaf(-shift, shift, sums.y * inv_n);
+      if (again || !(shift * shift > var)) break;
+      pivot += shift;  // it lay far out: again about the mean
+    }
+    if (!BLOCK) __syncwarp();
+    if (g.t == 0) fetch(r + stages * g.step, s);  // every thread has its part of the stage in registers
+    const float rstd = rsqrtf(var + eps), minus = -shift * rstd;
+    if (g.t == 0) {
+      if (mean_out) mean_out[r] = pivot + shift;
       if (rstd_out) rstd_out[r] = rstd;
     }
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = (t + j * G) * VEC;
-      if (c < D) {
+    for (int j = 0; j < NV; ++j)
+      if (col.any(j)) {
         float o[VEC];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) o[i] = v[j][i] * rstd;
-        if (w) {
-          const Pack<T, VEC> pw = load_pack<T, VEC>(w + c);
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) o[i] *= to_f<T>(pw.e[i]);
+        for (int i = 0; i < VEC / 2; ++i) {
+          const float2 u = fma2(fma2(v[j][i], both(rstd), both(minus)), pw[j][i], pb[j][i]);
+          o[2 * i] = u.x;
+          o[2 * i + 1] = u.y;
         }
-        if (b) {
-          const Pack<T, VEC> pb = load_pack<T, VEC>(b + c);
+        unsigned char* to = out + j * g.size * VEC * yes;
+        if (!EDGE || (aligned && col.whole(j))) {
+          store_as<VEC>(to, ydt, 0, o);
+        } else {
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) o[i] += to_f<T>(pb.e[i]);
+          for (int i = 0; i < VEC; ++i)
+            if (col.has(j, i)) store_one(to, ydt, i, o[i]);
         }
-        store_as<VEC>(y, ydt, r * (int64_t)D + c, o);
       }
+    if (++s == stages) {
+      s = 0;
+      parity ^= 1;
     }
   }
 }
@@ -158,19 +332,19 @@ template <typename T>
 __global__ void __launch_bounds__(NORM_MAX_THREADS)
     k_norm_long(const T* __restrict__ x, int64_t xs, int64_t rows, int64_t D, const T* __restrict__ w, const T* __restrict__ b,
                 float eps, void* __restrict__ y, int ydt, float* __restrict__ mean_out, float* __restrict__ rstd_out) {
-  __shared__ float red[2][16][2];
+  __shared__ __align__(16) float red[2][16][2];
   const int nw = blockDim.x >> 5;
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const T* xr = x + r * xs;
     float s = 0.f;
     for (int64_t c = threadIdx.x; c < D; c += blockDim.x) s += to_f<T>(xr[c]);
-    const float mean = group_sum2<true>(s, 0.f, red[0], nw).x / (float)D;
+    const float mean = group_sum<true>(s, red[0], nw) / (float)D;
     float q = 0.f;
     for (int64_t c = threadIdx.x; c < D; c += blockDim.x) {
       const float d = to_f<T>(xr[c]) - mean;
       q = fmaf(d, d, q);
     }
-    const float rstd = 1.0f / sqrtf(group_sum2<true>(q, 0.f, red[1], nw).x / (float)D + eps);
+    const float rstd = 1.0f / sqrtf(group_sum<true>(q, red[1], nw) / (float)D + eps);
     if (threadIdx.x == 0) {
       if (mean_out) mean_out[r] = mean;
       if (rstd_out) rstd_out[r] = rstd;
@@ -185,106 +359,148 @@ __global__ void __launch_bounds__(NORM_MAX_THREADS)
 }
 
 // dx, and with a weight the block's partial sums of dw and db in part[blockIdx.x][2][D].
-template <typename T, int VEC, int NV, bool BLOCK>
+template <typename T, int NV, bool BLOCK, bool EDGE>
 __global__ void __launch_bounds__(BLOCK ? NORM_MAX_THREADS : 32 * NORM_WARPS)
     k_norm_grad(const T* __restrict__ dy, int64_t gs, const T* __restrict__ x, int64_t xs, int64_t rows, int D,
                 const float* __restrict__ mean, const float* __restrict__ rstd, const T* __restrict__ w, T* __restrict__ dx,
-                float* __restrict__ part) {
-  __shared__ float red[2][16][2];
-  __shared__ float cols[BLOCK ? 1 : 2 * 32 * NV * VEC];
-  const int G = BLOCK ? blockDim.x : 32, t = BLOCK ? threadIdx.x : threadIdx.x & 31, nw = BLOCK ? blockDim.x >> 5 : 1;
-  const int64_t per = BLOCK ? 1 : NORM_WARPS, first = BLOCK ? blockIdx.x : (int64_t)blockIdx.x * NORM_WARPS + (threadIdx.x >> 5);
-  const int64_t step = (int64_t)gridDim.x * per;
-  const float n = (float)D;
-  float dw[NV][VEC], db[NV][VEC];
+                float* __restrict__ part, int stages, int pitch) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ __align__(16) float red[2][16][2];
+  const Group<BLOCK> g;
+  const Ring ring = make_ring<BLOCK>(smem, stages, pitch, 2, g.t);
+  const int bytes = D * (int)sizeof(T);
+  auto fetch = [&](int64_t r, int s) {
+    if (r < rows) {
+      const T *xr = x + r * xs, *gr = dy + r * gs;
+      unsigned char* to = ring.base + (size_t)s * 2 * pitch;
+      ring_expect(ring.bars + s, ring_bytes(xr, bytes) + ring_bytes(gr, bytes));
+      ring_copy(to, xr, bytes, ring.bars + s);
+      ring_copy(to + pitch, gr, bytes, ring.bars + s);
+    }
+  };
+  if (g.t == 0)
+    for (int s = 0; s < stages; ++s) fetch(g.first + s * g.step, s);
+  const int off = EDGE ? (int)(((uintptr_t)(x + g.first * xs) & 15) / sizeof(T)) : 0;
+  const int goff = EDGE ? (int)(((uintptr_t)(dy + g.first * gs) & 15) / sizeof(T)) : 0;
+  const Columns<VEC, NV> col{off, D, g.t, g.size};
+  float2 pw[NV][VEC / 2];
+  load_columns(col, w, 1.f, pw);
+  const float inv_n = 1.0f / (float)D;
+  T* out_row = dx + g.first * D + col.at(0);
+  const int64_t hop = g.step * D;
+  const bool aligned = !EDGE || (uintptr_t)(dx + g.first * D - off) % 16 == 0;
+  float2 dw[NV][VEC / 2], db[NV][VEC / 2];
 #pragma unroll
   for (int j = 0; j < NV; ++j)
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) dw[j][i] = db[j][i] = 0.f;
-  Pack<T, VEC> px[NV], pg[NV];
-  auto fetch = [&](int64_t r) {
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = (t + j * G) * VEC;
-      if (c < D) {
-        px[j] = load_pack_stream<T, VEC>(x + r * xs + c);
-        pg[j] = load_pack_stream<T, VEC>(dy + r * gs + c);
-      }
+    for (int i = 0; i < VEC / 2; ++i) dw[j][i] = db[j][i] = both(0.f);
+  int s = 0, parity = 0, turn = 0;
+  float next_mu = 0.f, next_rs = 0.f;
+  if (g.first < rows) {
+    next_mu = mean[g.first];
+    next_rs = rstd[g.first];
+  }
+  for (int64_t r = g.first; r < rows; r += g.step, turn ^= 1, out_row += hop) {
+    const float mu = next_mu, rs = next_rs;
+    if (r + g.step < rows) {
+      next_mu = mean[r + g.step];
+      next_rs = rstd[r + g.step];
     }
-  };
-  if (first < rows) fetch(first);
-  int turn = 0;
-  for (int64_t r = first; r < rows; r += step, turn ^= 1) {
-    const float mu = mean[r], rs = rstd[r];
-    float a = 0.f, q = 0.f;
+    if (!ring_wait(ring.bars + s, parity)) break;
+    const T* sx = reinterpret_cast<const T*>(ring.base + (size_t)s * 2 * pitch);
+    const T* sg = reinterpret_cast<const T*>(ring.base + (size_t)s * 2 * pitch + pitch);
+    // h and dy of word j, 0 outside the row
+    auto row_values = [&](int j, float2 (&h)[VEC / 2], float2 (&gv)[VEC / 2]) {
+      word_pairs<T, VEC, NV, EDGE>(col, j, load_pack<T, VEC>(sx + (g.t + j * g.size) * VEC), mu, h);
+      Pack<T, VEC> q;
+      if (!EDGE || goff == off) {
+        q = load_pack<T, VEC>(sg + (g.t + j * g.size) * VEC);
+      } else {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = (t + j * G) * VEC;
-      if (c < D) {
-        Pack<T, VEC> pw;
-        if (w) pw = load_pack<T, VEC>(w + c);
+        for (int i = 0; i < VEC; ++i) q.e[i] = col.has(j, i) ? sg[goff + col.at(j) + i] : from_f<T>(0.f);
+      }
+      word_pairs<T, VEC, NV, EDGE>(col, j, q, 0.f, gv);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float g = to_f<T>(pg[j].e[i]), h = (to_f<T>(px[j].e[i]) - mu) * rs;
-          const float u = w ? g * to_f<T>(pw.e[i]) : g;
-          a += u;
-          q = fmaf(u, h, q);
-          dw[j][i] = fmaf(g, h, dw[j][i]);
-          db[j][i] += g;
+      for (int i = 0; i < VEC / 2; ++i) h[i] = mul2(add2(h[i], both(-mu)), both(rs));
+    };
+    float2 a = both(0.f), q = both(0.f);
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if (col.any(j)) {
+        float2 h[VEC / 2], gv[VEC / 2];
+        row_values(j, h, gv);
+#pragma unroll
+        for (int i = 0; i < VEC / 2; ++i) {
+          const float2 u = mul2(gv[i], pw[j][i]);
+          a = add2(a, u);
+          q = fma2(u, h[i], q);
+          dw[j][i] = fma2(gv[i], h[i], dw[j][i]);
+          db[j][i] = add2(db[j][i], gv[i]);
         }
       }
-    }
-    const float2 sums = group_sum2<BLOCK>(a, q, red[turn], nw);
-    const float ma = sums.x / n, mq = sums.y / n;
+    const float2 sums = group_sum2<BLOCK>(a.x + a.y, q.x + q.y, red[turn], g.warps);
+    if (!BLOCK) __syncwarp();
+    // all threads are past the row before this one: its stage is free
+    if (g.t == 0 && r != g.first) fetch(r + (stages - 1) * g.step, s == 0 ? stages - 1 : s - 1);
+    const float ma = sums.x * inv_n, mq = sums.y * inv_n;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = (t + j * G) * VEC;
-      if (c < D) {
-        Pack<T, VEC> pw, o;
-        if (w) pw = load_pack<T, VEC>(w + c);
+    for (int j = 0; j < NV; ++j)
+      if (col.any(j)) {
+        float2 h[VEC / 2], gv[VEC / 2];
+        row_values(j, h, gv);
+        Pack<T, VEC> o;
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float g = to_f<T>(pg[j].e[i]), h = (to_f<T>(px[j].e[i]) - mu) * rs;
-          const float u = w ? g * to_f<T>(pw.e[i]) : g;
-          o.e[i] = from_f<T>(rs * (u - ma - h * mq));
+        for (int i = 0; i < VEC / 2; ++i) {
+          const float2 d = mul2(both(rs), fma2(h[i], both(-mq), add2(mul2(gv[i], pw[j][i]), both(-ma))));
+          o.e[2 * i] = from_f<T>(d.x);
+          o.e[2 * i + 1] = from_f<T>(d.y);
         }
-        store_pack<T, VEC>(dx + r * (int64_t)D + c, o);
+        T* to = out_row + j * g.size * VEC;
+        if (!EDGE || (aligned && col.whole(j))) {
+          store_pack<T, VEC>(to, o);
+        } else {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i)
+            if (col.has(j, i)) to[i] = o.e[i];
+        }
       }
+    if (++s == stages) {
+      s = 0;
+      parity ^= 1;
     }
-    if (r + step < rows) fetch(r + step);
   }
   if (!part) return;
   float* out = part + (int64_t)blockIdx.x * 2 * D;
   if (BLOCK) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = (t + j * G) * VEC;
-      if (c < D) {
+    for (int j = 0; j < NV; ++j)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          out[c + i] = dw[j][i];
-          out[D + c + i] = db[j][i];
+      for (int i = 0; i < VEC; ++i)
+        if (col.has(j, i)) {
+          out[col.at(j) + i] = i & 1 ? dw[j][i / 2].y : dw[j][i / 2].x;
+          out[D + col.at(j) + i] = i & 1 ? db[j][i / 2].y : db[j][i / 2].x;
         }
-      }
-    }
-  } else {  // the block's warps one after the other, a fixed order
-    constexpr int W = 32 * NV * VEC;
+  } else {  // the block's warps one after the other, a fixed order; their copies have all arrived
+    float* cols = reinterpret_cast<float*>(smem + NORM_WARPS * RING_MOST * 8);
     for (int k = 0; k < NORM_WARPS; ++k) {
+      __syncthreads();
       if ((threadIdx.x >> 5) == k) {
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            const int c = (t + j * G) * VEC + i;
-            cols[c] = (k ? cols[c] : 0.f) + dw[j][i];
-            cols[W + c] = (k ? cols[W + c] : 0.f) + db[j][i];
-          }
+          for (int i = 0; i < VEC; ++i)
+            if (col.has(j, i)) {
+              const int c = col.at(j) + i;
+              cols[c] = (k ? cols[c] : 0.f) + (i & 1 ? dw[j][i / 2].y : dw[j][i / 2].x);
+              cols[D + c] = (k ? cols[D + c] : 0.f) + (i & 1 ? db[j][i / 2].y : db[j][i / 2].x);
+            }
       }
-      __syncthreads();
     }
+    __syncthreads();
     for (int c = threadIdx.x; c < D; c += blockDim.x) {
       out[c] = cols[c];
-      out[D + c] = cols[W + c];
+      out[D + c] = cols[D + c];
     }
   }
 }
@@ -294,7 +510,7 @@ template <typename T>
 __global__ void __launch_bounds__(NORM_MAX_THREADS)
     k_norm_grad_long(const T* __restrict__ dy, int64_t gs, const T* __restrict__ x, int64_t xs, int64_t rows, int64_t D,
                      const float* __restrict__ mean, const float* __restrict__ rstd, const T* __restrict__ w, T* __restrict__ dx) {
-  __shared__ float red[2][16][2];
+  __shared__ __align__(16) float red[2][16][2];
   const int nw = blockDim.x >> 5;
   int turn = 0;
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x, turn ^= 1) {
@@ -330,91 +546,109 @@ __global__ void __launch_bounds__(256)
   part[(int64_t)blockIdx.y * 2 * D + D + c] = db;
 }
 
-// out[c] = sum of part[p][c] over p in a fixed order; c runs over dw's and then db's columns.
+// out[c] = sum of part[p][c] over p in a fixed order; c runs over dw's and then db's columns.  A block takes 32 columns, four
+// to a thread, and 64 partial rows at a time.
 template <typename T>
 __global__ void __launch_bounds__(512)
     k_norm_grad_reduce(const float* __restrict__ part, int64_t P, int64_t D, T* __restrict__ dw, T* __restrict__ db) {
-  __shared__ float sum[16][33];
-  const int64_t c = (int64_t)blockIdx.x * 32 + threadIdx.x;
-  float s = 0.f;
-  if (c < 2 * D)
-    for (int64_t p = threadIdx.y; p < P; p += 16) s += part[p * 2 * D + c];
-  sum[threadIdx.y][threadIdx.x] = s;
-  __syncthreads();
-  if (threadIdx.y == 0 && c < 2 * D) {
-#pragma unroll
-    for (int k = 1; k < 16; ++k) s += sum[k][threadIdx.x];
+  column_sums(part, P, 2 * D, [&](int64_t c, float v) {
     if (c < D)
-      dw[c] = from_f<T>(s);
+      dw[c] = from_f<T>(v);
     else
-      db[c - D] = from_f<T>(s);
-  }
+      db[c - D] = from_f<T>(v);
+  });
 }
 
 struct NormPlan {
-  bool is_long, block;
-  int vec_bytes;   // width of one access
-  int elems;       // elements per thread: 8, 16 or 32
-  int threads;
+  bool is_long, block, edge;
+  int words;           // 16-byte words per thread: 1, 2, 4 or 8
+  int threads, stages, pitch;
   int64_t grid;
+  size_t smem;
 };
 
-// One warp per row while a row fits one (32 elements a lane at most) and there are rows enough to fill the
-// GPU with warps; else one block per row.
-NormPlan plan_norm(int64_t rows, int64_t D, int dtype, bool grad, int vec_bytes, int sms) {
+// One warp per row while a row fits one (64 bytes a lane at most) and there are rows enough to fill the GPU with warps; else
+// one block per row.  Threads hold one or two words each as long as 512 threads suffice.  The ring takes what shared memory
+// leaves to the blocks that run side by side.
+NormPlan plan_norm(int64_t rows, int64_t D, int dtype, bool grad, bool edge, int sms) {
   NormPlan p{};
-  const int64_t most = grad && dtype == FV_F32 ? 8192 : 16384;
-  p.is_long = D > most;
-  p.vec_bytes = vec_bytes;
+  const int64_t es = (int64_t)elem_size(dtype), bytes = D * es;
+  const int64_t words = (bytes + 15) / 16 + (edge ? 1 : 0);
+  p.edge = edge;
+  p.is_long = words > (!grad && dtype == FV_F32 ? 8 : 4) * NORM_MAX_THREADS;
   if (p.is_long) {
     p.block = true;
     p.threads = NORM_MAX_THREADS;
     p.grid = std::min<int64_t>(rows, (int64_t)sms * 4);
     return p;
   }
-  p.block = !(D <= 256 || (D <= 1024 && rows >= 4 * sms));
+  const int arrays = grad ? 2 : 1;
+  p.pitch = (int)(words * 16 + 15) / 16 * 16;
+  p.block = !(words <= 32 || (words <= 128 && rows >= 4 * sms));
+  int per_sm, groups = 1;
   if (!p.block) {
-    p.elems = D <= 256 ? 8 : D <= 512 ? 16 : 32;
+    p.words = words <= 32 ? 1 : words <= 64 ? 2 : 4;
     p.threads = 32 * NORM_WARPS;
-    p.grid = std::min<int64_t>((rows + NORM_WARPS - 1) / NORM_WARPS, (int64_t)sms * (grad ? 4 : 16));
+    groups = NORM_WARPS;
+    per_sm = !grad ? 8 : p.words == 4 ? 3 : 6;  // 8192 x 1024 bf16, gradient: 3 blocks 84 us, 4 103 us; 256 columns: 6 91 us, 3 102 us
   } else {
-    p.elems = D <= 8 * NORM_MAX_THREADS ? 8 : D <= 16 * NORM_MAX_THREADS ? 16 : 32;
-    p.threads = (int)(((D + p.elems - 1) / p.elems + 31) / 32 * 32);
-    p.grid = std::min<int64_t>(rows, grad ? (int64_t)sms * std::max(1, 1024 / p.threads) : (int64_t)sms * (2048 / p.threads) * 4);
+    // 16384 x 4096, forward: bf16 with 4 words 55 us, with 2 60 us; float with 2 words 92 us, with 4 101 us
+    p.words = !grad && dtype != FV_F32 ? 4 : 2;
+    while (words > (int64_t)p.words * NORM_MAX_THREADS) p.words *= 2;
+    p.threads = (int)(((words + p.words - 1) / p.words + 31) / 32 * 32);
+    per_sm = std::max(1, std::min(16, (grad ? 768 : 1024) / p.threads));
   }
+  const int64_t fixed = (int64_t)groups * RING_MOST * 8, stage = (int64_t)groups * arrays * p.pitch;
+  while (per_sm > 1 && (208 << 10) / per_sm < fixed + 2 * stage) --per_sm;
+  p.stages = (int)std::max<int64_t>(2, std::min<int64_t>(RING_MOST, ((208 << 10) / per_sm - fixed) / stage));
+  const int64_t all = (rows + groups - 1) / groups;
+  p.grid = std::min<int64_t>(all, (int64_t)sms * per_sm);
+  // a block's partial sums cost as much as a row or two: four rows to a block at least
+  if (grad) p.grid = std::min<int64_t>(p.grid, std::max<int64_t>(std::min<int64_t>(all, sms), all / 4));
+  // a group's rows start at the same place in a word when they are a multiple of 8 apart
+  if (p.edge && p.grid < all) p.grid = std::max<int64_t>(8, p.grid / 8 * 8);
+  p.smem = (size_t)(fixed + stage * p.stages);
+  if (grad && !p.block) p.smem = std::max(p.smem, (size_t)(fixed + 2 * D * 4));
   return p;
 }
 
-template <typename T, int VEC, int E>
-void launch_norm(const NormPlan& p, cudaStream_t st, const T* x, int64_t xs, int64_t rows, int D, const T* w, const T* b, float eps,
-                 void* y, int ydt, float* mean, float* rstd) {
-  if (p.block)
-    k_norm<T, VEC, E / VEC, true><<<(unsigned)p.grid, p.threads, 0, st>>>(x, xs, rows, D, w, b, eps, y, ydt, mean, rstd);
-  else
-    k_norm<T, VEC, E / VEC, false><<<(unsigned)p.grid, p.threads, 0, st>>>(x, xs, rows, D, w, b, eps, y, ydt, mean, rstd);
+template <typename T, int NV, bool BLOCK, bool EDGE>
+cudaError_t launch_norm(const NormPlan& p, cudaStream_t st, const T* x, int64_t xs, int64_t rows, int D, const T* w, const T* b, float eps,
+                        void* y, int ydt, float* mean, float* rstd) {
+  const auto kernel = k_norm<T, NV, BLOCK, EDGE>;
+  if (p.smem > 48 << 10) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p.smem);
+  kernel<<<(unsigned)p.grid, p.threads, p.smem, st>>>(x, xs, rows, D, w, b, eps, y, ydt, mean, rstd, p.stages, p.pitch);
+  return cudaGetLastError();
 }
-template <typename T, int VEC, int E>
-void launch_norm_grad(const NormPlan& p, cudaStream_t st, const T* dy, int64_t gs, const T* x, int64_t xs, int64_t rows, int D,
-                      const float* mean, const float* rstd, const T* w, T* dx, float* part) {
-  if (p.block)
-    k_norm_grad<T, VEC, E / VEC, true><<<(unsigned)p.grid, p.threads, 0, st>>>(dy, gs, x, xs, rows, D, mean, rstd, w, dx, part);
-  else
-    k_norm_grad<T, VEC, E / VEC, false><<<(unsigned)p.grid, p.threads, 0, st>>>(dy, gs, x, xs, rows, D, mean, rstd, w, dx, part);
+template <typename T, int NV, bool BLOCK, bool EDGE>
+cudaError_t launch_norm_grad(const NormPlan& p, cudaStream_t st, const T* dy, int64_t gs, const T* x, int64_t xs, int64_t rows, int D,
+                             const float* mean, const float* rstd, const T* w, T* dx, float* part) {
+  const auto kernel = k_norm_grad<T, NV, BLOCK, EDGE>;
+  if (p.smem > 48 << 10) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p.smem);
+  kernel<<<(unsigned)p.grid, p.threads, p.smem, st>>>(dy, gs, x, xs, rows, D, mean, rstd, w, dx, part, p.stages, p.pitch);
+  return cudaGetLastError();
 }
 
-#define NORM_ELEMS(p, T, VEC, FN, ...)                             \
-  do {                                                             \
-    if ((p).elems == 8) FN<T, VEC, 8>(p, __VA_ARGS__);             \
-    else if ((p).elems == 16) FN<T, VEC, 16>(p, __VA_ARGS__);      \
-    else FN<T, VEC, 32>(p, __VA_ARGS__);                           \
-  } while (0)
-#define NORM_VEC(p, T, FN, ...)                                                   \
-  do {                                                                            \
-    constexpr int V16 = 16 / (int)sizeof(T), V4 = 4 / (int)sizeof(T);             \
-    if ((p).vec_bytes == 16) NORM_ELEMS(p, T, V16, FN, __VA_ARGS__);              \
-    else if (V4 > 1 && (p).vec_bytes == 4) NORM_ELEMS(p, T, V4, FN, __VA_ARGS__);      \
-    else NORM_ELEMS(p, T, 1, FN, __VA_ARGS__);                                    \
-  } while (0)
+// eight words a thread: the float forward pass alone
+template <typename T, int NV, bool BLOCK, bool EDGE, typename... A>
+cudaError_t launch_norm_widest(const NormPlan& p, A... a) {
+  if constexpr (sizeof(T) == 4) return launch_norm<T, NV, BLOCK, EDGE>(p, a...);
+  return cudaErrorInvalidValue;
+}
+template <typename T, int NV, bool BLOCK, bool EDGE, typename... A>
+cudaError_t launch_norm_grad_widest(const NormPlan&, A...) {
+  return cudaErrorInvalidValue;
+}
+
+#define NORM_EDGE(p, FN, T, NV, BLOCK, ...) ((p).edge ? FN<T, NV, BLOCK, true>(p, __VA_ARGS__) : FN<T, NV, BLOCK, false>(p, __VA_ARGS__))
+#define NORM_LAUNCH(p, FN, T, ...)                                                                                   \
+  (!(p).block ? ((p).words == 1   ? NORM_EDGE(p, FN, T, 1, false, __VA_ARGS__)                                       \
+                 : (p).words == 2 ? NORM_EDGE(p, FN, T, 2, false, __VA_ARGS__)                                       \
+                                  : NORM_EDGE(p, FN, T, 4, false, __VA_ARGS__))                                      \
+              : ((p).words == 1   ? NORM_EDGE(p, FN, T, 1, true, __VA_ARGS__)                                        \
+                 : (p).words == 2 ? NORM_EDGE(p, FN, T, 2, true, __VA_ARGS__)                                        \
+                 : (p).words == 4 ? NORM_EDGE(p, FN, T, 4, true, __VA_ARGS__)                                        \
+                                  : NORM_EDGE(p, FN##_widest, T, 8, true, __VA_ARGS__)))
 
 int64_t grad_parts(const NormPlan& p, int64_t rows, int64_t D, int sms) {
   if (!p.is_long) return p.grid;
@@ -422,17 +656,23 @@ int64_t grad_parts(const NormPlan& p, int64_t rows, int64_t D, int sms) {
   return std::max<int64_t>(1, std::min<int64_t>(rows, (int64_t)sms * 8 / blocks));
 }
 
-int norm_vec_bytes(int64_t D, size_t es, std::initializer_list<std::pair<const void*, int64_t>> arrays) {
-  for (unsigned bytes : {16u, 4u}) {
-    if (bytes <= es && bytes != 16u) break;
-    bool ok = D % (int64_t)(bytes / es) == 0;
-    for (const auto& a : arrays) ok = ok && (!a.first || vec_ok(a.first, a.second, es, bytes));
-    if (ok) return (int)bytes;
-  }
-  return (int)es;
+// Whole words only: every row of every array starts and ends on a 16-byte boundary.
+bool norm_even(int64_t D, size_t es, std::initializer_list<std::pair<const void*, int64_t>> arrays) {
+  bool ok = D * (int64_t)es % 16 == 0;
+  for (const auto& a : arrays) ok = ok && vec_ok(a.first, a.second, es, 16);
+  return ok;
 }
 
 }  // namespace
+}  // namespace fvo
+
+namespace fvo {
+cudaError_t norm_status(uint32_t* word) {
+  cudaError_t e = cudaMemcpyFromSymbol(word, g_norm_status, sizeof(uint32_t));
+  const uint32_t zero = 0;
+  if (e == cudaSuccess && *word) e = cudaMemcpyToSymbol(g_norm_status, &zero, sizeof(zero));
+  return e;
+}
 }  // namespace fvo
 
 using namespace fvo;
@@ -454,28 +694,29 @@ int fv_layer_norm(int device, void* stream, const void* x, int64_t x_stride, int
   const int sms = sm_count(device);
   FV_REQUIRE(guard.ok && sms > 0, FV_ERR_CUDA, "cannot select device %d", device);
   const size_t es = elem_size(dtype);
-  int vb = norm_vec_bytes(cols, es, {{x, x_stride}, {weight, 0}, {bias, 0}});
-  // y is dense and may be wider than x: its rows must admit the same element count per access
-  while (vb > (int)es && ((uintptr_t)y % std::min<size_t>(16, vb / es * elem_size(y_dtype)) != 0)) vb = vb == 16 && es == 2 ? 4 : (int)es;
-  const NormPlan p = plan_norm(rows, cols, dtype, false, vb, sms);
+  // y is dense; its words (of as many elements as x's) must start on boundaries too
+  const bool even = norm_even(cols, es, {{x, x_stride}}) && (uintptr_t)y % 16 == 0;
+  const NormPlan p = plan_norm(rows, cols, dtype, false, !even, sms);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e = cudaSuccess;
   FV_DTYPE_SWITCH(dtype, T, {
     const T *px = static_cast<const T*>(x), *pw = static_cast<const T*>(weight), *pb = static_cast<const T*>(bias);
-    if (p.is_long)
+    if (p.is_long) {
       k_norm_long<T><<<(unsigned)p.grid, p.threads, 0, st>>>(px, x_stride, rows, cols, pw, pb, eps, y, y_dtype, mean, rstd);
-    else
-      NORM_VEC(p, T, launch_norm, st, px, x_stride, rows, (int)cols, pw, pb, eps, y, y_dtype, mean, rstd);
+      e = cudaGetLastError();
+    } else {
+      e = NORM_LAUNCH(p, launch_norm, T, st, px, x_stride, rows, (int)cols, pw, pb, eps, y, y_dtype, mean, rstd);
+    }
   });
-  FV_CUDA(cudaGetLastError());
+  FV_CUDA(e);
   return FV_OK;
 }
 
 static int norm_grad_plan(int device, const void* dy, int64_t gs, const void* x, int64_t xs, int64_t rows, int64_t cols, int dtype,
-                          const void* weight, const void* dx, NormPlan* p, int64_t* parts) {
+                          const void* dx, NormPlan* p, int64_t* parts) {
   const int sms = sm_count(device);
   FV_REQUIRE(sms > 0, FV_ERR_CUDA, "cannot select device %d", device);
-  const int vb = norm_vec_bytes(cols, elem_size(dtype), {{dy, gs}, {x, xs}, {weight, 0}, {dx, 0}});
-  *p = plan_norm(rows, cols, dtype, true, vb, sms);
+  *p = plan_norm(rows, cols, dtype, true, !norm_even(cols, elem_size(dtype), {{dy, gs}, {x, xs}, {dx, 0}}), sms);
   *parts = grad_parts(*p, rows, cols, sms);
   return FV_OK;
 }
@@ -483,9 +724,11 @@ static int norm_grad_plan(int device, const void* dy, int64_t gs, const void* x,
 int fv_layer_norm_backward_workspace(int device, int64_t rows, int64_t cols, int dtype, size_t* bytes) {
   FV_CHECK_DTYPE(dtype, "fv_layer_norm_backward_workspace");
   FV_REQUIRE(bytes && rows >= 0 && cols >= 1 && cols < (1ll << 31), FV_ERR_INVALID, "fv_layer_norm_backward_workspace: bad argument");
-  NormPlan p;
+  // the plan for aligned rows and the one for others may differ in their number of blocks
+  const int sms = sm_count(device);
+  FV_REQUIRE(sms > 0, FV_ERR_CUDA, "cannot select device %d", device);
   int64_t parts = 0;
-  if (int rc = norm_grad_plan(device, nullptr, 0, nullptr, 0, rows, cols, dtype, nullptr, nullptr, &p, &parts)) return rc;
+  for (bool edge : {false, true}) parts = std::max(parts, grad_parts(plan_norm(rows, cols, dtype, true, edge, sms), rows, cols, sms));
   *bytes = (size_t)std::max<int64_t>(parts, 1) * 2 * (size_t)cols * sizeof(float);
   return FV_OK;
 }
@@ -509,14 +752,15 @@ int fv_layer_norm_backward(int device, void* stream, const void* dy, int64_t dy_
     FV_CUDA(cudaMemsetAsync(dbias, 0, (size_t)cols * elem_size(dtype), st));
     return FV_OK;
   }
-  NormPlan p;
+  NormPlan p{};
   int64_t parts = 0;
-  if (int rc = norm_grad_plan(device, dy, dy_stride, x, x_stride, rows, cols, dtype, weight, dx, &p, &parts)) return rc;
+  if (int rc = norm_grad_plan(device, dy, dy_stride, x, x_stride, rows, cols, dtype, dx, &p, &parts)) return rc;
   const size_t need = (size_t)parts * 2 * (size_t)cols * sizeof(float);
   FV_REQUIRE(!weight || (workspace && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0), FV_ERR_INVALID,
              "fv_layer_norm_backward: the workspace must be 16-byte aligned and hold %llu bytes, got %llu", (unsigned long long)need,
              (unsigned long long)workspace_bytes);
   float* part = weight ? static_cast<float*>(workspace) : nullptr;
+  cudaError_t e = cudaSuccess;
   FV_DTYPE_SWITCH(dtype, T, {
     const T *pg = static_cast<const T*>(dy), *px = static_cast<const T*>(x), *pw = static_cast<const T*>(weight);
     T* pd = static_cast<T*>(dx);
@@ -526,12 +770,13 @@ int fv_layer_norm_backward(int device, void* stream, const void* dy, int64_t dy_
         k_norm_grad_cols<T><<<dim3((unsigned)((cols + 255) / 256), (unsigned)parts), 256, 0, st>>>(pg, dy_stride, px, x_stride, rows, cols,
                                                                                                   mean, rstd, part);
     } else {
-      NORM_VEC(p, T, launch_norm_grad, st, pg, dy_stride, px, x_stride, rows, (int)cols, mean, rstd, pw, pd, part);
+      e = NORM_LAUNCH(p, launch_norm_grad, T, st, pg, dy_stride, px, x_stride, rows, (int)cols, mean, rstd, pw, pd, part);
     }
     if (part)
-      k_norm_grad_reduce<T><<<(unsigned)((2 * cols + 31) / 32), dim3(32, 16), 0, st>>>(part, parts, cols, static_cast<T*>(dweight),
+      k_norm_grad_reduce<T><<<(unsigned)((2 * cols + 31) / 32), 512, 0, st>>>(part, parts, cols, static_cast<T*>(dweight),
                                                                                        static_cast<T*>(dbias));
   });
+  FV_CUDA(e);
   FV_CUDA(cudaGetLastError());
   return FV_OK;
 }

@@ -117,6 +117,53 @@ __device__ __forceinline__ float2 fma2(float2 x, float2 y, float2 z) {
   return unpack2(r);
 }
 
+// Sums of the columns of part[P][n] in a fixed order, 32 columns to a block of 512 threads: four columns to a thread, 64
+// rows at a time, then a tree.  `out(c, v)` is called once per column.
+template <typename F>
+__device__ __forceinline__ void column_sums(const float* __restrict__ part, int64_t P, int64_t n, F out) {
+  __shared__ float4 sum[64][8];
+  const int q = threadIdx.x & 7, lane = threadIdx.x >> 3;
+  const int64_t c = (int64_t)blockIdx.x * 32 + 4 * q;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (n % 4 == 0 && c < n) {
+#pragma unroll 8
+    for (int64_t p = lane; p < P; p += 64) {
+      const float4 v = __ldcs(reinterpret_cast<const float4*>(part + p * n + c));
+      s.x += v.x;
+      s.y += v.y;
+      s.z += v.z;
+      s.w += v.w;
+    }
+  } else {
+#pragma unroll 4
+    for (int64_t p = lane; p < P; p += 64) {
+      const float* v = part + p * n + c;
+      if (c < n) s.x += v[0];
+      if (c + 1 < n) s.y += v[1];
+      if (c + 2 < n) s.z += v[2];
+      if (c + 3 < n) s.w += v[3];
+    }
+  }
+  sum[lane][q] = s;
+  for (int k = 32; k; k >>= 1) {
+    __syncthreads();
+    if (lane < k) {
+      const float4 v = sum[lane + k][q];
+      s.x += v.x;
+      s.y += v.y;
+      s.z += v.z;
+      s.w += v.w;
+      sum[lane][q] = s;
+    }
+  }
+  if (lane == 0) {
+    if (c < n) out(c, s.x);
+    if (c + 1 < n) out(c + 1, s.y);
+    if (c + 2 < n) out(c + 2, s.z);
+    if (c + 3 < n) out(c + 3, s.w);
+  }
+}
+
 // Bytes that divide an address and a stride: which vector width a row-major array admits.
 inline unsigned common_alignment(uintptr_t a) { return a == 0 ? 4096u : (unsigned)(a & (~a + 1)); }
 inline bool vec_ok(const void* p, int64_t stride_elems, size_t elem, unsigned bytes) {
@@ -125,6 +172,7 @@ inline bool vec_ok(const void* p, int64_t stride_elems, size_t elem, unsigned by
 inline size_t elem_size(int dtype) { return dtype == FV_F32 ? 4 : 2; }
 
 int sm_count(int device);  // cached per device; 0 after an error
+cudaError_t norm_status(uint32_t* word);  // reads and clears the error bits of fv_norm.cu's kernels
 
 }  // namespace fvo
 
