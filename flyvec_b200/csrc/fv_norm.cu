@@ -616,7 +616,8 @@ template <typename T, int NV, bool BLOCK, bool EDGE>
 cudaError_t launch_norm(const NormPlan& p, cudaStream_t st, const T* x, int64_t xs, int64_t rows, int D, const T* w, const T* b, float eps,
                         void* y, int ydt, float* mean, float* rstd) {
   const auto kernel = k_norm<T, NV, BLOCK, EDGE>;
-  if (p.smem > 48 << 10) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p.smem);
+  static size_t given[64] = {0};
+  if (cudaError_t e = allow_smem((const void*)kernel, given, p.smem)) return e;
   kernel<<<(unsigned)p.grid, p.threads, p.smem, st>>>(x, xs, rows, D, w, b, eps, y, ydt, mean, rstd, p.stages, p.pitch);
   return cudaGetLastError();
 }
@@ -624,7 +625,8 @@ template <typename T, int NV, bool BLOCK, bool EDGE>
 cudaError_t launch_norm_grad(const NormPlan& p, cudaStream_t st, const T* dy, int64_t gs, const T* x, int64_t xs, int64_t rows, int D,
                              const float* mean, const float* rstd, const T* w, T* dx, float* part) {
   const auto kernel = k_norm_grad<T, NV, BLOCK, EDGE>;
-  if (p.smem > 48 << 10) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)p.smem);
+  static size_t given[64] = {0};
+  if (cudaError_t e = allow_smem((const void*)kernel, given, p.smem)) return e;
   kernel<<<(unsigned)p.grid, p.threads, p.smem, st>>>(dy, gs, x, xs, rows, D, mean, rstd, w, dx, part, p.stages, p.pitch);
   return cudaGetLastError();
 }

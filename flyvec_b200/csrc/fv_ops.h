@@ -171,6 +171,18 @@ inline bool vec_ok(const void* p, int64_t stride_elems, size_t elem, unsigned by
 }
 inline size_t elem_size(int dtype) { return dtype == FV_F32 ? 4 : 2; }
 
+// Lets a kernel have `bytes` of dynamic shared memory on the current device; `done` is the kernel's own record of what it was
+// given per device (a race between threads repeats a call that does no harm).
+inline cudaError_t allow_smem(const void* kernel, size_t (&done)[64], size_t bytes) {
+  if (bytes <= (48u << 10)) return cudaSuccess;
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess || (device < 64 && done[device] >= bytes)) return e;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess && device < 64) done[device] = bytes;
+  return e;
+}
+
 int sm_count(int device);  // cached per device; 0 after an error
 cudaError_t norm_status(uint32_t* word);  // reads and clears the error bits of fv_norm.cu's kernels
 

@@ -429,7 +429,7 @@ class DeviceArray(DeviceBuffer):
     """Dense row-major array in device memory, the operand of :mod:`flyvec_b200.ops` where no PyTorch is at hand.
     ``dtype`` is a name ("float32", "bfloat16", "float16", "int32", "int64", "uint8")."""
 
-    is_cuda = True
+    is_cuda, requires_grad = True, False  # what the operators ask of an array
     _NUMPY = {"float32": np.float32, "float16": np.float16, "int32": np.int32, "int64": np.int64, "uint8": np.uint8,
               "bfloat16": np.uint16}
 
@@ -476,6 +476,9 @@ class DeviceArray(DeviceBuffer):
 
     def get_device(self) -> int:
         return self.device
+
+    def is_neg(self) -> bool:
+        return False
 
     def stride(self):
         out, step = [], 1

@@ -20,6 +20,7 @@ from __future__ import annotations
 import ctypes as C
 import math
 import sys
+from functools import lru_cache
 from typing import Any, NamedTuple
 
 from . import _lib
@@ -34,6 +35,7 @@ MAX_TOP = 64
 
 _names: dict = {}  # dtype object -> name
 _torch_types: dict = {}  # name -> torch dtype
+_raw_stream = None  # (device) -> handle of the current stream
 
 
 def _type(x) -> str:
@@ -43,10 +45,10 @@ def _type(x) -> str:
     return name
 
 
-def _check(x, what: str, types=None, like=None):
-    """One argument: a device array, of one of ``types``, on the device and of the kind of ``like``."""
+def _refuse(x, what: str, types, like):
+    """The error of an argument that :func:`_check` did not pass."""
     if not isinstance(x, DeviceArray):
-        if not (hasattr(x, "data_ptr") and hasattr(x, "is_cuda")):
+        if not (hasattr(x, "data_ptr") and hasattr(x, "is_cuda") and hasattr(x, "is_neg")):
             raise TypeError(f"{what} must be a DeviceArray or a CUDA tensor, got {type(x).__name__}")
         if not x.is_cuda:
             raise ValueError(f"{what} must be on a GPU, got a tensor on {x.device}")
@@ -54,7 +56,7 @@ def _check(x, what: str, types=None, like=None):
             raise ValueError(f"{what} requires a gradient, which these operators do not record: pass {what}.detach()")
         if x.is_neg():
             raise ValueError(f"{what} is a lazily negated view: pass {what}.resolve_neg()")
-    if types is not None and _type(x) not in types:
+    if _type(x) not in types:
         raise TypeError(f"{what} must have one of the types {', '.join(types)}, got {_type(x)}")
     if like is not None:
         if isinstance(x, DeviceArray) != isinstance(like, DeviceArray):
@@ -63,10 +65,23 @@ def _check(x, what: str, types=None, like=None):
             raise ValueError(f"{what} is on device {x.get_device()}, the first argument on device {like.get_device()}")
 
 
+def _check(x, what: str, types, like=None):
+    """One argument: a device array, of one of ``types``, on the device and of the kind of ``like``."""
+    try:
+        if x.is_cuda and not x.requires_grad and not x.is_neg() and _names.get(x.dtype) in types and (
+                like is None or (type(x) is type(like) and x.get_device() == like.get_device())):
+            return
+    except AttributeError:
+        pass
+    _refuse(x, what, types, like)
+
+
 def _rows(x, what: str):
     """(rows, columns, row stride) of an array whose leading axes are taken together."""
-    shape, strides = tuple(x.shape), x.stride()
-    if not shape:
+    shape, strides = x.shape, x.stride()
+    if len(shape) == 2 and strides[1] == 1:
+        return shape[0], shape[1], strides[0] if shape[0] != 1 else shape[1]
+    if not len(shape):
         raise ValueError(f"{what} must have at least one axis")
     cols = shape[-1]
     if cols > 1 and strides[-1] != 1:
@@ -77,7 +92,7 @@ def _rows(x, what: str):
             if step is None:
                 step = s
             elif s != step * rows and rows:
-                raise ValueError(f"the leading axes of {what} (shape {shape}, strides {strides}) do not lie at one common distance: "
+                raise ValueError(f"the leading axes of {what} (shape {tuple(shape)}, strides {strides}) do not lie at one common distance: "
                                  f"pass {what}.contiguous()")
         rows *= n
     return rows, cols, cols if step is None else step
@@ -85,9 +100,11 @@ def _rows(x, what: str):
 
 def _matrix(x, what: str):
     """(rows, columns, row stride, column stride); two axes may be stored either way round."""
-    if len(x.shape) == 2:
-        (n, k), (rs, cs) = x.shape, x.stride()
-        if (cs == 1 or k <= 1) or (rs == 1 or n <= 1):
+    shape = x.shape
+    if len(shape) == 2:
+        n, k = shape
+        rs, cs = x.stride()
+        if cs == 1 or k <= 1 or rs == 1 or n <= 1:
             return n, k, rs, cs
         raise ValueError(f"one axis of {what} must be contiguous, its strides are {(rs, cs)}: pass {what}.contiguous()")
     rows, cols, step = _rows(x, what)
@@ -95,7 +112,7 @@ def _matrix(x, what: str):
 
 
 def _empty(like, shape, dtype: str):
-    if isinstance(like, DeviceArray):
+    if type(like) is DeviceArray:
         return like.new_empty(shape, dtype)
     t = _torch_types.get(dtype)
     if t is None:
@@ -103,10 +120,22 @@ def _empty(like, shape, dtype: str):
     return like.new_empty(shape, dtype=t)
 
 
-def _stream(x):
-    if isinstance(x, DeviceArray):
+def _floats(like, n: int, shape):
+    """n float32 arrays of one shape."""
+    if type(like) is DeviceArray:
+        return [like.new_empty(shape, "float32") for _ in range(n)]
+    return _empty(like, (n, *shape), "float32").unbind(0)  # one allocation
+
+
+def _stream(x, device: int):
+    """Handle of the stream the work goes to."""
+    global _raw_stream
+    if type(x) is DeviceArray:
         return None
-    return sys.modules["torch"].cuda.current_stream(x.get_device()).cuda_stream
+    if _raw_stream is None:
+        torch = sys.modules["torch"]
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
+    return _raw_stream(device)
 
 
 def _ptr(x):
@@ -116,9 +145,9 @@ def _ptr(x):
 def _vector(x, n: int, what: str, like, types):
     """A dense vector of n elements (any shape of n elements is taken in order)."""
     _check(x, what, types, like)
-    if math.prod(x.shape) != n:
+    if (x.size if type(x) is DeviceArray else x.numel()) != n:
         raise ValueError(f"{what} must have {n} elements, got shape {tuple(x.shape)}")
-    return x if isinstance(x, DeviceArray) or x.is_contiguous() else x.contiguous()
+    return x if type(x) is DeviceArray or x.is_contiguous() else x.contiguous()
 
 
 def _same_shape(x, shape, what: str):
@@ -131,6 +160,29 @@ def _activation(name) -> int:
     if code is None:
         raise ValueError(f"activation must be one of {', '.join(ACTIVATIONS)}, got {name!r}")
     return code
+
+
+# workspace sizes: functions of sizes, strides and the alignment of the operands alone
+@lru_cache(maxsize=1024)
+def _norm_workspace(device: int, rows: int, cols: int, dtype: int) -> int:
+    need = C.c_size_t(0)
+    check(_lib.lib().fv_layer_norm_backward_workspace(device, rows, cols, dtype, C.byref(need)))
+    return need.value
+
+
+@lru_cache(maxsize=1024)
+def _linear_workspace(rows: int, inner: int, outer: int, x: int, xr: int, xc: int, w: int, wr: int, wc: int) -> int:
+    need = C.c_size_t(0)
+    check(_lib.lib().fv_linear_workspace(rows, inner, outer, x, xr, xc, w, wr, wc, C.byref(need)))
+    return need.value
+
+
+@lru_cache(maxsize=1024)
+def _linear_backward_workspace(device: int, rows: int, inner: int, outer: int, dy: int, gs: int, x: int, xr: int, xc: int, w: int, wr: int,
+                               wc: int, act: int) -> int:
+    need = C.c_size_t(0)
+    check(_lib.lib().fv_linear_backward_workspace(device, rows, inner, outer, dy, gs, x, xr, xc, w, wr, wc, act, C.byref(need)))
+    return need.value
 
 
 # ---- layer norm ------------------------------------------------------------------------------------
@@ -156,11 +208,11 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, out_dtype: str | No
         weight = _vector(weight, cols, "weight", x, (kind,))
     if bias is not None:
         bias = _vector(bias, cols, "bias", x, (kind,))
-    lead = tuple(x.shape[:-1])
-    y = _empty(x, tuple(x.shape), out_dtype)
-    mean = _empty(x, lead, "float32") if return_stats else None
-    rstd = _empty(x, lead, "float32") if return_stats else None
-    check(_lib.lib().fv_layer_norm(x.get_device(), _stream(x), x.data_ptr(), step, rows, cols, DTYPES[kind], _ptr(weight), _ptr(bias), eps,
+    y, mean, rstd, dev = _empty(x, x.shape, out_dtype), None, None, x.get_device()
+    if return_stats:
+        lead = x.shape[:-1]
+        mean, rstd = _empty(x, lead, "float32"), _empty(x, lead, "float32")
+    check(_lib.lib().fv_layer_norm(dev, _stream(x, dev), x.data_ptr(), step, rows, cols, DTYPES[kind], _ptr(weight), _ptr(bias), eps,
                                    y.data_ptr(), DTYPES[out_dtype], _ptr(mean), _ptr(rstd)))
     return (y, mean, rstd) if return_stats else y
 
@@ -181,16 +233,14 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None):
     rstd = _vector(rstd, rows, "rstd", x, ("float32",))
     if weight is not None:
         weight = _vector(weight, cols, "weight", x, (kind,))
-    dx = _empty(x, tuple(x.shape), kind)
+    dx = _empty(x, x.shape, kind)
     dev, lib = x.get_device(), _lib.lib()
     dw = db = ws = None
     size = 0
     if weight is not None:
-        need = C.c_size_t(0)
-        check(lib.fv_layer_norm_backward_workspace(dev, rows, cols, DTYPES[kind], C.byref(need)))
-        size = need.value
+        size = _norm_workspace(dev, rows, cols, DTYPES[kind])
         dw, db, ws = _empty(x, (cols,), kind), _empty(x, (cols,), kind), _empty(x, (size,), "uint8")
-    check(lib.fv_layer_norm_backward(dev, _stream(x), dy.data_ptr(), gstep, x.data_ptr(), step, rows, cols, DTYPES[kind], mean.data_ptr(),
+    check(lib.fv_layer_norm_backward(dev, _stream(x, dev), dy.data_ptr(), gstep, x.data_ptr(), step, rows, cols, DTYPES[kind], mean.data_ptr(),
                                      rstd.data_ptr(), _ptr(weight), dx.data_ptr(), _ptr(dw), _ptr(db), _ptr(ws), size))
     return dx, dw, db
 
@@ -232,14 +282,11 @@ def linear(x, weight, bias=None, activation: str | None = None, residual=None, o
         _, _, rstep = _rows(residual, "residual")
     y = _empty(x, shape, out_dtype)
     z = _empty(x, shape, kind) if return_preactivation else None
-    lib, size, ws = _lib.lib(), 0, None
-    need = C.c_size_t(0)
-    check(lib.fv_linear_workspace(rows, inner, outer, x.data_ptr(), xr, xc, weight.data_ptr(), wr, wc, C.byref(need)))
-    if need.value:
-        size = need.value
-        ws = _empty(x, (size,), "uint8")
-    check(lib.fv_linear(x.get_device(), _stream(x), x.data_ptr(), xr, xc, weight.data_ptr(), wr, wc, rows, inner, outer, DTYPES[kind],
-                        _ptr(bias), act, _ptr(residual), rstep, y.data_ptr(), DTYPES[out_dtype], _ptr(z), _ptr(ws), size))
+    dev, px, pw = x.get_device(), x.data_ptr(), weight.data_ptr()
+    size = _linear_workspace(rows, inner, outer, px & 15, xr, xc, pw & 15, wr, wc)
+    ws = _empty(x, (size,), "uint8") if size else None
+    check(_lib.lib().fv_linear(dev, _stream(x, dev), px, xr, xc, pw, wr, wc, rows, inner, outer, DTYPES[kind], _ptr(bias), act,
+                               _ptr(residual), rstep, y.data_ptr(), DTYPES[out_dtype], _ptr(z), _ptr(ws), size))
     return (y, z) if return_preactivation else y
 
 
@@ -271,19 +318,19 @@ def linear_backward(dy, x, weight, preactivation=None, activation: str | None = 
         _, _, zstep = _rows(preactivation, "preactivation")
     else:
         preactivation = None
-    dx, dw, db = _empty(x, tuple(x.shape), kind), _empty(x, (outer, inner), kind), _empty(x, (outer,), kind)
-    dev, lib = x.get_device(), _lib.lib()
-    need = C.c_size_t(0)
-    check(lib.fv_linear_backward_workspace(dev, rows, inner, outer, dy.data_ptr(), gstep, x.data_ptr(), xr, xc, weight.data_ptr(), wr, wc,
-                                           act, C.byref(need)))
-    size = need.value
+    dx, dw, db = _empty(x, x.shape, kind), _empty(x, (outer, inner), kind), _empty(x, (outer,), kind)
+    dev, pg, px, pw = x.get_device(), dy.data_ptr(), x.data_ptr(), weight.data_ptr()
+    size = _linear_backward_workspace(dev, rows, inner, outer, pg & 15, gstep, px & 15, xr, xc, pw & 15, wr, wc, act)
     ws = _empty(x, (size,), "uint8") if size else None
-    check(lib.fv_linear_backward(dev, _stream(x), dy.data_ptr(), gstep, x.data_ptr(), xr, xc, weight.data_ptr(), wr, wc, rows, inner, outer,
-                                 DTYPES[kind], _ptr(preactivation), zstep, act, dx.data_ptr(), dw.data_ptr(), db.data_ptr(), _ptr(ws), size))
+    check(_lib.lib().fv_linear_backward(dev, _stream(x, dev), pg, gstep, px, xr, xc, pw, wr, wc, rows, inner, outer, DTYPES[kind],
+                                        _ptr(preactivation), zstep, act, dx.data_ptr(), dw.data_ptr(), db.data_ptr(), _ptr(ws), size))
     return dx, dw, db
 
 
 # ---- log probabilities -----------------------------------------------------------------------------
+_INTS = ("int32", "int64")
+
+
 class TokenLogProbs(NamedTuple):
     """What :func:`token_log_probs` answers, float32 except the int32 ``top_ids``; the last two are None for ``top=0``."""
     log_prob: Any
@@ -312,13 +359,13 @@ def token_log_probs(logits, targets, beta: float = 1.0, top: int = 0) -> TokenLo
     if not 0 <= top <= min(MAX_TOP, vocab):
         raise ValueError(f"top must be between 0 and min({MAX_TOP}, {vocab}), got {top}")
     lead = tuple(logits.shape[:-1])
-    _check(targets, "targets", ("int32", "int64"), logits)
+    targets = _vector(targets, rows, "targets", logits, _INTS)
     _same_shape(targets, lead, "targets")
-    targets = _vector(targets, rows, "targets", logits, ("int32", "int64"))
-    lp, ent, mx, lz = (_empty(logits, lead, "float32") for _ in range(4))
+    lp, ent, mx, lz = _floats(logits, 4, lead)
+    dev = logits.get_device()
     ids = _empty(logits, lead + (top,), "int32") if top else None
     tlp = _empty(logits, lead + (top,), "float32") if top else None
-    check(_lib.lib().fv_token_log_probs(logits.get_device(), _stream(logits), logits.data_ptr(), step, rows, vocab, DTYPES[_type(logits)],
+    check(_lib.lib().fv_token_log_probs(dev, _stream(logits, dev), logits.data_ptr(), step, rows, vocab, DTYPES[_type(logits)],
                                         targets.data_ptr(), int(_type(targets) == "int64"), beta, top, lp.data_ptr(), ent.data_ptr(),
                                         mx.data_ptr(), lz.data_ptr(), _ptr(ids), _ptr(tlp)))
     return TokenLogProbs(lp, ent, mx, lz, ids, tlp)
@@ -334,9 +381,8 @@ def token_log_probs_backward(grad_log_prob, logits, targets, row_max, log_z, ent
         raise ValueError("the vocabulary is empty")
     if not (0 < beta < math.inf):
         raise ValueError(f"beta must be positive and finite, got {beta}")
-    _check(targets, "targets", ("int32", "int64"), logits)
+    targets = _vector(targets, rows, "targets", logits, _INTS)
     _same_shape(targets, logits.shape[:-1], "targets")
-    targets = _vector(targets, rows, "targets", logits, ("int32", "int64"))
     f32 = ("float32",)
     grad_log_prob = _vector(grad_log_prob, rows, "grad_log_prob", logits, f32)
     row_max, log_z = _vector(row_max, rows, "row_max", logits, f32), _vector(log_z, rows, "log_z", logits, f32)
@@ -347,8 +393,8 @@ def token_log_probs_backward(grad_log_prob, logits, targets, row_max, log_z, ent
         entropy = _vector(entropy, rows, "entropy", logits, f32)
     else:
         entropy = None
-    dx = _empty(logits, tuple(logits.shape), _type(logits))
-    check(_lib.lib().fv_token_log_probs_backward(logits.get_device(), _stream(logits), grad_log_prob.data_ptr(), _ptr(grad_entropy),
+    dx, dev = _empty(logits, logits.shape, _type(logits)), logits.get_device()
+    check(_lib.lib().fv_token_log_probs_backward(dev, _stream(logits, dev), grad_log_prob.data_ptr(), _ptr(grad_entropy),
                                                  logits.data_ptr(), step, rows, vocab, DTYPES[_type(logits)], targets.data_ptr(),
                                                  int(_type(targets) == "int64"), row_max.data_ptr(), log_z.data_ptr(), _ptr(entropy), beta,
                                                  dx.data_ptr()))

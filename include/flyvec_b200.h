@@ -320,7 +320,8 @@ int fv_layer_norm_backward(int device, void* stream, const void* dy, int64_t dy_
 /* z = x w^T + bias, y = act(z) + residual.  x [rows][inner] and w [outer][inner] in bfloat16 or float16, each given by a row and a
  * column stride of which one is 1 (so a transposed weight needs no copy); bias [outer] and residual [rows][outer] of
  * the same type or NULL; y in that type or float; z (may be NULL) receives the pre-activation for the backward pass.
- * The workspace is empty unless x or w has rows that do not start on 16-byte boundaries. */
+ * The workspace is empty unless x or w has rows that do not start on 16-byte boundaries; of the pointers given to the
+ * ..._workspace functions only the alignment counts. */
 int fv_linear_workspace(int64_t rows, int64_t inner, int64_t outer, const void* x, int64_t x_rs, int64_t x_cs, const void* w, int64_t w_rs,
                         int64_t w_cs, size_t* bytes);
 int fv_linear(int device, void* stream, const void* x, int64_t x_rs, int64_t x_cs, const void* w, int64_t w_rs, int64_t w_cs, int64_t rows,
