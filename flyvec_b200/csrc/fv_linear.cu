@@ -256,7 +256,7 @@ constexpr int GEMM_SMEM = 1024 + RING_BYTES + EPI_WARPS * (STAGE_OUT + 128) + 25
 
 struct GemmParams {
   int64_t m, n;        // rows of A, rows of B
-  int kblocks, tiles_m, tiles_n, splits;
+  int kblocks, tiles_m, tiles_n;
   int a_mn, b_mn;      // operand stored with its row index contiguous
   uint32_t idesc;
   int act, out_f32, swap;  // swap: D is stored transposed, out[n][m]; bias runs along m
@@ -264,6 +264,16 @@ struct GemmParams {
   const void *bias, *residual;
   void *y, *z;
   int64_t ldr, ldy, ldz;
+};
+// One launch: one product, or two of the same tile shape whose tiles follow one another (a backward pass's dx and dw, so
+// that the second fills the SMs the first leaves idle).
+struct GemmMaps {
+  CUtensorMap a[2], b[2], y[2];
+};
+struct GemmJob {
+  GemmParams p[2];
+  int tiles0, tiles;  // of the first product, of both
+  int splits;
 };
 
 // Where a tile lies.  Tiles are taken in bands of 16 row tiles, column by column within a band, so that the blocks
@@ -401,13 +411,46 @@ __device__ __forceinline__ void store_one(const GemmParams& p, int64_t r, int64_
     static_cast<T*>(p.y)[r * p.ldy + c] = from_f<T>(v);
 }
 
+// four consecutive columns of row r; c is a multiple of 4
+template <typename T>
+__device__ __forceinline__ void store_four(const GemmParams& p, int64_t r, int64_t c, float (&v)[4]) {
+  if (c + 4 > p.n || !p.vec_y || (p.z && !p.vec_z) || (p.residual && !p.vec_r)) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (c + j < p.n) store_one<T>(p, r, c + j, v[j] + (p.bias ? to_f<T>(static_cast<const T*>(p.bias)[c + j]) : 0.f));
+    return;
+  }
+  if (p.bias) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] += to_f<T>(static_cast<const T*>(p.bias)[c + j]);
+  }
+  Pack<T, 4> o;
+  if (p.z) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o.e[j] = from_f<T>(v[j]);
+    store_pack<T, 4>(static_cast<T*>(p.z) + r * p.ldz + c, o);
+  }
+  act_values(v, p.act);
+  if (p.residual) {
+    const Pack<T, 4> q = load_pack<T, 4>(static_cast<const T*>(p.residual) + r * p.ldr + c);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] += to_f<T>(q.e[j]);
+  }
+  if (p.out_f32) {
+    *reinterpret_cast<float4*>(static_cast<float*>(p.y) + r * p.ldy + c) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o.e[j] = from_f<T>(v[j]);
+    store_pack<T, 4>(static_cast<T*>(p.y) + r * p.ldy + c, o);
+  }
+}
+
 // PAIR: two neighbouring blocks (a cluster) work on one 256 x BN tile: each loads its 128 rows of A and half of B's rows, the
 // first one's thread issues the products of both (they read both blocks' shared memory), and each takes its own 128 rows of
 // the accumulator through the epilogue.
 template <typename T, int BN, bool PAIR>
 __global__ void __launch_bounds__(GEMM_THREADS, 1)
-    k_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_y,
-           const __grid_constant__ GemmParams p) {
+    k_gemm(const __grid_constant__ GemmMaps maps, const __grid_constant__ GemmJob job) {
   constexpr int BROWS = PAIR ? BN / 2 : BN;  // rows of B this block loads
   constexpr int A_BYTES = BM * BK * 2, B_BYTES = BROWS * BK * 2, STAGE = A_BYTES + B_BYTES, STAGES = RING_BYTES / STAGE;
   constexpr int TMEM_COLS = 2 * BN;
@@ -458,18 +501,28 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
   const uint32_t tmem = *tmem_slot;
 
   // blocks of one cluster (splits > 1) share a tile and divide its k-blocks; otherwise a block walks over its tiles
-  const int rank = !PAIR && p.splits > 1 ? blockIdx.x % p.splits : 0;
-  const int kb0 = (int)((int64_t)p.kblocks * rank / p.splits), kb1 = (int)((int64_t)p.kblocks * (rank + 1) / p.splits);
-  const int group = PAIR ? 2 : p.splits, first = blockIdx.x / group, step = gridDim.x / group, tiles = p.tiles_m * p.tiles_n;
+  const int rank = !PAIR && job.splits > 1 ? blockIdx.x % job.splits : 0;
+  const int group = PAIR ? 2 : job.splits, first = blockIdx.x / group, step = gridDim.x / group;
+  // tile t: its product, place and k-blocks
+  auto locate = [&](int t, int& tm, int& tn) {
+    const int which = t >= job.tiles0;
+    tile_at(job.p[which], which ? t - job.tiles0 : t, tm, tn);
+    return which;
+  };
+  auto first_k = [&](const GemmParams& p) { return (int)((int64_t)p.kblocks * rank / job.splits); };
+  auto last_k = [&](const GemmParams& p) { return (int)((int64_t)p.kblocks * (rank + 1) / job.splits); };
 
   if (warp == 0) {
     if (elect_one()) {  // loads
       int s = 0, phase = 0, issued = 0;
       bool ok = true;
-      for (int t = first; t < tiles && ok; t += step) {
+      for (int t = first; t < job.tiles && ok; t += step) {
         int tm, tn;
-        tile_at(p, t, tm, tn);
-        for (int kb = kb0; kb < kb1; ++kb) {
+        const int which = locate(t, tm, tn);
+        const GemmParams& p = job.p[which];
+        const CUtensorMap *map_a = &maps.a[which], *map_b = &maps.b[which];
+        const int kb1 = last_k(p);
+        for (int kb = first_k(p); kb < kb1; ++kb) {
           if (!(ok = mbar_wait(empty(s), phase ^ 1, stop))) break;
           const uint32_t a = ring + s * STAGE, b = a + A_BYTES;
           const int ra = PAIR ? tm * 2 * BM + side * BM : tm * BM, rb = tn * BN + side * BROWS;
@@ -477,15 +530,15 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
           if (side == 0) mbar_expect(full(s), PAIR ? 2 * STAGE : STAGE);
           if (p.a_mn) {
 #pragma unroll
-            for (int j = 0; j < BM / 64; ++j) tma_load<PAIR>(a + j * 8192, &map_a, ra + j * 64, kb * BK, bar);
+            for (int j = 0; j < BM / 64; ++j) tma_load<PAIR>(a + j * 8192, map_a, ra + j * 64, kb * BK, bar);
           } else {
-            tma_load<PAIR>(a, &map_a, kb * BK, ra, bar);
+            tma_load<PAIR>(a, map_a, kb * BK, ra, bar);
           }
           if (p.b_mn) {
 #pragma unroll
-            for (int j = 0; j < BROWS / 64; ++j) tma_load<PAIR>(b + j * 8192, &map_b, rb + j * 64, kb * BK, bar);
+            for (int j = 0; j < BROWS / 64; ++j) tma_load<PAIR>(b + j * 8192, map_b, rb + j * 64, kb * BK, bar);
           } else {
-            tma_load<PAIR>(b, &map_b, kb * BK, rb, bar);
+            tma_load<PAIR>(b, map_b, kb * BK, rb, bar);
           }
           ++issued;
           if (++s == STAGES) {
@@ -507,12 +560,15 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
     }
   } else if (warp == 1) {
     if (side == 0 && elect_one()) {  // products
-      // one 16-deep step inside a 64-deep k-block: 32 bytes along k-major rows, 16 rows of 128 bytes otherwise
-      const uint32_t a_step = p.a_mn ? 2048 : 32, b_step = p.b_mn ? 2048 : 32;
-      const uint32_t a_lead = p.a_mn ? 8192 : 16, b_lead = p.b_mn ? 8192 : 16;
       int s = 0, phase = 0, acc = 0, acc_phase = 0;
       bool ok = true;
-      for (int t = first; t < tiles && ok; t += step) {
+      for (int t = first; t < job.tiles && ok; t += step) {
+        const GemmParams& p = job.p[t >= job.tiles0];
+        // one 16-deep step inside a 64-deep k-block: 32 bytes along k-major rows, 16 rows of 128 bytes otherwise
+        const uint32_t a_step = p.a_mn ? 2048 : 32, b_step = p.b_mn ? 2048 : 32;
+        const uint32_t a_lead = p.a_mn ? 8192 : 16, b_lead = p.b_mn ? 8192 : 16;
+        const uint32_t idesc = p.idesc;
+        const int kb0 = first_k(p), kb1 = last_k(p);
         if (!(ok = mbar_wait(acc_empty(acc), acc_phase ^ 1, stop))) break;
         tc_fence_after();
         for (int kb = kb0; kb < kb1; ++kb) {
@@ -521,7 +577,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
           const uint32_t a = ring + s * STAGE, b = a + A_BYTES;
 #pragma unroll
           for (int k = 0; k < BK / 16; ++k)
-            mma_f16<PAIR>(tmem + acc * BN, smem_desc(a + k * a_step, a_lead, 1024), smem_desc(b + k * b_step, b_lead, 1024), p.idesc,
+            mma_f16<PAIR>(tmem + acc * BN, smem_desc(a + k * a_step, a_lead, 1024), smem_desc(b + k * b_step, b_lead, 1024), idesc,
                     kb != kb0 || k != 0);
           mma_commit<PAIR>(empty(s));
           if (++s == STAGES) {
@@ -547,17 +603,18 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
     const int quarter = warp & 3, half = (warp - 2) >> 2;
     uint8_t* stage = staging + (warp - 2) * STAGE_OUT;
     float* bias_slice = bias_slices + (warp - 2) * 32;
-    const T* bias = static_cast<const T*>(p.bias);
     int acc = 0, acc_phase = 0;
-    for (int t = first; t < tiles; t += step) {
+    for (int t = first; t < job.tiles; t += step) {
       int tm, tn;
-      tile_at(p, t, tm, tn);
+      const int which = locate(t, tm, tn);
+      const GemmParams& p = job.p[which];
+      const T* bias = static_cast<const T*>(p.bias);
       const int64_t r0 = (int64_t)(PAIR ? tm * 2 + side : tm) * BM + quarter * 32;
       uint4 early[8];
-      if (p.residual && p.splits == 1 && !p.swap && half * 64 < BN)
+      if (p.residual && job.splits == 1 && !p.swap && half * 64 < BN)
         fetch_in(early, p.residual, p.ldr, p.vec_r, r0, (int64_t)tn * BN + half * 64, p.m, p.n);
       float bias_reg[4];  // this warp's two slices, a column a lane
-      if (bias && p.splits == 1 && !p.swap) {
+      if (bias && job.splits == 1 && !p.swap) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int64_t c = (int64_t)tn * BN + half * 64 + (j >> 1) * 128 + (j & 1) * 32 + lane;
@@ -567,7 +624,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
       if (!mbar_wait(acc_full(acc), acc_phase, stop)) break;
       tc_fence_after();
       const uint32_t src = tmem + acc * BN + ((uint32_t)(quarter * 32) << 16);
-      if (!PAIR && p.splits > 1) {  // to shared memory (the ring is free: every load was consumed before acc_full)
+      if (!PAIR && job.splits > 1) {  // to shared memory (the ring is free: every load was consumed before acc_full)
         float* part = reinterpret_cast<float*>(smem);
         for (int c = half * 32; c < BN; c += 64) {
           float v[32];
@@ -646,7 +703,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
               if (!p.z) stage_free();
               stage_row_f32(stage, lane, v);
               if (p.vec_y)
-                stage_store(stage, &map_y, r0, ch);
+                stage_store(stage, &maps.y[which], r0, ch);
               else
                 stage_out(stage, p.y, p.ldy, 4, 0, r0, ch, p.m, p.n);
               if (p.z) stage_free();
@@ -668,7 +725,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
 #pragma unroll
             for (int k = 0; k < 8; ++k) *reinterpret_cast<uint4*>(stage + lane * 128 + ((k ^ (lane & 7)) << 4)) = res[k];
             if (p.vec_y) {
-              stage_store(stage, &map_y, r0, c0);
+              stage_store(stage, &maps.y[which], r0, c0);
             } else {
               stage_out(stage, p.y, p.ldy, 2, 0, r0, c0, p.m, p.n);
               if (c0 + 32 < p.n) stage_out(stage, p.y, p.ldy, 2, 1, r0, c0 + 32, p.m, p.n);
@@ -692,15 +749,16 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // shared memory outlives the stores that read it
   }
   __syncwarp();
-  if (!PAIR && p.splits > 1) {
+  if (!PAIR && job.splits > 1) {
     __syncthreads();
     __syncwarp();
     cluster_barrier();
     // this block finishes 128 / splits rows of the tile from all blocks' partial tiles
-    if (!*stop && first < tiles) {
+    if (!*stop && first < job.tiles) {
+      const GemmParams& p = job.p[0];
       int tm, tn;
       tile_at(p, first, tm, tn);
-      const int rows = BM / p.splits, row0 = rank * rows;
+      const int rows = BM / job.splits, row0 = rank * rows;
       const T* bias = static_cast<const T*>(p.bias);
       constexpr int QUADS = BN / 4;
       for (int i = threadIdx.x; i < rows * QUADS; i += GEMM_THREADS) {
@@ -709,23 +767,26 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
         const int64_t m = (int64_t)tm * BM + r, n = (int64_t)tn * BN + c;
         if (m >= p.m || n >= p.n) continue;
         const uint32_t at = ring + (r * (BN + 4) + c) * 4;
-        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int k = 0; k < p.splits; ++k) {
-          const float4 q = ld_cluster4(at, k);
-          s.x += q.x;
-          s.y += q.y;
-          s.z += q.z;
-          s.w += q.w;
-        }
-        const float v[4] = {s.x, s.y, s.z, s.w};
+        float4 q[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (n + j < p.n) {
-            if (p.swap)
-              store_one<T>(p, n + j, m, v[j] + (bias ? to_f<T>(bias[m]) : 0.f));
-            else
-              store_one<T>(p, m, n + j, v[j] + (bias ? to_f<T>(bias[n + j]) : 0.f));
+        for (int k = 0; k < 8; ++k)
+          if (k < job.splits) q[k] = ld_cluster4(at, k);
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (k < job.splits) {
+            v[0] += q[k].x;
+            v[1] += q[k].y;
+            v[2] += q[k].z;
+            v[3] += q[k].w;
           }
+        if (p.swap) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (n + j < p.n) store_one<T>(p, n + j, m, v[j] + (bias ? to_f<T>(bias[m]) : 0.f));
+        } else {
+          store_four<T>(p, m, n, v);
+        }
       }
     }
     __syncwarp();
@@ -810,18 +871,25 @@ __global__ void __launch_bounds__(GEMV_THREADS)
 }
 
 // ---- copies, gradients' first step ------------------------------------------------------------------
-// src [rows][cols] with any row stride to dst with rows of `pitch` (a multiple of 8) elements.
-__global__ void __launch_bounds__(256) k_pack(const uint16_t* __restrict__ src, int64_t ld, int64_t rows, int64_t cols, uint16_t* __restrict__ dst,
-                                              int64_t pitch) {
+// src [rows][cols] with any row stride to dst with rows of `pitch` (a multiple of 8) elements; blockIdx.z chooses one of
+// two.
+struct PackJob {
+  struct {
+    const uint16_t* src;
+    uint16_t* dst;
+    int64_t ld, rows, cols, pitch;
+  } one[2];
+};
+__global__ void __launch_bounds__(256) k_pack(const __grid_constant__ PackJob job) {
+  const auto& j = job.one[blockIdx.z];
   const int64_t c0 = ((int64_t)blockIdx.x * 32 + (threadIdx.x & 31)) * 8;
-  if (c0 >= cols) return;
-  for (int64_t r = (int64_t)blockIdx.y * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.y * 8) {
-    Pack<__half, 8> o;
+  if (c0 >= j.cols) return;
+  for (int64_t r = (int64_t)blockIdx.y * 8 + (threadIdx.x >> 5); r < j.rows; r += (int64_t)gridDim.y * 8) {
     uint16_t v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c0 + i < cols ? __ldg(src + r * ld + c0 + i) : (uint16_t)0;
-    o.w = make_uint4(v[0] | (uint32_t)v[1] << 16, v[2] | (uint32_t)v[3] << 16, v[4] | (uint32_t)v[5] << 16, v[6] | (uint32_t)v[7] << 16);
-    *reinterpret_cast<uint4*>(dst + r * pitch + c0) = o.w;
+    for (int i = 0; i < 8; ++i) v[i] = c0 + i < j.cols ? __ldg(j.src + r * j.ld + c0 + i) : (uint16_t)0;
+    *reinterpret_cast<uint4*>(j.dst + r * j.pitch + c0) =
+        make_uint4(v[0] | (uint32_t)v[1] << 16, v[2] | (uint32_t)v[3] << 16, v[4] | (uint32_t)v[5] << 16, v[6] | (uint32_t)v[7] << 16);
   }
 }
 
@@ -933,18 +1001,26 @@ struct Workspace {
   }
 };
 
-int pack_operand(Operand& o, Workspace& ws, cudaStream_t st) {
-  if (o.tma_ok()) return FV_OK;
-  const int64_t pitch = pad8(o.inner());
-  uint16_t* dst = static_cast<uint16_t*>(ws.take((size_t)o.outer() * (size_t)pitch * 2));
+// Copies of those of two operands that TMA cannot read, in one launch.
+int pack_operands(Operand& a, Operand& b, Workspace& ws, cudaStream_t st) {
+  PackJob job{};
+  int count = 0;
+  int64_t most = 0, widest = 0;
+  for (Operand* o : {&a, &b}) {
+    if (o->tma_ok()) continue;
+    const int64_t pitch = pad8(o->inner());
+    uint16_t* dst = static_cast<uint16_t*>(ws.take((size_t)o->outer() * (size_t)pitch * 2));
+    job.one[count++] = {static_cast<const uint16_t*>(o->p), dst, o->ld, o->outer(), o->inner(), pitch};
+    most = std::max(most, o->outer());
+    widest = std::max(widest, o->inner());
+    o->p = dst;
+    o->ld = pitch;
+  }
+  if (!count) return FV_OK;
   FV_REQUIRE(ws.used <= ws.size, FV_ERR_INVALID, "workspace too small: %llu bytes needed so far, got %llu", (unsigned long long)ws.used,
              (unsigned long long)ws.size);
-  const unsigned gx = (unsigned)((o.inner() + 255) / 256);
-  const unsigned gy = (unsigned)std::min<int64_t>((o.outer() + 7) / 8, 4096);
-  k_pack<<<dim3(gx, gy), 256, 0, st>>>(static_cast<const uint16_t*>(o.p), o.ld, o.outer(), o.inner(), dst, pitch);
+  k_pack<<<dim3((unsigned)((widest + 255) / 256), (unsigned)std::min<int64_t>((most + 7) / 8, 4096), (unsigned)count), 256, 0, st>>>(job);
   FV_CUDA(cudaGetLastError());
-  o.p = dst;
-  o.ld = pitch;
   return FV_OK;
 }
 
@@ -986,33 +1062,62 @@ struct Shape {
   int bn, splits;
   bool pair;
 };
-// Tile and split of k: the combination with the least estimated time, in units of one 128 x 64 x 64 product.  A block
-// pays for its k-blocks (bound by the issue of loads below a width of 3 units), about six units to fill the pipeline
-// and drain the tile, and with a split two more for the exchange.
-Shape choose_shape(int64_t m, int64_t n, int64_t kblocks, int sms, bool narrow) {
+struct Size {
+  int64_t m, n, kblocks;
+};
+// Estimated microseconds of one launch, from measurements on a B200: a k-block costs `few` with a handful of blocks at
+// work (bound by the issue of loads up to a width of 128, by the products above) and `many` with all SMs at work (L2, power); a
+// tile's epilogue costs `epi` and runs under the next tile's products; launch, set-up and drain cost 3.5.
+struct Cost {
+  int bn;
+  bool pair;
+  double few, many, epi;
+};
+constexpr Cost COSTS[] = {{256, true, 0.28, 0.36, 4.4}, {256, false, 0.28, 0.42, 4.2}, {128, false, 0.20, 0.235, 2.5}, {64, false, 0.197, 0.20, 1.3}};
+double estimate(const Cost& c, int splits, const Size* sizes, int count, int sms) {
+  const double places = c.pair ? sms / 2 : sms / splits;
+  double tiles = 0, work = 0, longest = 0;
+  for (int i = 0; i < count; ++i) {
+    const int64_t rows = c.pair ? 2 * BM : BM;
+    const double t = (double)((sizes[i].m + rows - 1) / rows) * (double)((sizes[i].n + c.bn - 1) / c.bn);
+    tiles += t;
+  }
+  const double busy = std::min(1.0, tiles / places), kb = c.few + (c.many - c.few) * busy;
+  for (int i = 0; i < count; ++i) {
+    const int64_t rows = c.pair ? 2 * BM : BM;
+    const double t = (double)((sizes[i].m + rows - 1) / rows) * (double)((sizes[i].n + c.bn - 1) / c.bn);
+    const double one = std::max((double)((sizes[i].kblocks + splits - 1) / splits) * kb, tiles > places ? c.epi : 0.0);
+    work += t * one;
+    longest = std::max(longest, one);
+  }
+  const double waves = (double)((int64_t)((tiles + places - 1) / places));
+  const double run = tiles <= places ? longest : count == 1 ? waves * longest : std::max(work / places, longest) + 0.1 * longest;
+  return 3.5 + run + c.epi + (splits > 1 ? 1.5 + 0.3 * splits + c.epi : 0.0);
+}
+// Tile shape and split of k with the least estimate.
+Shape choose_shape(const Size* sizes, int count, int sms, bool narrow, double* time) {
   Shape best{64, 1, false};
   double least = 1e300;
-  for (int bn : {512, 256, 128, 64}) {  // 512: a pair on 256 x 256
-    if (narrow && bn > 64) continue;
-    const bool pair = bn == 512;
-    const int64_t tm = (m + (pair ? 2 * BM : BM) - 1) / (pair ? 2 * BM : BM), tn = (n + (pair ? 256 : bn) - 1) / (pair ? 256 : bn);
-    const double tiles = (double)tm * (double)tn, places = pair ? sms / 2 : sms;
+  for (const Cost& c : COSTS) {
+    if (narrow && c.bn > 64) continue;
     for (int s : {1, 2, 4, 8}) {
-      if (s > 1 && (pair || s > kblocks || tiles * s > sms)) break;
-      const double waves = (double)((int64_t)((tiles * s + places - 1) / places));
-      const double width = pair ? 4.0 : bn == 256 ? 4.6 : bn == 128 ? 3.2 : 2.9;
-      const double t = waves * ((double)((kblocks + s - 1) / s) * width + bn / 64.0) + 6.0 + (s > 1 ? 2.0 + width : 0.0);
+      if (s > 1) {  // one tile per cluster: all of them at once
+        const double tiles = (double)((sizes[0].m + BM - 1) / BM) * (double)((sizes[0].n + c.bn - 1) / c.bn);
+        if (c.pair || count > 1 || s > sizes[0].kblocks || tiles * s > sms) break;
+      }
+      const double t = estimate(c, s, sizes, count, sms);
       if (t < least) {
         least = t;
-        best = {pair ? 256 : bn, s, pair};
+        best = {c.bn, s, c.pair};
       }
     }
   }
+  if (time) *time = least;
   return best;
 }
 
 template <typename T, int BN, bool PAIR>
-int launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& y, const GemmParams& p, unsigned grid, int splits, cudaStream_t st) {
+int launch_gemm(const GemmMaps& maps, const GemmJob& job, unsigned grid, int splits, cudaStream_t st) {
   static size_t given[64] = {0};
   FV_CUDA(allow_smem((const void*)k_gemm<T, BN, PAIR>, given, GEMM_SMEM));
   cudaLaunchConfig_t cfg{};
@@ -1026,40 +1131,52 @@ int launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& y
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = PAIR || splits > 1 ? 1 : 0;
-  FV_CUDA(cudaLaunchKernelEx(&cfg, k_gemm<T, BN, PAIR>, a, b, y, p));
+  FV_CUDA(cudaLaunchKernelEx(&cfg, k_gemm<T, BN, PAIR>, maps, job));
   return FV_OK;
 }
 
-// D = A B^T with the epilogue that `p` describes (its output side is filled in by the caller).
-int gemm(Operand a, Operand b, int dtype, GemmParams p, Workspace& ws, int sms, bool narrow, cudaStream_t st) {
-  if (int rc = pack_operand(a, ws, st)) return rc;
-  if (int rc = pack_operand(b, ws, st)) return rc;
-  p.m = a.rows;
-  p.n = b.rows;
-  p.kblocks = (int)((a.depth + BK - 1) / BK);
-  const Shape s = choose_shape(p.m, p.n, p.kblocks, sms, narrow);
-  p.splits = s.splits;
+// One product D = A B^T with the epilogue that `p` describes (its output side is filled in by the caller).
+struct Product {
+  Operand a, b;
+  GemmParams p;
+};
+Size size_of(const Product& d) { return Size{d.a.rows, d.b.rows, (d.a.depth + BK - 1) / BK}; }
+
+int gemm(Product* d, int count, int dtype, const Shape& s, int sms, cudaStream_t st) {
+  GemmMaps maps{};
+  GemmJob job{};
+  job.splits = s.splits;
   const int rows = s.pair ? 2 * BM : BM;
-  p.tiles_m = (int)((p.m + rows - 1) / rows);
-  p.tiles_n = (int)((p.n + s.bn - 1) / s.bn);
-  FV_REQUIRE((int64_t)p.tiles_m * p.tiles_n < (1ll << 30), FV_ERR_INVALID, "the product is too large");
-  p.a_mn = a.mn;
-  p.b_mn = b.mn;
-  const uint32_t type = dtype == FV_BF16 ? 1u : 0u;
-  p.idesc = 1u << 4 | type << 7 | type << 10 | (uint32_t)a.mn << 15 | (uint32_t)b.mn << 16 | (uint32_t)(s.bn / 8) << 17 | (uint32_t)(rows / 16) << 24;
-  CUtensorMap ma, mb, my{};
-  if (!p.swap && s.splits == 1 && p.vec_y)
-    if (int rc = make_out_map(&my, p.y, p.m, p.n, p.out_f32 ? FV_F32 : dtype)) return rc;
-  if (int rc = make_map(&ma, a, dtype, BM)) return rc;
-  if (int rc = make_map(&mb, b, dtype, s.pair ? s.bn / 2 : s.bn)) return rc;
-  const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
+  int64_t tiles = 0;
+  for (int i = 0; i < count; ++i) {
+    GemmParams& p = d[i].p;
+    const Operand &a = d[i].a, &b = d[i].b;
+    p.m = a.rows;
+    p.n = b.rows;
+    p.kblocks = (int)((a.depth + BK - 1) / BK);
+    p.tiles_m = (int)((p.m + rows - 1) / rows);
+    p.tiles_n = (int)((p.n + s.bn - 1) / s.bn);
+    tiles += (int64_t)p.tiles_m * p.tiles_n;
+    FV_REQUIRE(tiles < (1ll << 30), FV_ERR_INVALID, "the product is too large");
+    if (i == 0) job.tiles0 = (int)tiles;
+    p.a_mn = a.mn;
+    p.b_mn = b.mn;
+    const uint32_t type = dtype == FV_BF16 ? 1u : 0u;
+    p.idesc = 1u << 4 | type << 7 | type << 10 | (uint32_t)a.mn << 15 | (uint32_t)b.mn << 16 | (uint32_t)(s.bn / 8) << 17 | (uint32_t)(rows / 16) << 24;
+    if (!p.swap && s.splits == 1 && p.vec_y)
+      if (int rc = make_out_map(&maps.y[i], p.y, p.m, p.n, p.out_f32 ? FV_F32 : dtype)) return rc;
+    if (int rc = make_map(&maps.a[i], a, dtype, BM)) return rc;
+    if (int rc = make_map(&maps.b[i], b, dtype, s.pair ? s.bn / 2 : s.bn)) return rc;
+    job.p[i] = p;
+  }
+  job.tiles = (int)tiles;
   const unsigned grid = (unsigned)(s.splits > 1 ? tiles * s.splits : std::min<int64_t>(tiles, s.pair ? sms / 2 : sms) * (s.pair ? 2 : 1));
   auto go = [&](auto tag) {
     using T = decltype(tag);
-    return s.pair        ? launch_gemm<T, 256, true>(ma, mb, my, p, grid, 1, st)
-           : s.bn == 256 ? launch_gemm<T, 256, false>(ma, mb, my, p, grid, s.splits, st)
-           : s.bn == 128 ? launch_gemm<T, 128, false>(ma, mb, my, p, grid, s.splits, st)
-                         : launch_gemm<T, 64, false>(ma, mb, my, p, grid, s.splits, st);
+    return s.pair        ? launch_gemm<T, 256, true>(maps, job, grid, 1, st)
+           : s.bn == 256 ? launch_gemm<T, 256, false>(maps, job, grid, s.splits, st)
+           : s.bn == 128 ? launch_gemm<T, 128, false>(maps, job, grid, s.splits, st)
+                         : launch_gemm<T, 64, false>(maps, job, grid, s.splits, st);
   };
   return dtype == FV_BF16 ? go(__nv_bfloat16{}) : go(__half{});
 }
@@ -1197,11 +1314,12 @@ int fv_linear(int device, void* stream, const void* x, int64_t x_rs, int64_t x_c
     return FV_OK;
   }
   Workspace ws{static_cast<uint8_t*>(workspace), workspace_bytes};
-  if (rows <= NARROW_ROWS) {
-    p.swap = 1;
-    return gemm(ow, ox, dtype, p, ws, sms, true, st);
-  }
-  return gemm(ox, ow, dtype, p, ws, sms, false, st);
+  if (int rc = pack_operands(ox, ow, ws, st)) return rc;
+  const bool narrow = rows <= NARROW_ROWS;  // w's rows on the wide side of the tiles
+  p.swap = narrow;
+  Product d = narrow ? Product{ow, ox, p} : Product{ox, ow, p};
+  const Size size = size_of(d);
+  return gemm(&d, 1, dtype, choose_shape(&size, 1, sms, narrow, nullptr), sms, st);
 }
 
 // dz is written when there is an activation, or when dy cannot be read by TMA.
@@ -1279,16 +1397,23 @@ int fv_linear_backward(int device, void* stream, const void* dy, int64_t dy_stri
   if (dtype == FV_BF16) first(__nv_bfloat16{});
   else first(__half{});
   FV_CUDA(cudaGetLastError());
-  if (int rc = pack_operand(ox, ws, st)) return rc;
-  if (int rc = pack_operand(ow, ws, st)) return rc;
-  GemmParams p{};
-  p.y = dx;
-  p.ldy = inner;
-  p.vec_y = vec_ok(dx, inner, 2, 16);
-  if (int rc = gemm(od, transposed(ow), dtype, p, ws, sms, false, st)) return rc;
-  p.y = dw;
-  p.vec_y = vec_ok(dw, inner, 2, 16);
-  return gemm(transposed(od), transposed(ox), dtype, p, ws, sms, false, st);
+  if (int rc = pack_operands(ox, ow, ws, st)) return rc;
+  GemmParams px{}, pw{};
+  px.y = dx;
+  pw.y = dw;
+  px.ldy = pw.ldy = inner;
+  px.vec_y = vec_ok(dx, inner, 2, 16);
+  pw.vec_y = vec_ok(dw, inner, 2, 16);
+  Product d[2] = {{od, transposed(ow), px}, {transposed(od), transposed(ox), pw}};
+  if (rows > outer) std::swap(d[0], d[1]);  // the one with the longer sums first, so that the short tiles fill the end
+  const Size sizes[2] = {size_of(d[0]), size_of(d[1])};
+  double one = 0, two[2] = {0, 0};
+  const Shape joint = choose_shape(sizes, 2, sms, false, &one);
+  const Shape each[2] = {choose_shape(&sizes[0], 1, sms, false, &two[0]), choose_shape(&sizes[1], 1, sms, false, &two[1])};
+  if (one <= two[0] + two[1]) return gemm(d, 2, dtype, joint, sms, st);
+  for (int i = 0; i < 2; ++i)
+    if (int rc = gemm(&d[i], 1, dtype, each[i], sms, st)) return rc;
+  return FV_OK;
 }
 
 }  // extern "C"
