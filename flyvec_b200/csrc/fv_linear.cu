@@ -250,7 +250,7 @@ __device__ __forceinline__ void cluster_barrier() {
 constexpr int BM = 128, BK = 64;                 // tile rows, depth of a k-block
 constexpr int RING_BYTES = 192 << 10;            // operand ring
 constexpr int EPI_WARPS = 8;
-constexpr int GEMM_THREADS = 64 + 32 * EPI_WARPS;
+constexpr int GEMM_THREADS = 96 + 32 * EPI_WARPS; // loads of A, products, epilogue, loads of B
 constexpr int STAGE_OUT = 32 * 128;              // an epilogue warp's staging: 32 rows of 128 bytes
 constexpr int GEMM_SMEM = 1024 + RING_BYTES + EPI_WARPS * (STAGE_OUT + 128) + 256;  // + 32 floats of bias a warp
 
@@ -272,9 +272,26 @@ struct GemmMaps {
 };
 struct GemmJob {
   GemmParams p[2];
-  int tiles0, tiles;  // of the first product, of both
+  int tiles0, tiles;  // of the first product (the one with the longer sums), of both
   int splits;
+  int spare;          // tiles of the second product that cost as much as one of the first
 };
+// The k-th tile of place c of `places` (blocks, pairs or clusters); -1 after the last.  The first product's tiles go round
+// the places; those that get none in the last round take `spare` tiles of the second product meanwhile, whose other
+// tiles go round all places.
+__device__ __forceinline__ int tile_of(const GemmJob& j, int c, int k, int places) {
+  const int rounds = j.tiles0 / places, rest = j.tiles0 - rounds * places, idle = places - rest;
+  if (k < rounds) return c + k * places;
+  k -= rounds;
+  int i;
+  if (c < rest) {
+    if (k == 0) return rounds * places + c;
+    i = j.spare * idle + c + (k - 1) * places;
+  } else {
+    i = k < j.spare ? c - rest + k * idle : j.spare * idle + c + (k - j.spare) * places;
+  }
+  return j.tiles0 + i < j.tiles ? j.tiles0 + i : -1;
+}
 
 // Where a tile lies.  Tiles are taken in bands of 16 row tiles, column by column within a band, so that the blocks
 // at work at one time share operand tiles in L2.
@@ -512,33 +529,29 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
   auto first_k = [&](const GemmParams& p) { return (int)((int64_t)p.kblocks * rank / job.splits); };
   auto last_k = [&](const GemmParams& p) { return (int)((int64_t)p.kblocks * (rank + 1) / job.splits); };
 
-  if (warp == 0) {
-    if (elect_one()) {  // loads
+  if (warp == 0 || warp == 2 + EPI_WARPS) {
+    // loads: one thread for A and one for B, because one alone issues a load every 0.09 us
+    const bool is_a = warp == 0;
+    if (elect_one()) {
       int s = 0, phase = 0, issued = 0;
       bool ok = true;
-      for (int t = first; t < job.tiles && ok; t += step) {
+      for (int i = 0, t; ok && (t = tile_of(job, first, i, step)) >= 0; ++i) {
         int tm, tn;
         const int which = locate(t, tm, tn);
         const GemmParams& p = job.p[which];
-        const CUtensorMap *map_a = &maps.a[which], *map_b = &maps.b[which];
-        const int kb1 = last_k(p);
+        const CUtensorMap* map = is_a ? &maps.a[which] : &maps.b[which];
+        const bool mn = is_a ? p.a_mn : p.b_mn;
+        const int kb1 = last_k(p), row = is_a ? (PAIR ? tm * 2 + side : tm) * BM : tn * BN + side * BROWS;
         for (int kb = first_k(p); kb < kb1; ++kb) {
           if (!(ok = mbar_wait(empty(s), phase ^ 1, stop))) break;
-          const uint32_t a = ring + s * STAGE, b = a + A_BYTES;
-          const int ra = PAIR ? tm * 2 * BM + side * BM : tm * BM, rb = tn * BN + side * BROWS;
+          const uint32_t to = ring + s * STAGE + (is_a ? 0 : A_BYTES);
           const uint32_t bar = PAIR ? cluster_addr(full(s), 0) : full(s);  // a pair's loads report to its first block
-          if (side == 0) mbar_expect(full(s), PAIR ? 2 * STAGE : STAGE);
-          if (p.a_mn) {
-#pragma unroll
-            for (int j = 0; j < BM / 64; ++j) tma_load<PAIR>(a + j * 8192, map_a, ra + j * 64, kb * BK, bar);
+          if (is_a && side == 0) mbar_expect(full(s), PAIR ? 2 * STAGE : STAGE);
+          if (mn) {
+            const int panels = (is_a ? BM : BROWS) / 64;
+            for (int j = 0; j < panels; ++j) tma_load<PAIR>(to + j * 8192, map, row + j * 64, kb * BK, bar);
           } else {
-            tma_load<PAIR>(a, map_a, kb * BK, ra, bar);
-          }
-          if (p.b_mn) {
-#pragma unroll
-            for (int j = 0; j < BROWS / 64; ++j) tma_load<PAIR>(b + j * 8192, map_b, rb + j * 64, kb * BK, bar);
-          } else {
-            tma_load<PAIR>(b, map_b, kb * BK, rb, bar);
+            tma_load<PAIR>(to, map, kb * BK, row, bar);
           }
           ++issued;
           if (++s == STAGES) {
@@ -547,9 +560,9 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
           }
         }
       }
-      if (!ok && side == 0) {  // the copies in flight must land before the block (the pair: both meet below) ends
+      if (!ok && side == 0 && is_a) {  // the copies in flight must land before the block (the pair: both meet below) ends
         volatile int never = 0;
-        for (int i = 0; i < STAGES && i < issued; ++i) {
+        for (int k = 0; k < STAGES && k < issued; ++k) {
           if (--s < 0) {
             s = STAGES - 1;
             phase ^= 1;
@@ -562,7 +575,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
     if (side == 0 && elect_one()) {  // products
       int s = 0, phase = 0, acc = 0, acc_phase = 0;
       bool ok = true;
-      for (int t = first; t < job.tiles && ok; t += step) {
+      for (int i = 0, t; ok && (t = tile_of(job, first, i, step)) >= 0; ++i) {
         const GemmParams& p = job.p[t >= job.tiles0];
         // one 16-deep step inside a 64-deep k-block: 32 bytes along k-major rows, 16 rows of 128 bytes otherwise
         const uint32_t a_step = p.a_mn ? 2048 : 32, b_step = p.b_mn ? 2048 : 32;
@@ -604,7 +617,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
     uint8_t* stage = staging + (warp - 2) * STAGE_OUT;
     float* bias_slice = bias_slices + (warp - 2) * 32;
     int acc = 0, acc_phase = 0;
-    for (int t = first; t < job.tiles; t += step) {
+    for (int i = 0, t; (t = tile_of(job, first, i, step)) >= 0; ++i) {
       int tm, tn;
       const int which = locate(t, tm, tn);
       const GemmParams& p = job.p[which];
@@ -1073,7 +1086,7 @@ struct Cost {
   bool pair;
   double few, many, epi;
 };
-constexpr Cost COSTS[] = {{256, true, 0.28, 0.36, 4.4}, {256, false, 0.28, 0.42, 4.2}, {128, false, 0.20, 0.235, 2.5}, {64, false, 0.197, 0.20, 1.3}};
+constexpr Cost COSTS[] = {{256, true, 0.28, 0.36, 4.4}, {256, false, 0.28, 0.42, 4.2}, {128, false, 0.165, 0.23, 2.5}, {64, false, 0.165, 0.175, 1.3}};
 double estimate(const Cost& c, int splits, const Size* sizes, int count, int sms) {
   const double places = c.pair ? sms / 2 : sms / splits;
   double tiles = 0, work = 0, longest = 0;
@@ -1170,6 +1183,8 @@ int gemm(Product* d, int count, int dtype, const Shape& s, int sms, cudaStream_t
     job.p[i] = p;
   }
   job.tiles = (int)tiles;
+  // with a remainder round of the first product; an epilogue is worth about a dozen k-blocks
+  if (count == 2) job.spare = std::max(job.p[0].kblocks, 12) / std::max(job.p[1].kblocks, 12);
   const unsigned grid = (unsigned)(s.splits > 1 ? tiles * s.splits : std::min<int64_t>(tiles, s.pair ? sms / 2 : sms) * (s.pair ? 2 : 1));
   auto go = [&](auto tag) {
     using T = decltype(tag);
@@ -1405,7 +1420,7 @@ int fv_linear_backward(int device, void* stream, const void* dy, int64_t dy_stri
   px.vec_y = vec_ok(dx, inner, 2, 16);
   pw.vec_y = vec_ok(dw, inner, 2, 16);
   Product d[2] = {{od, transposed(ow), px}, {transposed(od), transposed(ox), pw}};
-  if (rows > outer) std::swap(d[0], d[1]);  // the one with the longer sums first, so that the short tiles fill the end
+  if (rows > outer) std::swap(d[0], d[1]);  // the one with the longer sums first
   const Size sizes[2] = {size_of(d[0]), size_of(d[1])};
   double one = 0, two[2] = {0, 0};
   const Shape joint = choose_shape(sizes, 2, sms, false, &one);
