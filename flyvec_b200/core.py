@@ -191,3 +191,47 @@ class FlyVec:
         """Context-dependent codes of windows of input ids (centre id offset by the
         vocabulary size), weighted by ``inv_freq`` when given."""
         return self.hasher.hash_windows(idx, inv_freq=inv_freq, hash_length=hash_length, packed=packed)
+
+    # -- words by their dense embeddings ---------------------------------------
+    @cached_property
+    def _word_table(self):
+        """Every word's dense embedding, standardised over its neurons, bfloat16 ``[V][K]`` on the GPU."""
+        from . import ops
+
+        V = self.hasher.V
+        return ops.layer_norm(self.hasher.activations(np.arange(V, 2 * V, dtype=np.int32)[:, None]), out_dtype="bfloat16")
+
+    def word_log_probs(self, idx, words, beta: float = 20.0, top: int = 0):
+        """How well words fit contexts: ``softmax(beta * r)`` over the vocabulary, ``r`` the correlation (over the
+        neurons) of a context's dense activation with a word's dense embedding.
+
+        ``idx``: int32 ``[n][w]`` input ids of the contexts as in :meth:`hash_windows` (negative: padding); ``words``: ``[n]`` token
+        ids, -1 for none.  Returns :class:`flyvec_b200.ops.TokenLogProbs` of host arrays: the words' log probabilities, the
+        entropies and the ``top`` best words with theirs.  The products are taken in bfloat16 with float sums."""
+        from . import ops
+        from .engine import DeviceArray
+
+        idx = np.ascontiguousarray(idx, np.int32)
+        words = np.ascontiguousarray(words, np.int64).reshape(-1)
+        if idx.ndim != 2 or len(words) != len(idx):
+            raise ValueError(f"idx must have shape [n][w] and words [n], got {idx.shape} and {words.shape}")
+        K, V, table = self.hasher.K, self.hasher.V, self._word_table
+        chunk = max(1, (256 << 20) // (4 * V))  # rows of scores held at once
+        parts = []
+        for a in range(0, max(len(idx), 1), chunk):
+            x = ops.layer_norm(self.hasher.activations(idx[a:a + chunk]), out_dtype="bfloat16")
+            scores = ops.linear(x, table, out_dtype="float32")  # K times the correlations
+            r = ops.token_log_probs(scores, DeviceArray.from_numpy(words[a:a + chunk], device=self.device), beta=beta / K, top=top)
+            parts.append([None if v is None else v.numpy() for v in r])
+        return ops.TokenLogProbs(*(None if v[0] is None else np.concatenate(v) for v in zip(*parts)))
+
+    def similar_words(self, word: str, top: int = 10, beta: float = 20.0):
+        """The ``top`` words whose dense embeddings correlate best with that of the first token of ``word``, itself left
+        out: a list of ``(token, log probability)`` under :meth:`word_log_probs`; empty for an unknown word."""
+        if self.is_unknown_token(word):
+            return []
+        tok_id = self.tokenizer.token2id(self.tokenizer.tokenize(word)[0])
+        V = self.hasher.V
+        r = self.word_log_probs([[V + tok_id]], [tok_id], beta=beta, top=min(top + 1, V))
+        found = [(self.tokenizer.id2token(int(i)), float(p)) for i, p in zip(r.top_ids[0], r.top_log_prob[0]) if i != tok_id]
+        return found[:top]

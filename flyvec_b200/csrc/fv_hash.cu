@@ -614,7 +614,57 @@ int create_hasher(fv_hasher* hs, const float* w_kn, int K, int N, int normalize,
 
 }  // namespace
 
+namespace {
+// Dense activations of windows: out[i][mu] = sum over the window's ids of wt[id][mu], added in double as the reference
+// does and stored as float.  A warp per window; the ids are few, so every lane walks over all of them.
+__global__ void __launch_bounds__(256)
+    k_activations(HDev h, const int32_t* __restrict__ idx, uint64_t n, int window, float* __restrict__ out) {
+  const uint64_t i = ((uint64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  const int lane = threadIdx.x & 31;
+  if (i >= n) return;
+  const int32_t* ids = idx + i * window;
+  for (int k = lane; k < h.K; k += 32) {
+    double s = 0.0;
+    for (int c = 0; c < window; ++c) {
+      const int id = ids[c];
+      if (id < 0) continue;  // padding
+      if (id >= h.N) {
+        if (k == 0) atomicOr(h.error, FV_DEVERR_TOKEN_RANGE);
+        continue;
+      }
+      s += (double)h.wt[(size_t)id * h.Kp + k];
+    }
+    out[i * h.K + k] = (float)s;
+  }
+}
+}  // namespace
+
 extern "C" {
+
+int fv_hasher_activations(fv_hasher* hs, const int32_t* idx, uint64_t nwin, uint32_t window, float* d_out) {
+  FV_REQUIRE(hs && (nwin == 0 || (idx && d_out)), FV_ERR_INVALID, "fv_hasher_activations: NULL argument");
+  FV_REQUIRE(window >= 1 && window <= 32, FV_ERR_INVALID, "window must be in [1, 32], got %u", window);
+  FV_REQUIRE(nwin < (1ull << 32), FV_ERR_INVALID, "too many windows: %llu", (unsigned long long)nwin);
+  if (nwin == 0) return FV_OK;
+  fv::DeviceGuard guard(hs->device);
+  FV_REQUIRE(guard.ok, FV_ERR_CUDA, "cannot select device %d", hs->device);
+  int32_t* d_idx = nullptr;
+  const size_t bytes = (size_t)nwin * window * sizeof(int32_t);
+  FV_CUDA(cudaMalloc((void**)&d_idx, bytes));
+  uint32_t err = 0;
+  cudaError_t e = cudaMemsetAsync(hs->d_err, 0, sizeof(uint32_t), hs->stream);
+  if (e == cudaSuccess) e = cudaMemcpyAsync(d_idx, idx, bytes, cudaMemcpyHostToDevice, hs->stream);
+  if (e == cudaSuccess) {
+    k_activations<<<(unsigned)((nwin + 7) / 8), 256, 0, hs->stream>>>(hs->h, d_idx, nwin, (int)window, d_out);
+    e = cudaGetLastError();
+  }
+  if (e == cudaSuccess) e = cudaMemcpyAsync(&err, hs->d_err, sizeof(err), cudaMemcpyDeviceToHost, hs->stream);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(hs->stream);
+  cudaFree(d_idx);
+  FV_CUDA(e);
+  if (err & FV_DEVERR_TOKEN_RANGE) return fv::fail(FV_ERR_DATA, "an input id was out of range (device check)");
+  return FV_OK;
+}
 
 int fv_hasher_create(const float* w_kn, uint32_t hid, uint32_t n_cols, int normalize, float prec, int device,
                      fv_hasher** out) {

@@ -372,6 +372,16 @@ class Hasher:
                                          hash_length, flags, ptr(out)))
         return out if packed else out.view(np.int8)
 
+    def activations(self, idx) -> "DeviceArray":
+        """Dense activations float32 ``[n][K]``, on the GPU, of windows of input ids int32 ``[n][w]`` (as for
+        :meth:`hash_windows`; negative ids are padding, a target word's id has the vocabulary size added)."""
+        idx = as_c(idx, np.int32)
+        if idx.ndim != 2:
+            raise ValueError(f"idx must have shape [n][w], got {idx.shape}")
+        out = DeviceArray((idx.shape[0], self.K), "float32", self.device)
+        check(_lib.lib().fv_hasher_activations(self._h, ptr(idx), idx.shape[0], idx.shape[1], C.c_void_p(out.ptr)))
+        return out
+
     def set_inverse_frequency(self, f):
         f = as_c(f, np.float32)
         check(_lib.lib().fv_hasher_set_inverse_frequency(self._h, ptr(f), f.size))
@@ -479,6 +489,12 @@ class DeviceArray(DeviceBuffer):
 
     def is_neg(self) -> bool:
         return False
+
+    def is_contiguous(self) -> bool:
+        return True
+
+    def numel(self) -> int:
+        return self.size
 
     def stride(self):
         out, step = [], 1

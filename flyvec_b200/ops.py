@@ -112,7 +112,7 @@ def _matrix(x, what: str):
 
 
 def _empty(like, shape, dtype: str):
-    if type(like) is DeviceArray:
+    if isinstance(like, DeviceArray):
         return like.new_empty(shape, dtype)
     t = _torch_types.get(dtype)
     if t is None:
@@ -122,7 +122,7 @@ def _empty(like, shape, dtype: str):
 
 def _floats(like, n: int, shape):
     """n float32 arrays of one shape."""
-    if type(like) is DeviceArray:
+    if isinstance(like, DeviceArray):
         return [like.new_empty(shape, "float32") for _ in range(n)]
     return _empty(like, (n, *shape), "float32").unbind(0)  # one allocation
 
@@ -130,7 +130,7 @@ def _floats(like, n: int, shape):
 def _stream(x, device: int):
     """Handle of the stream the work goes to."""
     global _raw_stream
-    if type(x) is DeviceArray:
+    if isinstance(x, DeviceArray):
         return None
     if _raw_stream is None:
         torch = sys.modules["torch"]
@@ -145,9 +145,9 @@ def _ptr(x):
 def _vector(x, n: int, what: str, like, types):
     """A dense vector of n elements (any shape of n elements is taken in order)."""
     _check(x, what, types, like)
-    if (x.size if type(x) is DeviceArray else x.numel()) != n:
+    if x.numel() != n:
         raise ValueError(f"{what} must have {n} elements, got shape {tuple(x.shape)}")
-    return x if type(x) is DeviceArray or x.is_contiguous() else x.contiguous()
+    return x if x.is_contiguous() else x.contiguous()
 
 
 def _same_shape(x, shape, what: str):

@@ -260,6 +260,10 @@ int fv_hasher_create(const float* w_kn, uint32_t hid, uint32_t n_cols, int norma
 int fv_hasher_destroy(fv_hasher* h);
 /* The (possibly normalised) matrix back in checkpoint layout. */
 int fv_hasher_get_weights(fv_hasher* h, float* w_kn);
+/* Dense (unweighted) activations of windows of input ids, the vectors that fv_hash_windows with FV_HASH_RAW thresholds:
+ * d_out, device memory, float [nwin][K]; idx, host memory, int32 [nwin][window], negative ids are padding, a target
+ * word's id has the vocabulary size added.  Returns when d_out is written. */
+int fv_hasher_activations(fv_hasher* h, const int32_t* idx, uint64_t nwin, uint32_t window, float* d_out);
 /* FlyVec.get_sparse_embedding (flyvec/core.py:139-163) for a batch of token ids:
  * activations = column V+id, code = activation > midpoint of the hash_length-th
  * and next largest; id 0 gives zeros. */

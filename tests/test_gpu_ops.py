@@ -522,3 +522,253 @@ def test_linear_backward_empty(built_lib):
     x, w = torch.empty(0, 24, device="cuda", dtype=torch.bfloat16), made((40, 24), "bfloat16", 1)
     dx, dw, db = ops.linear_backward(torch.empty(0, 40, device="cuda", dtype=torch.bfloat16), x, w)
     assert dx.shape == (0, 24) and (dw == 0).all() and (db == 0).all()
+
+
+# ---- how the operators are used ------------------------------------------------------------------------
+def test_arrays_without_pytorch(built_lib):
+    """The same calls on DeviceArray."""
+    rng = np.random.default_rng(3)
+    x = rng.standard_normal((37, 400)).astype(np.float32)
+    a = DeviceArray.from_numpy(x)
+    y, mean, rstd = ops.layer_norm(a, return_stats=True)
+    t = torch.from_numpy(x).cuda()
+    ty, tm, tr = ops.layer_norm(t, return_stats=True)
+    assert isinstance(y, DeviceArray) and y.shape == (37, 400)
+    np.testing.assert_array_equal(y.numpy(), ty.cpu().numpy())
+    np.testing.assert_array_equal(rstd.numpy(), tr.cpu().numpy())
+    w = rng.standard_normal((90, 400)).astype(np.float32)
+    xb, wb = DeviceArray.from_numpy(x, "bfloat16"), DeviceArray.from_numpy(w, "bfloat16")
+    np.testing.assert_array_equal(xb.numpy(), t.bfloat16().float().cpu().numpy())  # rounded to nearest even
+    tw = torch.from_numpy(w).cuda().bfloat16()
+    s, ts = ops.linear(xb, wb, out_dtype="float32"), ops.linear(t.bfloat16(), tw, out_dtype="float32")
+    np.testing.assert_array_equal(s.numpy(), ts.cpu().numpy())
+    dy = DeviceArray.from_numpy(rng.standard_normal((37, 90)), "bfloat16")
+    for got, want in zip(ops.linear_backward(dy, xb, wb), ops.linear_backward(torch.from_numpy(dy.numpy()).cuda().bfloat16(), t.bfloat16(), tw)):
+        np.testing.assert_array_equal(got.numpy(), want.float().cpu().numpy())
+    ids = rng.integers(0, 90, 37)
+    r, tr_ = ops.token_log_probs(s, DeviceArray.from_numpy(ids), top=5), ops.token_log_probs(ts, torch.from_numpy(ids).cuda(), top=5)
+    for got, want in zip(r, tr_):
+        np.testing.assert_array_equal(got.numpy(), want.cpu().numpy())
+    one = DeviceArray.from_numpy(np.ones(37, np.float32))
+    d = ops.token_log_probs_backward(one, s, DeviceArray.from_numpy(ids), r.row_max, r.log_z, r.entropy, grad_entropy=one)
+    td = ops.token_log_probs_backward(torch.ones(37, device="cuda"), ts, torch.from_numpy(ids).cuda(), tr_.row_max, tr_.log_z, tr_.entropy,
+                                      grad_entropy=torch.ones(37, device="cuda"))
+    np.testing.assert_array_equal(d.numpy(), td.cpu().numpy())
+    with pytest.raises(TypeError, match="first argument"):
+        ops.layer_norm(a, torch.ones(400, device="cuda"))
+    half = DeviceArray.from_numpy(np.array([1.5, np.nan, -np.inf], np.float32), "float16").numpy()
+    assert half.dtype == np.float16 and half[0] == 1.5 and np.isnan(half[1]) and half[2] == -np.inf
+
+
+def head_forward(p, x, t):
+    """A readout: norm, hidden layer with a residual around it, norm, vocabulary, the token's log probability."""
+    h0, m0, r0 = ops.layer_norm(x, p["g0"], p["b0"], return_stats=True)
+    h1, z1 = ops.linear(h0, p["w1"], p["c1"], activation="gelu", residual=x, return_preactivation=True)
+    h2, m2, r2 = ops.layer_norm(h1, p["g2"], p["b2"], return_stats=True)
+    s = ops.linear(h2, p["w3"], p["c3"])
+    return ops.token_log_probs(s, t, top=3), (h0, m0, r0, h1, z1, h2, m2, r2, s)
+
+
+def head_backward(p, x, t, r, saved, g):
+    h0, m0, r0, h1, z1, h2, m2, r2, s = saved
+    ds = ops.token_log_probs_backward(g, s, t, r.row_max, r.log_z)
+    d = {}
+    dh2, d["w3"], d["c3"] = ops.linear_backward(ds, h2, p["w3"])
+    dh1, d["g2"], d["b2"] = ops.layer_norm_backward(dh2, h1, m2, r2, p["g2"])
+    dh0, d["w1"], d["c1"] = ops.linear_backward(dh1, h0, p["w1"], preactivation=z1, activation="gelu")
+    dx, d["g0"], d["b0"] = ops.layer_norm_backward(dh0, x, m0, r0, p["g0"])
+    return dx + dh1, d
+
+
+def head_problem(n=300, K=136, V=1003, seed=1):
+    p = {"g0": made((K,), "bfloat16", seed, 0, 0.2, 1.0), "b0": made((K,), "bfloat16", seed + 1, 0, 0.2), "w1": made((K, K), "bfloat16", seed + 2, 0, K ** -0.5),
+         "c1": made((K,), "bfloat16", seed + 3, 0, 0.2), "g2": made((K,), "bfloat16", seed + 4, 0, 0.2, 1.0), "b2": made((K,), "bfloat16", seed + 5, 0, 0.2),
+         "w3": made((V, K), "bfloat16", seed + 6, 0, K ** -0.5), "c3": made((V,), "bfloat16", seed + 7, 0, 0.2)}
+    x = made((n, K), "bfloat16", seed + 8)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    t = torch.randint(0, V, (n,), generator=g, device="cuda")
+    t[::17] = -1
+    return p, x, t
+
+
+def test_a_run_of_them_together(built_lib):
+    p, x, t = head_problem()
+    r, saved = head_forward(p, x, t)
+    up = torch.full((300,), 1.0 / 300, device="cuda")
+    dx, d = head_backward(p, x, t, r, saved, up)
+    # the same in 64 bits with automatic differentiation
+    q = {k: v.double().requires_grad_() for k, v in p.items()}
+    x64 = x.double().requires_grad_()
+    F = torch.nn.functional
+    h = F.layer_norm(x64, (136,), q["g0"], q["b0"])
+    h = ACTS["gelu"](h @ q["w1"].t() + q["c1"]) + x64
+    h = F.layer_norm(h, (136,), q["g2"], q["b2"])
+    lp = F.log_softmax(h @ q["w3"].t() + q["c3"], -1)
+    want = lp.gather(1, t.clamp_min(0)[:, None])[:, 0].masked_fill(t < 0, 0.0)
+    want.mean().backward()
+    # a chain of bfloat16 values: each of the 5 tensors between the operators is off by 2^-9 of its size, a logit of size about 3 by
+    # a few of these together
+    assert (r.log_prob.double() - want).abs().max() < 10 * 3 * 2.0 ** -8
+    for k, v in list(d.items()) + [("x", dx)]:
+        g = x64.grad if k == "x" else q[k].grad
+        rel = ((v.double() - g).norm() / g.norm()).item()
+        assert rel < 10 * 2.0 ** -8, (k, rel)
+
+
+def test_captured_and_replayed(built_lib):
+    """A training step captured once and replayed on new inputs gives what the calls give; two graphs share nothing."""
+    p, x, t = head_problem()
+    p2, x2, t2 = head_problem(n=300, seed=50)
+    up = torch.full((300,), 1.0 / 300, device="cuda")
+    run = lambda pp, xx, tt: (lambda r, s: (r.log_prob, *head_backward(pp, xx, tt, r, s, up)[1].values()))(*head_forward(pp, xx, tt))  # noqa: E731
+    want1, want2 = run(p, x, t), run(p2, x2, t2)
+    sx, st = x.clone(), t.clone()
+    sx2, st2 = x2.clone(), t2.clone()
+    run(p, sx, st)
+    torch.cuda.synchronize()
+    g1, g2 = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g1):
+        out1 = run(p, sx, st)
+    with torch.cuda.graph(g2):
+        out2 = run(p2, sx2, st2)
+    for _ in range(2):
+        g1.replay()
+        g2.replay()
+    g1.replay()
+    torch.cuda.synchronize()
+    for a, b in list(zip(out1, want1)) + list(zip(out2, want2)):
+        assert torch.equal(a, b)
+    x3 = made((300, 136), "bfloat16", 99)
+    sx.copy_(x3)
+    g1.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(out1, run(p, x3, t)):
+        assert torch.equal(a, b)
+
+
+def test_streams(built_lib):
+    """Work goes to the current stream; calls on two streams at once do not disturb each other."""
+    p, x, t = head_problem(n=2000)
+    p2, x2, t2 = head_problem(n=2000, seed=50)
+    want, want2 = head_forward(p, x, t)[0], head_forward(p2, x2, t2)[0]
+    torch.cuda.synchronize()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    outs = []
+    for _ in range(5):
+        with torch.cuda.stream(a):
+            outs.append((head_forward(p, x, t)[0], want))
+        with torch.cuda.stream(b):
+            outs.append((head_forward(p2, x2, t2)[0], want2))
+    torch.cuda.synchronize()
+    for r, w in outs:
+        for u, v in zip(r, w):
+            assert torch.equal(u, v)
+    # a slow producer on a side stream: the call waits for it because it runs on the same stream
+    with torch.cuda.stream(a):
+        big = torch.zeros(4000, 4000, device="cuda")
+        for _ in range(20):
+            big = big @ big
+        z = x * 2 + big[0, 0].bfloat16()
+        got = ops.layer_norm(z)
+    torch.cuda.synchronize()
+    assert torch.equal(got, ops.layer_norm(x * 2))
+
+
+def test_rows_behind_the_last_stay_as_they_were(built_lib):
+    """Outputs lie in larger buffers where the allocator puts them: nothing beyond their ends is written."""
+    import ctypes as C
+
+    from flyvec_b200 import _lib
+
+    lib = _lib.lib()
+    for rows, inner, outer in ((129, 64, 96), (130, 64, 103), (5, 64, 200), (2, 64, 30), (300, 4096, 300)):
+        x, w = made((rows, inner), "bfloat16", 1), made((outer, inner), "bfloat16", 2)
+        buf = torch.full((rows * outer + 512,), 7.0, device="cuda", dtype=torch.bfloat16)
+        st = torch.cuda.current_stream().cuda_stream
+        assert lib.fv_linear(0, st, x.data_ptr(), inner, 1, w.data_ptr(), inner, 1, rows, inner, outer, 1, None, 0, None, 0, buf.data_ptr(), 1, None,
+                             None, 0) == 0
+        assert (buf[rows * outer:] == 7).all()
+        assert torch.equal(buf[: rows * outer].view(rows, outer), ops.linear(x, w))
+    for cols in (400, 1001, 4097):
+        x = made((9, cols), "bfloat16", 3)
+        buf = torch.full((9 * cols + 512,), 7.0, device="cuda", dtype=torch.bfloat16)
+        assert lib.fv_layer_norm(0, torch.cuda.current_stream().cuda_stream, x.data_ptr(), cols, 9, cols, 1, None, None, 1e-5, buf.data_ptr(), 1,
+                                 None, None) == 0
+        assert (buf[9 * cols:] == 7).all() and torch.equal(buf[: 9 * cols].view(9, cols), ops.layer_norm(x))
+
+
+def test_tensors_that_need_gradients(built_lib):
+    x = torch.randn(3, 8, device="cuda", requires_grad=True)
+    with pytest.raises(ValueError, match="detach"):
+        ops.layer_norm(x)
+    with torch.no_grad():
+        assert torch.equal(ops.layer_norm(x), ops.layer_norm(x.detach()))
+    par = torch.nn.Parameter(torch.ones(8, device="cuda"), requires_grad=False)
+    assert torch.equal(ops.layer_norm(x.detach(), par), ops.layer_norm(x.detach()))
+    neg = torch.view_as_complex(torch.randn(3, 8, 2, device="cuda")).conj().imag
+    assert neg.is_neg()
+    with pytest.raises(ValueError, match="negated|contiguous"):
+        ops.layer_norm(neg)
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_another_device_than_the_current_one(built_lib):
+    p, x, t = head_problem()
+    want = head_forward(p, x, t)[0]
+    got = head_forward({k: v.to("cuda:1") for k, v in p.items()}, x.to("cuda:1"), t.to("cuda:1"))[0]
+    for a, b in zip(got, want):
+        assert a.device.index == 1 and torch.equal(a.cpu(), b.cpu())
+
+
+# ---- words by their dense embeddings ---------------------------------------------------------------------
+def test_window_activations(built_lib):
+    from flyvec_b200 import _lib, synth
+    from flyvec_b200.engine import Hasher
+
+    W = synth.make_weights(70, 2 * 90, seed=3)
+    h = Hasher(W)
+    rng = np.random.default_rng(1)
+    idx = rng.integers(-1, 180, (50, 7)).astype(np.int32)
+    ext = np.concatenate([W.astype(np.float64), np.zeros((70, 1))], 1)  # -1 is padding
+    np.testing.assert_array_equal(h.activations(idx).numpy(), ext[:, idx].sum(-1).T.astype(np.float32))
+    assert h.activations(np.zeros((0, 3), np.int32)).shape == (0, 70)
+    with pytest.raises(_lib.FlyvecError, match="out of range"):
+        h.activations(np.array([[180]]))
+    with pytest.raises(ValueError):
+        h.activations(np.zeros(3, np.int32))
+    h.close()
+
+
+def test_word_log_probs_and_similar_words(built_lib, tmp_path):
+    from flyvec_b200 import FlyVec, synth
+
+    K, V = 64, 500
+    W = synth.make_weights(K, 2 * V, seed=2)
+    W[:, V + 8] = W[:, V + 7] + 0.1 * W[:, V + 9]  # a near twin of word 7
+    np.save(tmp_path / "syn.npy", W)
+    (tmp_path / "vocab.txt").write_text("\n".join(["<UNK>"] + [f"w{i}" for i in range(1, V)]))
+    (tmp_path / "config.yaml").write_text("synapses: syn.npy\ntokenizer: vocab.txt\n")
+    m = FlyVec.from_config(tmp_path / "config.yaml")
+    rng = np.random.default_rng(5)
+    idx = rng.integers(0, V, (40, 4)).astype(np.int32)
+    words = rng.integers(0, V, 40)
+    words[3] = -1
+    r = m.word_log_probs(idx, words, beta=12.0, top=5)
+    z = lambda a: (a - a.mean(1, keepdims=True)) / a.std(1, keepdims=True)  # noqa: E731
+    corr = z(W[:, idx].sum(-1).T.astype(np.float64)) @ z(W[:, V:].T.astype(np.float64)).T / K
+    s = 12.0 * corr
+    lse = np.log(np.exp(s - s.max(1, keepdims=True)).sum(1)) + s.max(1)
+    want = np.where(words < 0, 0.0, s[np.arange(40), words] - lse)
+    # standardised values are rounded to bfloat16: a product of two is off by 2^-8 of its size at most, their sum of K such by
+    # 2^-8 of the sum of their magnitudes, at most 1 in units of the correlation (Cauchy and Schwarz); the maximum may move as much
+    tol = 2 * 12.0 * 2.0 ** -8 * 1.01
+    assert np.abs(r.log_prob - want).max() < tol
+    assert r.top_ids.shape == (40, 5)
+    best = np.take_along_axis(s, r.top_ids.astype(np.int64), 1)
+    assert (best[:, -1] >= np.sort(s, 1)[:, -5] - tol).all()
+    near = m.similar_words("w7", top=4)
+    assert len(near) == 4 and near[0][0] == "w8" and all(a[1] >= b[1] for a, b in zip(near, near[1:])) and "w7" not in dict(near)
+    assert m.similar_words("nothere") == []
+    with pytest.raises(ValueError):
+        m.word_log_probs(idx, words[:3])
