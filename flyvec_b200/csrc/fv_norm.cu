@@ -358,13 +358,16 @@ __global__ void __launch_bounds__(NORM_MAX_THREADS)
   }
 }
 
-// dx, and with a weight the block's partial sums of dw and db in part[blockIdx.x][2][D].
+// dx, and with a weight the block's partial sums of dw and db in part[blockIdx.x][2][D].  16-bit rows of at most two words
+// a thread keep h and u in registers between the sums and dx (16384 x 4096: 84 us; formed again from shared memory 97 us);
+// with four words, and for float, the registers cost more than the second reading.
 template <typename T, int NV, bool BLOCK, bool EDGE>
 __global__ void __launch_bounds__(BLOCK ? NORM_MAX_THREADS : 32 * NORM_WARPS)
     k_norm_grad(const T* __restrict__ dy, int64_t gs, const T* __restrict__ x, int64_t xs, int64_t rows, int D,
                 const float* __restrict__ mean, const float* __restrict__ rstd, const T* __restrict__ w, T* __restrict__ dx,
                 float* __restrict__ part, int stages, int pitch) {
   constexpr int VEC = 16 / (int)sizeof(T);
+  constexpr bool KEEP = sizeof(T) == 2 && NV <= 2;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ __align__(16) float red[2][16][2];
   const Group<BLOCK> g;
@@ -425,14 +428,16 @@ __global__ void __launch_bounds__(BLOCK ? NORM_MAX_THREADS : 32 * NORM_WARPS)
       for (int i = 0; i < VEC / 2; ++i) h[i] = mul2(add2(h[i], both(-mu)), both(rs));
     };
     float2 a = both(0.f), q = both(0.f);
+    float2 hk[NV][VEC / 2], uk[NV][VEC / 2];
 #pragma unroll
     for (int j = 0; j < NV; ++j)
       if (col.any(j)) {
-        float2 h[VEC / 2], gv[VEC / 2];
+        float2 (&h)[VEC / 2] = hk[j];
+        float2 gv[VEC / 2];
         row_values(j, h, gv);
 #pragma unroll
         for (int i = 0; i < VEC / 2; ++i) {
-          const float2 u = mul2(gv[i], pw[j][i]);
+          const float2 u = uk[j][i] = mul2(gv[i], pw[j][i]);
           a = add2(a, u);
           q = fma2(u, h[i], q);
           dw[j][i] = fma2(gv[i], h[i], dw[j][i]);
@@ -447,12 +452,16 @@ __global__ void __launch_bounds__(BLOCK ? NORM_MAX_THREADS : 32 * NORM_WARPS)
 #pragma unroll
     for (int j = 0; j < NV; ++j)
       if (col.any(j)) {
-        float2 h[VEC / 2], gv[VEC / 2];
-        row_values(j, h, gv);
+        if constexpr (!KEEP) {
+          float2 gv[VEC / 2];
+          row_values(j, hk[j], gv);
+#pragma unroll
+          for (int i = 0; i < VEC / 2; ++i) uk[j][i] = mul2(gv[i], pw[j][i]);
+        }
         Pack<T, VEC> o;
 #pragma unroll
         for (int i = 0; i < VEC / 2; ++i) {
-          const float2 d = mul2(both(rs), fma2(h[i], both(-mq), add2(mul2(gv[i], pw[j][i]), both(-ma))));
+          const float2 d = mul2(both(rs), fma2(hk[j][i], both(-mq), add2(uk[j][i], both(-ma))));
           o.e[2 * i] = from_f<T>(d.x);
           o.e[2 * i + 1] = from_f<T>(d.y);
         }
@@ -596,7 +605,7 @@ NormPlan plan_norm(int64_t rows, int64_t D, int dtype, bool grad, bool edge, int
     p.words = !grad && dtype != FV_F32 ? 4 : 2;
     while (words > (int64_t)p.words * NORM_MAX_THREADS) p.words *= 2;
     p.threads = (int)(((words + p.words - 1) / p.words + 31) / 32 * 32);
-    per_sm = std::max(1, std::min(16, (grad ? 768 : 1024) / p.threads));
+    per_sm = std::max(1, std::min(16, (!grad ? 1024 : dtype == FV_F32 ? 768 : 512) / p.threads));
   }
   const int64_t fixed = (int64_t)groups * RING_MOST * 8, stage = (int64_t)groups * arrays * p.pitch;
   while (per_sm > 1 && (208 << 10) / per_sm < fixed + 2 * stage) --per_sm;
