@@ -358,23 +358,21 @@ __device__ __forceinline__ void stage_out(const uint8_t* stage, void* out, int64
   }
   __syncwarp();
 }
-// The staged 64 columns of 16 bits to an array by plain stores, whole lines where its rows admit 16-byte words; unlike
-// the asynchronous copy it is done with the staging rows when it returns.
-__device__ __forceinline__ void copy_out(const uint8_t* stage, void* out, int64_t ld, bool vec, int64_t r0, int64_t c0, int64_t rows,
+// One staged half (32 columns of 16 bits) to an array by plain stores; unlike the asynchronous copy it is done with the
+// staging rows when it returns.
+__device__ __forceinline__ void copy_out(const uint8_t* stage, void* out, int64_t ld, bool vec, int half, int64_t r0, int64_t c0, int64_t rows,
                                          int64_t cols) {
-  if (!vec || c0 + 64 > cols) {
-    stage_out(stage, out, ld, 2, 0, r0, c0, rows, cols);
-    if (c0 + 32 < cols) stage_out(stage, out, ld, 2, 1, r0, c0 + 32, rows, cols);
+  if (!vec || c0 + 32 > cols) {
+    stage_out(stage, out, ld, 2, half, r0, c0, rows, cols);
     return;
   }
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, c = (lane & 3) + 4 * half;
   __syncwarp();
-  uint8_t* base = static_cast<uint8_t*>(out) + ((r0 + lane / 8) * ld + c0) * 2 + (lane & 7) * 16;
+  uint8_t* base = static_cast<uint8_t*>(out) + ((r0 + lane / 4) * ld + c0) * 2 + (lane & 3) * 16;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const int r = lane / 8 + 4 * k;
-    if (r0 + r < rows)
-      *reinterpret_cast<uint4*>(base + 8 * k * ld) = *reinterpret_cast<const uint4*>(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+  for (int k = 0; k < 4; ++k) {
+    const int r = lane / 4 + 8 * k;
+    if (r0 + r < rows) *reinterpret_cast<uint4*>(base + 16 * k * ld) = *reinterpret_cast<const uint4*>(stage + r * 128 + ((c ^ (r & 7)) << 4));
   }
   __syncwarp();
 }
@@ -617,23 +615,42 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
     uint8_t* stage = staging + (warp - 2) * STAGE_OUT;
     float* bias_slice = bias_slices + (warp - 2) * 32;
     int acc = 0, acc_phase = 0;
-    for (int i = 0, t; (t = tile_of(job, first, i, step)) >= 0; ++i) {
+    // The residual is fetched a slice ahead and the bias a tile ahead, over the tile's end: their latency would be waited
+    // for with the accumulator ready otherwise.
+    uint4 early[8];
+    float bias_reg[4], bias_next[4];  // of this warp's two slices, a column a lane
+    auto fetch_ahead = [&](int t, bool of_residual) {
+      if (t < 0 || job.splits > 1) return;
+      int tm, tn;
+      const int which = locate(t, tm, tn);
+      const GemmParams& p = job.p[which];
+      if (p.swap) return;
+      if (of_residual) {
+        if (p.residual && half * 64 < BN)
+          fetch_in(early, p.residual, p.ldr, p.vec_r, (int64_t)(PAIR ? tm * 2 + side : tm) * BM + quarter * 32, (int64_t)tn * BN + half * 64, p.m,
+                   p.n);
+      } else if (p.bias) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int64_t c = (int64_t)tn * BN + half * 64 + (j >> 1) * 128 + (j & 1) * 32 + lane;
+          bias_next[j] = c < p.n ? to_f<T>(static_cast<const T*>(p.bias)[c]) : 0.f;
+        }
+      }
+    };
+    int t_next = tile_of(job, first, 0, step);
+    fetch_ahead(t_next, true);
+    fetch_ahead(t_next, false);
+    for (int i = 0, t; (t = t_next) >= 0; ++i) {
       int tm, tn;
       const int which = locate(t, tm, tn);
       const GemmParams& p = job.p[which];
       const T* bias = static_cast<const T*>(p.bias);
       const int64_t r0 = (int64_t)(PAIR ? tm * 2 + side : tm) * BM + quarter * 32;
-      uint4 early[8];
-      if (p.residual && job.splits == 1 && !p.swap && half * 64 < BN)
-        fetch_in(early, p.residual, p.ldr, p.vec_r, r0, (int64_t)tn * BN + half * 64, p.m, p.n);
-      float bias_reg[4];  // this warp's two slices, a column a lane
-      if (bias && job.splits == 1 && !p.swap) {
+      t_next = tile_of(job, first, i + 1, step);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int64_t c = (int64_t)tn * BN + half * 64 + (j >> 1) * 128 + (j & 1) * 32 + lane;
-          bias_reg[j] = c < p.n ? to_f<T>(bias[c]) : 0.f;
-        }
-      }
+      for (int j = 0; j < 4; ++j) bias_reg[j] = bias_next[j];
+      fetch_ahead(t_next, false);
+      bool ahead = false;  // the next tile's first residual slice is on its way
       if (!mbar_wait(acc_full(acc), acc_phase, stop)) break;
       tc_fence_after();
       const uint32_t src = tmem + acc * BN + ((uint32_t)(quarter * 32) << 16);
@@ -666,21 +683,28 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
         for (int c = half * 64; c < BN; c += 128) {
           const int64_t c0 = (int64_t)tn * BN + c;
           if (c0 >= p.n || r0 >= p.m) continue;
-          uint4 res[8];  // the residual's row, then the result's
-          if (p.residual) {
-            stage_free();
-            stage_in(stage, early, p.residual, p.ldr, p.vec_r, r0, c0, p.m, p.n);
-            if (c + 128 < BN) fetch_in(early, p.residual, p.ldr, p.vec_r, r0, c0 + 128, p.m, p.n);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) res[k] = *reinterpret_cast<const uint4*>(stage + lane * 128 + ((k ^ (lane & 7)) << 4));
-            __syncwarp();
-          } else if (p.z) {
-            stage_free();
-          }
+          // A lane's staging row holds the residual's words, then in their place the pre-activation's on their way out, then the
+          // result's (a float result fills the whole row: the residual is staged again for the second half).
+          uint8_t* mine = stage + lane * 128;
+          auto word = [&](int k) { return reinterpret_cast<uint4*>(mine + ((k ^ (lane & 7)) << 4)); };
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int64_t ch = c0 + 32 * h;
             if (ch >= p.n) break;
+            if (h == 0 || p.out_f32) {
+              stage_free();
+              if (p.residual) {
+                stage_in(stage, early, p.residual, p.ldr, p.vec_r, r0, c0, p.m, p.n);
+                if (h == 1 || !p.out_f32 || c0 + 32 >= p.n) {  // no longer needed
+                  if (c + 128 < BN && c0 + 128 < p.n) {
+                    fetch_in(early, p.residual, p.ldr, p.vec_r, r0, c0 + 128, p.m, p.n);
+                  } else {
+                    fetch_ahead(t_next, true);
+                    ahead = true;
+                  }
+                }
+              }
+            }
             float v[32];
             if (bias) bias_slice[lane] = bias_reg[c >= 128 ? 2 + h : h];
             tmem_load32(src + c + 32 * h, v);
@@ -698,54 +722,45 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
               }
               __syncwarp();  // the slice may be written again
             }
+            uint4 res[4];
+            if (p.residual) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) res[k] = *word(4 * h + k);
+            }
             if (p.z) {
               stage_row<T>(stage, lane, v, h);
-              if (p.out_f32) stage_out(stage, p.z, p.ldz, 2, h, r0, ch, p.m, p.n);
+              copy_out(stage, p.z, p.ldz, p.vec_z, h, r0, ch, p.m, p.n);
             }
             act_values(v, p.act);
             if (p.residual) {
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
                 Pack<T, 8> w;
-                w.w = res[4 * h + k];
+                w.w = res[k];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[8 * k + i] += to_f<T>(w.e[i]);
+                for (int i = 0; i < 8; i += 2) {
+                  const float2 u = add2(make_float2(v[8 * k + i], v[8 * k + i + 1]), make_float2(to_f<T>(w.e[i]), to_f<T>(w.e[i + 1])));
+                  v[8 * k + i] = u.x;
+                  v[8 * k + i + 1] = u.y;
+                }
               }
             }
             if (p.out_f32) {
-              if (!p.z) stage_free();
+              __syncwarp();  // the other lanes have read their residual
               stage_row_f32(stage, lane, v);
               if (p.vec_y)
                 stage_store(stage, &maps.y[which], r0, ch);
               else
                 stage_out(stage, p.y, p.ldy, 4, 0, r0, ch, p.m, p.n);
-              if (p.z) stage_free();
             } else {
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                Pack<T, 8> o;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) o.e[i] = from_f<T>(v[8 * k + i]);
-                res[4 * h + k] = o.w;
-              }
+              stage_row<T>(stage, lane, v, h);
+              if (!p.vec_y) stage_out(stage, p.y, p.ldy, 2, h, r0, ch, p.m, p.n);
             }
           }
-          if (!p.out_f32) {
-            if (p.z)
-              copy_out(stage, p.z, p.ldz, p.vec_z, r0, c0, p.m, p.n);
-            else if (!p.residual)
-              stage_free();
-#pragma unroll
-            for (int k = 0; k < 8; ++k) *reinterpret_cast<uint4*>(stage + lane * 128 + ((k ^ (lane & 7)) << 4)) = res[k];
-            if (p.vec_y) {
-              stage_store(stage, &maps.y[which], r0, c0);
-            } else {
-              stage_out(stage, p.y, p.ldy, 2, 0, r0, c0, p.m, p.n);
-              if (c0 + 32 < p.n) stage_out(stage, p.y, p.ldy, 2, 1, r0, c0 + 32, p.m, p.n);
-            }
-          }
+          if (!p.out_f32 && p.vec_y) stage_store(stage, &maps.y[which], r0, c0);
         }
       }
+      if (!ahead) fetch_ahead(t_next, true);  // a tile without a slice for this warp
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
