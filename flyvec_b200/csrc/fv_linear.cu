@@ -836,7 +836,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
 // ---- up to four rows --------------------------------------------------------------------------------
 // G lanes share C output columns: each reads VEC elements of the columns' weight rows at a time and multiplies them with the
 // rows of x, which lie in shared memory in their own type (a 16-byte read per row and VEC elements, no bank conflicts).  Bound
-// by reading w once: 20000 columns of 400, one row: 5.2 us; 4096 of 4096: 7.9 us (out of L2).
+// by reading w once: 20000 columns of 400, one row: 4.3 us; 4096 of 4096: 6.1 us (both out of L2).
 constexpr int GEMV_THREADS = 256, GEMV_CHUNK = 4096;
 template <typename T, int VEC, int G, int MT, int C>
 __global__ void __launch_bounds__(GEMV_THREADS)
@@ -1263,7 +1263,7 @@ extern "C" {
 
 int fv_ops_status(int device, uint32_t* word) {
   FV_REQUIRE(word, FV_ERR_INVALID, "fv_ops_status: NULL argument");
-  fv::DeviceGuard guard(device);
+  OnDevice guard(device);
   FV_REQUIRE(guard.ok, FV_ERR_CUDA, "cannot select device %d", device);
   FV_CUDA(cudaMemcpyFromSymbol(word, g_status, sizeof(uint32_t)));
   if (*word) {
@@ -1306,7 +1306,7 @@ int fv_linear(int device, void* stream, const void* x, int64_t x_rs, int64_t x_c
              "fv_linear: one axis of x and of the weight must be contiguous");
   FV_REQUIRE(workspace_bytes == 0 || (workspace && (uintptr_t)workspace % 256 == 0), FV_ERR_INVALID,
              "fv_linear: the workspace must be 256-byte aligned");
-  fv::DeviceGuard guard(device);
+  OnDevice guard(device);
   const int sms = sm_count(device);
   FV_REQUIRE(guard.ok && sms > 0, FV_ERR_CUDA, "cannot select device %d", device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -1385,7 +1385,7 @@ int fv_linear_backward(int device, void* stream, const void* dy, int64_t dy_stri
   FV_REQUIRE(stride_ok(dy_stride) && stride_ok(z_stride) && stride_ok(x_rs) && stride_ok(x_cs) && stride_ok(w_rs) && stride_ok(w_cs),
              FV_ERR_INVALID, "fv_linear_backward: bad stride");
   FV_REQUIRE(dw && db, FV_ERR_INVALID, "fv_linear_backward: NULL argument");
-  fv::DeviceGuard guard(device);
+  OnDevice guard(device);
   const int sms = sm_count(device);
   FV_REQUIRE(guard.ok && sms > 0, FV_ERR_CUDA, "cannot select device %d", device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -784,7 +784,7 @@ int fv_token_log_probs(int device, void* stream, const void* logits, int64_t str
   if (rows == 0) return FV_OK;
   FV_REQUIRE(logits && targets && log_prob && entropy && row_max && log_z && (top == 0 || (top_ids && top_log_prob)), FV_ERR_INVALID,
              "fv_token_log_probs: NULL argument");
-  fv::DeviceGuard guard(device);
+  OnDevice guard(device);
   const int sms = sm_count(device);
   FV_REQUIRE(guard.ok && sms > 0, FV_ERR_CUDA, "cannot select device %d", device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -827,7 +827,7 @@ int fv_token_log_probs_backward(int device, void* stream, const float* grad_log_
   if (rows == 0) return FV_OK;
   FV_REQUIRE(grad_log_prob && logits && targets && row_max && log_z && (!grad_entropy || entropy) && dlogits, FV_ERR_INVALID,
              "fv_token_log_probs_backward: NULL argument");
-  fv::DeviceGuard guard(device);
+  OnDevice guard(device);
   const int sms = sm_count(device);
   FV_REQUIRE(guard.ok && sms > 0, FV_ERR_CUDA, "cannot select device %d", device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);

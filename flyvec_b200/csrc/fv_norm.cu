@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(BLOCK ? NORM_MAX_THREADS : 32 * NORM_WARPS)
     }
     if (!BLOCK) __syncwarp();
     if (g.t == 0) fetch(r + stages * g.step, s);  // every thread has its part of the stage in registers
-    const float rstd = rsqrtf(var + eps), minus = -shift * rstd;
+    const float rstd = rsqrtf(max_nan(var, 0.f) + eps), minus = -shift * rstd;
     if (g.t == 0) {
       if (mean_out) mean_out[r] = pivot + shift;
       if (rstd_out) rstd_out[r] = rstd;
@@ -701,7 +701,7 @@ int fv_layer_norm(int device, void* stream, const void* x, int64_t x_stride, int
   FV_REQUIRE(!bias || weight, FV_ERR_INVALID, "fv_layer_norm: a bias needs a weight");
   if (rows == 0) return FV_OK;
   FV_REQUIRE(x && y, FV_ERR_INVALID, "fv_layer_norm: NULL argument");
-  fv::DeviceGuard guard(device);
+  OnDevice guard(device);
   const int sms = sm_count(device);
   FV_REQUIRE(guard.ok && sms > 0, FV_ERR_CUDA, "cannot select device %d", device);
   const size_t es = elem_size(dtype);
@@ -755,7 +755,7 @@ int fv_layer_norm_backward(int device, void* stream, const void* dy, int64_t dy_
              "fv_layer_norm_backward: dweight and dbias go with a weight and not without one");
   FV_REQUIRE(rows == 0 || (dy && x && mean && rstd && dx), FV_ERR_INVALID, "fv_layer_norm_backward: NULL argument");
   if (rows == 0 && !weight) return FV_OK;
-  fv::DeviceGuard guard(device);
+  OnDevice guard(device);
   FV_REQUIRE(guard.ok, FV_ERR_CUDA, "cannot select device %d", device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (rows == 0) {

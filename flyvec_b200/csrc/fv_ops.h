@@ -171,6 +171,28 @@ inline bool vec_ok(const void* p, int64_t stride_elems, size_t elem, unsigned by
 }
 inline size_t elem_size(int dtype) { return dtype == FV_F32 ? 4 : 2; }
 
+// Makes `device` current for the scope.  Unlike fv::DeviceGuard it leaves the runtime alone when it already is: two calls
+// of 0.2 us saved where a whole operator call takes ten.
+struct OnDevice {
+  int prev = -1;
+  bool ok = false;
+  explicit OnDevice(int device) {
+    int now = -1;
+    if (cudaGetDevice(&now) != cudaSuccess) return;
+    if (now == device) {
+      ok = true;
+      return;
+    }
+    ok = cudaSetDevice(device) == cudaSuccess;
+    if (ok) prev = now;
+  }
+  ~OnDevice() {
+    if (prev >= 0) cudaSetDevice(prev);
+  }
+  OnDevice(const OnDevice&) = delete;
+  OnDevice& operator=(const OnDevice&) = delete;
+};
+
 // Lets a kernel have `bytes` of dynamic shared memory on the current device; `done` is the kernel's own record of what it was
 // given per device (a race between threads repeats a call that does no harm).
 inline cudaError_t allow_smem(const void* kernel, size_t (&done)[64], size_t bytes) {

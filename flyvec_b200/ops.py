@@ -120,6 +120,13 @@ def _empty(like, shape, dtype: str):
     return like.new_empty(shape, dtype=t)
 
 
+def _like(x):
+    """A dense array of x's shape and type."""
+    if not isinstance(x, DeviceArray) and x.is_contiguous():
+        return sys.modules["torch"].empty_like(x)
+    return _empty(x, x.shape, _type(x))
+
+
 def _floats(like, n: int, shape):
     """n float32 arrays of one shape."""
     if isinstance(like, DeviceArray):
@@ -208,7 +215,7 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, out_dtype: str | No
         weight = _vector(weight, cols, "weight", x, (kind,))
     if bias is not None:
         bias = _vector(bias, cols, "bias", x, (kind,))
-    y, mean, rstd, dev = _empty(x, x.shape, out_dtype), None, None, x.get_device()
+    y, mean, rstd, dev = _like(x) if out_dtype == kind else _empty(x, x.shape, out_dtype), None, None, x.get_device()
     if return_stats:
         lead = x.shape[:-1]
         mean, rstd = _empty(x, lead, "float32"), _empty(x, lead, "float32")
@@ -233,7 +240,7 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None):
     rstd = _vector(rstd, rows, "rstd", x, ("float32",))
     if weight is not None:
         weight = _vector(weight, cols, "weight", x, (kind,))
-    dx = _empty(x, x.shape, kind)
+    dx = _like(x)
     dev, lib = x.get_device(), _lib.lib()
     dw = db = ws = None
     size = 0
@@ -318,7 +325,7 @@ def linear_backward(dy, x, weight, preactivation=None, activation: str | None = 
         _, _, zstep = _rows(preactivation, "preactivation")
     else:
         preactivation = None
-    dx, dw, db = _empty(x, x.shape, kind), _empty(x, (outer, inner), kind), _empty(x, (outer,), kind)
+    dx, dw, db = _like(x), _empty(x, (outer, inner), kind), _empty(x, (outer,), kind)
     dev, pg, px, pw = x.get_device(), dy.data_ptr(), x.data_ptr(), weight.data_ptr()
     size = _linear_backward_workspace(dev, rows, inner, outer, pg & 15, gstep, px & 15, xr, xc, pw & 15, wr, wc, act)
     ws = _empty(x, (size,), "uint8") if size else None
@@ -393,7 +400,7 @@ def token_log_probs_backward(grad_log_prob, logits, targets, row_max, log_z, ent
         entropy = _vector(entropy, rows, "entropy", logits, f32)
     else:
         entropy = None
-    dx, dev = _empty(logits, logits.shape, _type(logits)), logits.get_device()
+    dx, dev = _like(logits), logits.get_device()
     check(_lib.lib().fv_token_log_probs_backward(dev, _stream(logits, dev), grad_log_prob.data_ptr(), _ptr(grad_entropy),
                                                  logits.data_ptr(), step, rows, vocab, DTYPES[_type(logits)], targets.data_ptr(),
                                                  int(_type(targets) == "int64"), row_max.data_ptr(), log_z.data_ptr(), _ptr(entropy), beta,
