@@ -128,6 +128,39 @@ __device__ __forceinline__ float2 exponents(float2 x, float minus_m, float bl2) 
   d.y = max_nan(d.y, -200.f);
   return d;
 }
+// the same from the i-th pair of a word: 16-bit elements are widened by the subtraction itself
+template <typename T>
+__device__ __forceinline__ float2 exponents_of(const uint4& q, int i, float minus_m, float bl2) {
+  float2 x;
+  if constexpr (sizeof(T) == 4) {
+    x = add2(pair_of<T>(q, i), both(minus_m));
+  } else {
+    const unsigned w[4] = {q.x, q.y, q.z, q.w};
+    const unsigned short lo = (unsigned short)w[i], hi = (unsigned short)(w[i] >> 16);
+    if constexpr (std::is_same<T, __half>::value) {
+      asm("add.f32.f16 %0, %1, %2;" : "=f"(x.x) : "h"(lo), "f"(minus_m));
+      asm("add.f32.f16 %0, %1, %2;" : "=f"(x.y) : "h"(hi), "f"(minus_m));
+    } else {
+      asm("add.f32.bf16 %0, %1, %2;" : "=f"(x.x) : "h"(lo), "f"(minus_m));
+      asm("add.f32.bf16 %0, %1, %2;" : "=f"(x.y) : "h"(hi), "f"(minus_m));
+    }
+  }
+  float2 d = mul2(x, both(bl2));
+  d.x = max_nan(d.x, -200.f);
+  d.y = max_nan(d.y, -200.f);
+  return d;
+}
+// the k-th element of a word in registers
+template <typename T>
+__device__ __forceinline__ float element_of(const uint4& q, int k) {
+  constexpr int PER = 4 / (int)sizeof(T);
+  const int i = k / PER;
+  const unsigned w = i < 2 ? (i == 0 ? q.x : q.y) : (i == 2 ? q.z : q.w);
+  if constexpr (PER == 1)
+    return __uint_as_float(w);
+  else
+    return k & 1 ? widen2<T>(w).y : widen2<T>(w).x;
+}
 // N words of elements: one rescaling for all of them, without a branch, then two elements per step.  Returns their
 // maximum.
 template <typename T, int N>
@@ -142,7 +175,7 @@ __device__ __forceinline__ float take(Stream& t, const uint4 (&q)[N], float bl2)
   for (int u = 0; u < N; ++u)
 #pragma unroll
     for (int i = 0; i < 8 / (int)sizeof(T); ++i) {
-      const float2 d = exponents(pair_of<T>(q[u], i), -m0, bl2), z = make_float2(ex2(d.x), ex2(d.y));
+      const float2 d = exponents_of<T>(q[u], i, -m0, bl2), z = make_float2(ex2(d.x), ex2(d.y));
       t.s = add2(t.s, z);
       t.a = fma2(z, d, t.a);
     }
@@ -398,7 +431,7 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS)
         }
         for (; hits; hits &= hits - 1) {
           const int k = __ffs(hits) - 1;
-          offer(to_f<T>(reinterpret_cast<const T*>(vecs + v)[k]), rw.vec_at(v0 + v) + k);
+          offer(element_of<T>(one[0], k), rw.vec_at(v0 + v) + k);
         }
       };
       if (tid < ends) offer(to_f<T>(rw.x[rw.end_at(tid)]), rw.end_at(tid));
@@ -406,7 +439,7 @@ __global__ void __launch_bounds__(THREADS, 1280 / THREADS)
         // the batches that reach the bound are listed, then their words are dealt to all threads
         if (my_key >= floor_key) {
           for (int b = 0; b < min(batch, LP_SLOTS); ++b)
-            if (key_of(slot_max[b][tid]) >= floor_key) {
+            if (!(slot_max[b][tid] < floor_value) && key_of(slot_max[b][tid]) >= floor_key) {
               const unsigned place = atomicAdd(&n_listed, 1u);
               if (place < LP_LIST) listed[place] = (unsigned short)(tid * LP_SLOTS + b);
             }
