@@ -23,6 +23,11 @@
 // TMA needs 16-byte aligned rows.  Operands without them are copied once into rows of a multiple of 8 elements
 // (k_pack) in the caller's workspace; everything else is read where it lies.
 //
+// What bounds it: large products the tensor cores under the power limit (8192 x 8192 x 2048, bf16: 178 us, 1.55 PFLOP/s,
+// cuBLAS 177 us); with pre-activation, gelu and residual the epilogue (232 us: eight warps take 17 us a tile where the products
+// take 13); small ones launch, set-up and drain (about 5 us) and 0.16 us per k-block, the rate at which one thread
+// issues loads.  256 x 256 pairs halve what a block reads of B: 0.36 instead of 0.42 us per k-block with all SMs at work.
+//
 // Roundings to 16 bits: the outputs, and dz before it enters the two products (as tensor-core operands have to be; db
 // is formed from the unrounded dz).
 //
@@ -311,10 +316,9 @@ __device__ __forceinline__ void stage_row(uint8_t* stage, int row, const float (
   uint8_t* base = stage + row * 128;
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
-    Pack<T, 8> o;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o.e[i] = from_f<T>(v[8 * c + i]);
-    *reinterpret_cast<uint4*>(base + (((c + 4 * half) ^ (row & 7)) << 4)) = o.w;
+    const float2 q[4] = {make_float2(v[8 * c], v[8 * c + 1]), make_float2(v[8 * c + 2], v[8 * c + 3]), make_float2(v[8 * c + 4], v[8 * c + 5]),
+                         make_float2(v[8 * c + 6], v[8 * c + 7])};
+    *reinterpret_cast<uint4*>(base + (((c + 4 * half) ^ (row & 7)) << 4)) = word_of<T>(q);
   }
 }
 __device__ __forceinline__ void stage_row_f32(uint8_t* stage, int row, const float (&v)[32]) {
@@ -735,11 +739,9 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
             if (p.residual) {
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
-                Pack<T, 8> w;
-                w.w = res[k];
 #pragma unroll
                 for (int i = 0; i < 8; i += 2) {
-                  const float2 u = add2(make_float2(v[8 * k + i], v[8 * k + i + 1]), make_float2(to_f<T>(w.e[i]), to_f<T>(w.e[i + 1])));
+                  const float2 u = add2(make_float2(v[8 * k + i], v[8 * k + i + 1]), pair_of<T>(res[k], i / 2));
                   v[8 * k + i] = u.x;
                   v[8 * k + i + 1] = u.y;
                 }
@@ -927,7 +929,7 @@ template <typename T, int VEC, int ACT>
 __global__ void __launch_bounds__(256)
     k_act_grad(const T* __restrict__ dy, int64_t ldg, const T* __restrict__ z, int64_t ldz, int64_t rows, int64_t outer,
                T* __restrict__ dz, int64_t pitch, float* __restrict__ part) {
-  constexpr int ROWS = 4;
+  constexpr int ROWS = ACT == FV_ACT_NONE ? 4 : 2;  // with an activation four rows cost registers and 5 % of the time
   __shared__ float sum[8][32 * VEC];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t c = ((int64_t)blockIdx.x * 32 + lane) * VEC;
@@ -947,15 +949,22 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
       for (int k = 0; k < ROWS; ++k)
         if (r + 8 * k < r1) {
+          if constexpr (VEC == 8) {
+            float2 v[4];
 #pragma unroll
-          for (int i = 0; i < VEC; i += 2) {
-            constexpr int one = VEC > 1;
-            float2 v = make_float2(to_f<T>(g[k].e[i]), to_f<T>(g[k].e[i + one]));
-            if (ACT != FV_ACT_NONE) v = mul2(v, act_slope<ACT>(make_float2(to_f<T>(q[k].e[i]), to_f<T>(q[k].e[i + one]))));
-            s[i] += v.x;
-            if (one) s[i + one] += v.y;
-            g[k].e[i] = from_f<T>(v.x);
-            if (one) g[k].e[i + one] = from_f<T>(v.y);
+            for (int i = 0; i < 4; ++i) {
+              v[i] = pair_of<T>(g[k].w, i);
+              if (ACT != FV_ACT_NONE) v[i] = mul2(v[i], act_slope<ACT>(pair_of<T>(q[k].w, i)));
+              const float2 t = add2(make_float2(s[2 * i], s[2 * i + 1]), v[i]);
+              s[2 * i] = t.x;
+              s[2 * i + 1] = t.y;
+            }
+            g[k].w = word_of<T>(v);
+          } else {
+            float2 v = both(to_f<T>(g[k].e[0]));
+            if (ACT != FV_ACT_NONE) v = mul2(v, act_slope<ACT>(both(to_f<T>(q[k].e[0]))));
+            s[0] += v.x;
+            g[k].e[0] = from_f<T>(v.x);
           }
           if (dz) store_pack<T, VEC>(dz + (r + 8 * k) * pitch + c, g[k]);
         }

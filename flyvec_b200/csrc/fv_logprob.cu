@@ -18,6 +18,10 @@
 // top-th largest element, only the threads whose maximum reaches it (about 2 top of 256) have anything to offer, and
 // their words are read again (L2).  The few candidates are ranked by counting (value first, then the lower index).
 // Rows of at most 1024 elements go to one warp each.
+//
+// 10000 x 20000 bf16: 73 us (5.5 TB/s) without alternatives, bound by the issue of ex2 and the arithmetic around it; 97 us with
+// ten, whose search (two more barriers, a second trip to L2) hides only in part behind the other blocks' rows.  4096 x 50000
+// float: 131 us (6.2 TB/s) and 155 us.  1280 threads per SM: 1024 are 5 % slower, 1536 spill.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -83,25 +87,6 @@ struct Stream {
   float m;
   float2 s, a;
 };
-// two elements of a 32-bit word (one element for float: the caller passes two words)
-template <typename T>
-__device__ __forceinline__ float2 widen2(unsigned w);
-template <>
-__device__ __forceinline__ float2 widen2<__nv_bfloat16>(unsigned w) {
-  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-}
-template <>
-__device__ __forceinline__ float2 widen2<__half>(unsigned w) {
-  return __half22float2(*reinterpret_cast<__half2*>(&w));
-}
-template <typename T>
-__device__ __forceinline__ float2 pair_of(const uint4& q, int i) {  // i-th pair of a 16-byte word
-  const unsigned w[4] = {q.x, q.y, q.z, q.w};
-  if constexpr (sizeof(T) == 4)
-    return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
-  else
-    return widen2<T>(w[i]);
-}
 // largest element (NaN if there is one) of N 16-byte words
 template <typename T, int N>
 __device__ __forceinline__ float words_max(const uint4 (&q)[N]) {
@@ -706,7 +691,8 @@ __device__ __forceinline__ GradRow grad_row(int64_t row, long long t, int64_t V,
   r.c1 = r.empty ? 0.f : -beta * r.gh * LN2;
   return r;
 }
-// A block takes `chunk` columns of one row; the vectors are aligned to the gradient, which is dense.
+// A block takes some 1024 words of one row, four to a thread; they are aligned to the gradient, which is dense.  Bound by
+// memory: 4096 x 50000, bf16 132 us (6.2 TB/s read and written), float 259 us (6.3 TB/s); half as many words a block 170 us.
 template <typename T>
 __global__ void __launch_bounds__(256)
     k_log_probs_grad(const T* __restrict__ logits, int64_t xs, int64_t V, int chunks, const void* __restrict__ targets, int t64,
@@ -749,12 +735,10 @@ __global__ void __launch_bounds__(256)
         const int64_t at = rw.vec_at(i);
         const int64_t ahead = t - at;
         Pack<T, VEC> o;
+        float2 d[VEC / 2];
 #pragma unroll
-        for (int k = 0; k < VEC; k += 2) {
-          const float2 d = grad_of(r, make_float2(to_f<T>(w[u].e[k]), to_f<T>(w[u].e[k + 1])));
-          o.e[k] = from_f<T>(d.x);
-          o.e[k + 1] = from_f<T>(d.y);
-        }
+        for (int k = 0; k < VEC / 2; ++k) d[k] = grad_of(r, pair_of<T>(w[u].w, k));
+        o.w = word_of<T>(d);
         if (ahead >= 0 && ahead < VEC) {
 #pragma unroll
           for (int k = 0; k < VEC; ++k)

@@ -117,6 +117,47 @@ __device__ __forceinline__ float2 fma2(float2 x, float2 y, float2 z) {
   return unpack2(r);
 }
 
+// two 16-bit elements of a 32-bit word as floats, and back (one conversion for both)
+template <typename T>
+__device__ __forceinline__ float2 widen2(unsigned w);
+template <>
+__device__ __forceinline__ float2 widen2<__nv_bfloat16>(unsigned w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ float2 widen2<__half>(unsigned w) {
+  return __half22float2(*reinterpret_cast<__half2*>(&w));
+}
+template <typename T>
+__device__ __forceinline__ unsigned join2(float2 v);
+template <>
+__device__ __forceinline__ unsigned join2<__nv_bfloat16>(float2 v) {
+  const __nv_bfloat162 r = __floats2bfloat162_rn(v.x, v.y);
+  return *reinterpret_cast<const unsigned*>(&r);
+}
+template <>
+__device__ __forceinline__ unsigned join2<__half>(float2 v) {
+  const __half2 r = __floats2half2_rn(v.x, v.y);
+  return *reinterpret_cast<const unsigned*>(&r);
+}
+// the i-th pair of elements of a 16-byte word
+template <typename T>
+__device__ __forceinline__ float2 pair_of(const uint4& q, int i) {
+  const unsigned w[4] = {q.x, q.y, q.z, q.w};
+  if constexpr (sizeof(T) == 4)
+    return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+  else
+    return widen2<T>(w[i]);
+}
+// a 16-byte word of pairs
+template <typename T>
+__device__ __forceinline__ uint4 word_of(const float2 (&v)[8 / sizeof(T)]) {
+  if constexpr (sizeof(T) == 4)
+    return make_uint4(__float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x), __float_as_uint(v[1].y));
+  else
+    return make_uint4(join2<T>(v[0]), join2<T>(v[1]), join2<T>(v[2]), join2<T>(v[3]));
+}
+
 // Sums of the columns of part[P][n] in a fixed order, 32 columns to a block of 512 threads: four columns to a thread, 64
 // rows at a time, then a tree.  `out(c, v)` is called once per column.
 template <typename F>
