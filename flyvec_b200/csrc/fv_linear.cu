@@ -16,8 +16,8 @@
 // When there are fewer tiles than SMs, 2 to 8 blocks of a cluster share a tile's k range and add their partial
 // tiles over distributed shared memory, in rank order (no atomics, no workspace: the same bits every time).
 //
-// With at most 64 rows (serving) the product is bound by reading w.  Up to 4 rows it is done by plain loads and float
-// FMAs (k_gemv), above that by k_gemm with the roles exchanged: w's rows fill the 128-row side of the tile and the few
+// With at most 64 rows (serving) the product is bound by reading w.  One or two rows (up to four where the sums are short)
+// are done by plain loads and float FMAs (k_gemv), more by k_gemm with the roles exchanged: w's rows fill the 128-row side of the tile and the few
 // rows of x its narrow side.
 //
 // TMA needs 16-byte aligned rows.  Operands without them are copied once into rows of a multiple of 8 elements
@@ -430,13 +430,50 @@ __device__ __forceinline__ void store_one(const GemmParams& p, int64_t r, int64_
     static_cast<T*>(p.y)[r * p.ldy + c] = from_f<T>(v);
 }
 
+// N consecutive rows of column c (the exchanged roles), each lane of a warp a column: the steps one after the other over
+// all rows, so that each is a short loop
+template <typename T, int N>
+__device__ __forceinline__ void store_column(const GemmParams& p, int64_t r, int64_t c, float (&v)[N]) {
+  const int n = (int)min((int64_t)N, p.n - r);  // p.n: rows of x
+  if (p.bias) {
+    const float b = to_f<T>(static_cast<const T*>(p.bias)[c]);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += b;
+  }
+  if (p.z) {
+    T* z = static_cast<T*>(p.z) + r * p.ldz + c;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < n) z[i * p.ldz] = from_f<T>(v[i]);
+  }
+  act_values(v, p.act);
+  if (p.residual) {
+    const T* q = static_cast<const T*>(p.residual) + r * p.ldr + c;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < n) v[i] += to_f<T>(q[i * p.ldr]);
+  }
+  if (p.out_f32) {
+    float* y = static_cast<float*>(p.y) + r * p.ldy + c;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < n) y[i * p.ldy] = v[i];
+  } else {
+    T* y = static_cast<T*>(p.y) + r * p.ldy + c;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < n) y[i * p.ldy] = from_f<T>(v[i]);
+  }
+}
 // four consecutive columns of row r; c is a multiple of 4
 template <typename T>
 __device__ __forceinline__ void store_four(const GemmParams& p, int64_t r, int64_t c, float (&v)[4]) {
   if (c + 4 > p.n || !p.vec_y || (p.z && !p.vec_z) || (p.residual && !p.vec_r)) {
-#pragma unroll
+#pragma unroll 1
     for (int j = 0; j < 4; ++j)
-      if (c + j < p.n) store_one<T>(p, r, c + j, v[j] + (p.bias ? to_f<T>(static_cast<const T*>(p.bias)[c + j]) : 0.f));
+      if (c + j < p.n)
+        store_one<T>(p, r, c + j, (j < 2 ? (j ? v[1] : v[0]) : (j == 2 ? v[2] : v[3])) +
+                                      (p.bias ? to_f<T>(static_cast<const T*>(p.bias)[c + j]) : 0.f));
     return;
   }
   if (p.bias) {
@@ -676,12 +713,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
           if (c0 >= p.n || r0 >= p.m) continue;  // nothing of this slice exists (uniform over the warp)
           float v[32];
           tmem_load32(src + c, v);
-          if (o < p.m) {
-            const float bv = bias ? to_f<T>(bias[o]) : 0.f;
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (c0 + i < p.n) store_one<T>(p, c0 + i, o, v[i] + bv);
-          }
+          if (o < p.m) store_column<T, 32>(p, c0, o, v);
         }
       } else {
         for (int c = half * 64; c < BN; c += 128) {
@@ -789,7 +821,6 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
       int tm, tn;
       tile_at(p, first, tm, tn);
       const int rows = BM / job.splits, row0 = rank * rows;
-      const T* bias = static_cast<const T*>(p.bias);
       constexpr int QUADS = BN / 4;
       for (int i = threadIdx.x; i < rows * QUADS; i += GEMM_THREADS) {
         // consecutive threads along the output's contiguous axis
@@ -811,9 +842,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
             v[3] += q[k].w;
           }
         if (p.swap) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (n + j < p.n) store_one<T>(p, n + j, m, v[j] + (bias ? to_f<T>(bias[m]) : 0.f));
+          store_column<T, 4>(p, n, m, v);
         } else {
           store_four<T>(p, m, n, v);
         }
@@ -1235,8 +1264,11 @@ void launch_gemv(const T* x, int64_t ldx, const T* w, int64_t ldw, int64_t rows,
 
 constexpr int64_t GEMV_ROWS = 4, NARROW_ROWS = 64;
 
-// w's layout: k-major rows for k_gemv
-bool use_gemv(int64_t rows, const Operand& w) { return rows <= GEMV_ROWS && !w.mn; }
+// k_gemv needs k-major rows of w (and of x).  Three and four rows go there when the sums are short or when k_gemm would have to
+// copy w first (4 rows: 4096 x 4096 12.7 us against k_gemm's 12.0, 400 x 20000 9.1 against 9.4).
+bool use_gemv(int64_t rows, const Operand& x, const Operand& w) {
+  return !w.mn && !x.mn && (rows <= 2 || (rows <= GEMV_ROWS && (w.depth <= 1024 || !w.tma_ok())));
+}
 
 // A matrix given by both strides: k-major when its second axis is contiguous, else its first must be.
 bool operand_of(const void* p, int64_t rows, int64_t depth, int64_t rs, int64_t cs, Operand* o) {
@@ -1292,7 +1324,7 @@ int fv_linear_workspace(int64_t rows, int64_t inner, int64_t outer, const void* 
   FV_REQUIRE(operand_of(x, rows, inner, x_rs, x_cs, &ox) && operand_of(w, outer, inner, w_rs, w_cs, &ow), FV_ERR_INVALID,
              "fv_linear: one axis of x and of the weight must be contiguous");
   *bytes = 0;
-  if (rows == 0 || (use_gemv(rows, ow) && !ox.mn)) return FV_OK;
+  if (rows == 0 || use_gemv(rows, ox, ow)) return FV_OK;
   if (!ox.tma_ok()) *bytes += packed_bytes(ox);
   if (!ow.tma_ok()) *bytes += packed_bytes(ow);
   return FV_OK;
@@ -1332,7 +1364,7 @@ int fv_linear(int device, void* stream, const void* x, int64_t x_rs, int64_t x_c
   p.vec_y = vec_ok(y, outer, ys, 16);
   p.vec_z = z && vec_ok(z, outer, 2, 16);
   p.vec_r = residual && vec_ok(residual, residual_stride, 2, 16);
-  if (use_gemv(rows, ow) && !ox.mn) {
+  if (use_gemv(rows, ox, ow)) {
     // Eight lanes to a column when that fills the GPU, else a warp; two columns to a group when there are enough of them.
     // 16-byte loads where the rows of w allow them.
     const int64_t ldw = outer > 1 ? ow.ld : 0;

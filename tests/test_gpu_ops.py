@@ -436,7 +436,7 @@ def product_slack(a, b, depth):
 
 
 @pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
-@pytest.mark.parametrize("rows,inner,outer", [(1, 400, 1000), (1, 7, 3), (2, 64, 130), (3, 4097, 65), (4, 5000, 257), (4, 9000, 40), (1, 400, 20000), (5, 64, 128),
+@pytest.mark.parametrize("rows,inner,outer", [(1, 400, 1000), (1, 7, 3), (2, 64, 130), (3, 4097, 65), (4, 5000, 257), (4, 9000, 40), (3, 2048, 1000), (4, 4096, 512), (4, 1032, 90), (1, 400, 20000), (5, 64, 128),
                                               (5, 1, 1), (17, 130, 300), (33, 501, 127), (64, 400, 4000), (64, 2048, 264), (65, 64, 64), (127, 65, 129),
                                               (128, 128, 256), (129, 1000, 257), (300, 63, 1003), (777, 501, 1003), (1000, 2048, 512), (2500, 136, 1600)])
 def test_linear(built_lib, rows, inner, outer, dtype):
