@@ -723,7 +723,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
           // result's (a float result fills the whole row: the residual is staged again for the second half).
           uint8_t* mine = stage + lane * 128;
           auto word = [&](int k) { return reinterpret_cast<uint4*>(mine + ((k ^ (lane & 7)) << 4)); };
-#pragma unroll
+#pragma unroll 1  // half the code: the instruction cache is short of it
           for (int h = 0; h < 2; ++h) {
             const int64_t ch = c0 + 32 * h;
             if (ch >= p.n) break;
@@ -742,7 +742,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
               }
             }
             float v[32];
-            if (bias) bias_slice[lane] = bias_reg[c >= 128 ? 2 + h : h];
+            if (bias) bias_slice[lane] = c >= 128 ? (h ? bias_reg[3] : bias_reg[2]) : (h ? bias_reg[1] : bias_reg[0]);
             tmem_load32(src + c + 32 * h, v);
             if (bias) {
               __syncwarp();
