@@ -205,8 +205,6 @@ __device__ __forceinline__ void column_sums(const float* __restrict__ part, int6
   }
 }
 
-// Bytes that divide an address and a stride: which vector width a row-major array admits.
-inline unsigned common_alignment(uintptr_t a) { return a == 0 ? 4096u : (unsigned)(a & (~a + 1)); }
 inline bool vec_ok(const void* p, int64_t stride_elems, size_t elem, unsigned bytes) {
   return (uintptr_t)p % bytes == 0 && ((uint64_t)stride_elems * elem) % bytes == 0;
 }
