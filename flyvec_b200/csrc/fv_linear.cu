@@ -24,7 +24,7 @@
 // (k_pack) in the caller's workspace; everything else is read where it lies.
 //
 // What bounds it: large products the tensor cores under the power limit (8192 x 8192 x 2048, bf16: 178 us, 1.55 PFLOP/s,
-// cuBLAS 177 us); with pre-activation, gelu and residual the epilogue (232 us: eight warps take 17 us a tile where the products
+// cuBLAS 177 us); with pre-activation, gelu and residual the epilogue (235 us: eight warps take 17 us a tile where the products
 // take 13); small ones launch, set-up and drain (about 5 us) and 0.16 us per k-block, the rate at which one thread
 // issues loads.  256 x 256 pairs halve what a block reads of B: 0.36 instead of 0.42 us per k-block with all SMs at work.
 //
@@ -867,7 +867,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
 // ---- up to four rows --------------------------------------------------------------------------------
 // G lanes share C output columns: each reads VEC elements of the columns' weight rows at a time and multiplies them with the
 // rows of x, which lie in shared memory in their own type (a 16-byte read per row and VEC elements, no bank conflicts).  Bound
-// by reading w once: 20000 columns of 400, one row: 4.3 us; 4096 of 4096: 6.1 us (both out of L2).
+// by reading w once: 20000 columns of 400, one row: 4.4 us; 4096 of 4096: 6.1 us (both out of L2).
 constexpr int GEMV_THREADS = 256, GEMV_CHUNK = 4096;
 template <typename T, int VEC, int G, int MT, int C>
 __global__ void __launch_bounds__(GEMV_THREADS)
@@ -930,19 +930,21 @@ __global__ void __launch_bounds__(GEMV_THREADS)
 }
 
 // ---- copies, gradients' first step ------------------------------------------------------------------
-// src [rows][cols] with any row stride to dst with rows of `pitch` (a multiple of 8) elements; blockIdx.z chooses one of
-// two.
+// src [rows][cols] with any row stride to dst with rows of `pitch` (a multiple of 8) elements, for up to two operands.
 struct PackJob {
   struct {
     const uint16_t* src;
     uint16_t* dst;
     int64_t ld, rows, cols, pitch;
   } one[2];
+  int count;
+  int64_t rows, cols;  // the most of either
 };
-__global__ void __launch_bounds__(256) k_pack(const __grid_constant__ PackJob job) {
-  const auto& j = job.one[blockIdx.z];
+__device__ __forceinline__ void pack_rows(const PackJob& job, int which) {
+  const auto& j = job.one[which];
   const int64_t c0 = ((int64_t)blockIdx.x * 32 + (threadIdx.x & 31)) * 8;
   if (c0 >= j.cols) return;
+#pragma unroll 2
   for (int64_t r = (int64_t)blockIdx.y * 8 + (threadIdx.x >> 5); r < j.rows; r += (int64_t)gridDim.y * 8) {
     uint16_t v[8];
 #pragma unroll
@@ -951,15 +953,22 @@ __global__ void __launch_bounds__(256) k_pack(const __grid_constant__ PackJob jo
         make_uint4(v[0] | (uint32_t)v[1] << 16, v[2] | (uint32_t)v[3] << 16, v[4] | (uint32_t)v[5] << 16, v[6] | (uint32_t)v[7] << 16);
   }
 }
+__global__ void __launch_bounds__(256) k_pack(const __grid_constant__ PackJob job) { pack_rows(job, blockIdx.z); }
 
-// dz = dy act'(z) (if dz) and the partial column sums part[blockIdx.y][outer]; a warp takes every eighth row of the
-// block's range, a lane VEC columns, ROWS rows in flight.
+// dz = dy act'(z) (if dz) and the column sums: partial ones to part[blockIdx.y][outer], or, when the blocks of one range of
+// columns form a cluster (few rows), the whole ones to db.  A warp takes every eighth row of the block's range, a lane VEC
+// columns, ROWS rows in flight.  Further planes of the grid copy operands, so that few rows need one launch for all of it.
 template <typename T, int VEC, int ACT>
 __global__ void __launch_bounds__(256)
     k_act_grad(const T* __restrict__ dy, int64_t ldg, const T* __restrict__ z, int64_t ldz, int64_t rows, int64_t outer,
-               T* __restrict__ dz, int64_t pitch, float* __restrict__ part) {
+               T* __restrict__ dz, int64_t pitch, float* __restrict__ part, T* __restrict__ db, const __grid_constant__ PackJob job) {
+  if (blockIdx.z) {
+    pack_rows(job, blockIdx.z - 1);
+    return;
+  }
   constexpr int ROWS = ACT == FV_ACT_NONE ? 4 : 2;  // with an activation four rows cost registers and 5 % of the time
   __shared__ float sum[8][32 * VEC];
+  __shared__ __align__(16) float total[32 * VEC];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t c = ((int64_t)blockIdx.x * 32 + lane) * VEC;
   const int64_t r0 = rows * blockIdx.y / gridDim.y, r1 = rows * (blockIdx.y + 1) / gridDim.y;
@@ -1007,19 +1016,52 @@ __global__ void __launch_bounds__(256)
     float v = 0.f;
 #pragma unroll
     for (int w = 0; w < 8; ++w) v += sum[w][i];
-    if (col < outer) part[(int64_t)blockIdx.y * outer + col] = v;
+    if (db)
+      total[i] = v;
+    else if (col < outer)
+      part[(int64_t)blockIdx.y * outer + col] = v;
   }
+  if (!db) return;
+  __syncwarp();
+  cluster_barrier();
+  if (blockIdx.y == 0 && threadIdx.x < 8 * VEC) {  // the cluster's blocks in their order
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    for (unsigned k = 0; k < gridDim.y; ++k) {
+      const float4 q = ld_cluster4(smem_u32(total + 4 * threadIdx.x), k);
+      v[0] += q.x;
+      v[1] += q.y;
+      v[2] += q.z;
+      v[3] += q.w;
+    }
+    const int64_t col = (int64_t)blockIdx.x * 32 * VEC + 4 * threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (col + i < outer) db[col + i] = from_f<T>(v[i]);
+  }
+  __syncwarp();
+  cluster_barrier();  // nobody leaves while its sums are read
 }
 template <typename T, int VEC>
-void launch_act_grad(cudaStream_t st, const T* dy, int64_t ldg, const T* z, int64_t ldz, int64_t rows, int64_t outer, int act, T* dz,
-                     int64_t pitch, float* part, int64_t chunks) {
-  const dim3 grid((unsigned)((outer + 32 * VEC - 1) / (32 * VEC)), (unsigned)chunks);
+cudaError_t launch_act_grad(cudaStream_t st, const T* dy, int64_t ldg, const T* z, int64_t ldz, int64_t rows, int64_t outer, int act, T* dz,
+                            int64_t pitch, float* part, T* db, int64_t chunks, const PackJob& job) {
+  const unsigned gx = (unsigned)((outer + 32 * VEC - 1) / (32 * VEC)), px = job.count ? (unsigned)((job.cols + 255) / 256) : 0u;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(std::max(gx, px), (unsigned)chunks, 1u + (unsigned)job.count);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = attr[0].val.clusterDim.z = 1;
+  attr[0].val.clusterDim.y = (unsigned)chunks;
+  cfg.attrs = attr;
+  cfg.numAttrs = db ? 1 : 0;
+  auto go = [&](auto kernel) { return cudaLaunchKernelEx(&cfg, kernel, dy, ldg, z, ldz, rows, outer, dz, pitch, part, db, job); };
   switch (act) {
-    case FV_ACT_RELU: k_act_grad<T, VEC, FV_ACT_RELU><<<grid, 256, 0, st>>>(dy, ldg, z, ldz, rows, outer, dz, pitch, part); break;
-    case FV_ACT_GELU: k_act_grad<T, VEC, FV_ACT_GELU><<<grid, 256, 0, st>>>(dy, ldg, z, ldz, rows, outer, dz, pitch, part); break;
-    case FV_ACT_GELU_TANH: k_act_grad<T, VEC, FV_ACT_GELU_TANH><<<grid, 256, 0, st>>>(dy, ldg, z, ldz, rows, outer, dz, pitch, part); break;
-    case FV_ACT_SILU: k_act_grad<T, VEC, FV_ACT_SILU><<<grid, 256, 0, st>>>(dy, ldg, z, ldz, rows, outer, dz, pitch, part); break;
-    default: k_act_grad<T, VEC, FV_ACT_NONE><<<grid, 256, 0, st>>>(dy, ldg, z, ldz, rows, outer, dz, pitch, part);
+    case FV_ACT_RELU: return go(k_act_grad<T, VEC, FV_ACT_RELU>);
+    case FV_ACT_GELU: return go(k_act_grad<T, VEC, FV_ACT_GELU>);
+    case FV_ACT_GELU_TANH: return go(k_act_grad<T, VEC, FV_ACT_GELU_TANH>);
+    case FV_ACT_SILU: return go(k_act_grad<T, VEC, FV_ACT_SILU>);
+    default: return go(k_act_grad<T, VEC, FV_ACT_NONE>);
   }
 }
 template <typename T>
@@ -1067,25 +1109,26 @@ struct Workspace {
   }
 };
 
-// Copies of those of two operands that TMA cannot read, in one launch.
-int pack_operands(Operand& a, Operand& b, Workspace& ws, cudaStream_t st) {
-  PackJob job{};
-  int count = 0;
-  int64_t most = 0, widest = 0;
+// Copies of those of two operands that TMA cannot read: the operands afterwards, and the job that fills them.
+int plan_pack(Operand& a, Operand& b, Workspace& ws, PackJob* job) {
+  *job = PackJob{};
   for (Operand* o : {&a, &b}) {
     if (o->tma_ok()) continue;
     const int64_t pitch = pad8(o->inner());
     uint16_t* dst = static_cast<uint16_t*>(ws.take((size_t)o->outer() * (size_t)pitch * 2));
-    job.one[count++] = {static_cast<const uint16_t*>(o->p), dst, o->ld, o->outer(), o->inner(), pitch};
-    most = std::max(most, o->outer());
-    widest = std::max(widest, o->inner());
+    job->one[job->count++] = {static_cast<const uint16_t*>(o->p), dst, o->ld, o->outer(), o->inner(), pitch};
+    job->rows = std::max(job->rows, o->outer());
+    job->cols = std::max(job->cols, o->inner());
     o->p = dst;
     o->ld = pitch;
   }
-  if (!count) return FV_OK;
-  FV_REQUIRE(ws.used <= ws.size, FV_ERR_INVALID, "workspace too small: %llu bytes needed so far, got %llu", (unsigned long long)ws.used,
-             (unsigned long long)ws.size);
-  k_pack<<<dim3((unsigned)((widest + 255) / 256), (unsigned)std::min<int64_t>((most + 7) / 8, 4096), (unsigned)count), 256, 0, st>>>(job);
+  FV_REQUIRE(!job->count || ws.used <= ws.size, FV_ERR_INVALID, "workspace too small: %llu bytes needed so far, got %llu",
+             (unsigned long long)ws.used, (unsigned long long)ws.size);
+  return FV_OK;
+}
+int pack_operands(const PackJob& job, cudaStream_t st) {
+  if (!job.count) return FV_OK;
+  k_pack<<<dim3((unsigned)((job.cols + 255) / 256), (unsigned)std::min<int64_t>((job.rows + 7) / 8, 4096), (unsigned)job.count), 256, 0, st>>>(job);
   FV_CUDA(cudaGetLastError());
   return FV_OK;
 }
@@ -1262,7 +1305,7 @@ void launch_gemv(const T* x, int64_t ldx, const T* w, int64_t ldw, int64_t rows,
   }
 }
 
-constexpr int64_t GEMV_ROWS = 4, NARROW_ROWS = 64;
+constexpr int64_t GEMV_ROWS = 4, NARROW_ROWS = 64, FEW_ROWS = 1024;
 
 // k_gemv needs k-major rows of w (and of x).  Three and four rows go there when the sums are short or when k_gemm would have to
 // copy w first (4 rows: 4096 x 4096 12.7 us against k_gemm's 12.0, 400 x 20000 9.1 against 9.4).
@@ -1385,7 +1428,9 @@ int fv_linear(int device, void* stream, const void* x, int64_t x_rs, int64_t x_c
     return FV_OK;
   }
   Workspace ws{static_cast<uint8_t*>(workspace), workspace_bytes};
-  if (int rc = pack_operands(ox, ow, ws, st)) return rc;
+  PackJob job;
+  if (int rc = plan_pack(ox, ow, ws, &job)) return rc;
+  if (int rc = pack_operands(job, st)) return rc;
   const bool narrow = rows <= NARROW_ROWS;  // w's rows on the wide side of the tiles
   p.swap = narrow;
   Product d = narrow ? Product{ow, ox, p} : Product{ox, ow, p};
@@ -1454,21 +1499,33 @@ int fv_linear_backward(int device, void* stream, const void* dy, int64_t dy_stri
     od = Operand{dz, rows, outer, pitch, false};
   }
   const bool vec = outer % 8 == 0 && vec_ok(dy, dy_stride, 2, 16) && (act == FV_ACT_NONE || vec_ok(z, z_stride, 2, 16));
-  const int64_t chunks = act_grad_chunks(rows, outer, vec ? 8 : 1, sms);
-  float* part = static_cast<float*>(ws.take((size_t)chunks * (size_t)outer * sizeof(float)));
+  // Few rows: one launch forms dz, its whole column sums (clusters of up to eight blocks) and the copies.  777 x 501 x 1003 18 us
+  // instead of 22 with three launches; 2000 rows of 256: 26 us instead of 18, too many rows for eight blocks.
+  const bool few = rows <= FEW_ROWS;
+  const int64_t chunks = few ? std::min<int64_t>(8, (rows + 63) / 64) : act_grad_chunks(rows, outer, vec ? 8 : 1, sms);
+  float* part = few ? nullptr : static_cast<float*>(ws.take((size_t)chunks * (size_t)outer * sizeof(float)));
+  PackJob job;
+  if (int rc = plan_pack(ox, ow, ws, &job)) return rc;
+  const bool together = few && job.rows <= FEW_ROWS;
   auto first = [&](auto tag) {
     using T = decltype(tag);
     const T *pg = static_cast<const T*>(dy), *pz = static_cast<const T*>(z);
-    if (vec)
-      launch_act_grad<T, 8>(st, pg, dy_stride, pz, z_stride, rows, outer, act, static_cast<T*>(dz), pitch, part, chunks);
-    else
-      launch_act_grad<T, 1>(st, pg, dy_stride, pz, z_stride, rows, outer, act, static_cast<T*>(dz), pitch, part, chunks);
-    k_col_sum<T><<<(unsigned)((outer + 31) / 32), 512, 0, st>>>(part, chunks, outer, static_cast<T*>(db));
+    T *pd = static_cast<T*>(dz), *sums = few ? static_cast<T*>(db) : nullptr;
+    const PackJob with = together ? job : PackJob{};
+    return vec ? launch_act_grad<T, 8>(st, pg, dy_stride, pz, z_stride, rows, outer, act, pd, pitch, part, sums, chunks, with)
+               : launch_act_grad<T, 1>(st, pg, dy_stride, pz, z_stride, rows, outer, act, pd, pitch, part, sums, chunks, with);
   };
-  if (dtype == FV_BF16) first(__nv_bfloat16{});
-  else first(__half{});
-  FV_CUDA(cudaGetLastError());
-  if (int rc = pack_operands(ox, ow, ws, st)) return rc;
+  FV_CUDA(dtype == FV_BF16 ? first(__nv_bfloat16{}) : first(__half{}));
+  if (!few) {
+    const unsigned grid = (unsigned)((outer + 31) / 32);
+    if (dtype == FV_BF16)
+      k_col_sum<__nv_bfloat16><<<grid, 512, 0, st>>>(part, chunks, outer, static_cast<__nv_bfloat16*>(db));
+    else
+      k_col_sum<__half><<<grid, 512, 0, st>>>(part, chunks, outer, static_cast<__half*>(db));
+    FV_CUDA(cudaGetLastError());
+  }
+  if (!together)
+    if (int rc = pack_operands(job, st)) return rc;
   GemmParams px{}, pw{};
   px.y = dx;
   pw.y = dw;
