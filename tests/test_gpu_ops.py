@@ -772,3 +772,59 @@ def test_word_log_probs_and_similar_words(built_lib, tmp_path):
     assert m.similar_words("nothere") == []
     with pytest.raises(ValueError):
         m.word_log_probs(idx, words[:3])
+
+
+def test_two_host_threads(built_lib):
+    """Calls from two threads at once, each on its own stream."""
+    import threading
+
+    problems = [head_problem(n=500, seed=s) for s in (1, 70)]
+    want = [head_forward(*p)[0] for p in problems]
+    torch.cuda.synchronize()
+    got, errors = [[], []], []
+
+    def work(k):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got[k].append(head_forward(*problems[k])[0])
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001  reported below
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for k in range(2):
+        for r in got[k]:
+            assert all(torch.equal(a, b) for a, b in zip(r, want[k]))
+
+
+def test_small_workspaces_are_refused(built_lib):
+    """A workspace that does not hold what the size function answers ends the call before anything is launched."""
+    import ctypes as C
+
+    lib, n = built_lib, C.c_size_t(0)
+    x, w = made((300, 63), "bfloat16", 1), made((40, 63), "bfloat16", 2)
+    y = torch.zeros(300, 40, device="cuda", dtype=torch.bfloat16)
+    ws = torch.empty(1 << 20, device="cuda", dtype=torch.uint8)
+    st = torch.cuda.current_stream().cuda_stream
+    assert lib.fv_linear_workspace(300, 63, 40, x.data_ptr(), 63, 1, w.data_ptr(), 63, 1, C.byref(n)) == 0 and n.value > 0
+    args = (0, st, x.data_ptr(), 63, 1, w.data_ptr(), 63, 1, 300, 63, 40, 1, None, 0, None, 0, y.data_ptr(), 1, None)
+    assert lib.fv_linear(*args, ws.data_ptr(), n.value - 256) == 1 and b"workspace" in lib.fv_last_error()
+    assert lib.fv_linear(*args, None, 0) == 1
+    assert (y == 0).all()
+    assert lib.fv_linear(*args, ws.data_ptr(), n.value) == 0 and torch.equal(y, ops.linear(x, w))
+    dx, dw, db = torch.empty_like(x), torch.empty_like(w), torch.empty(40, device="cuda", dtype=torch.bfloat16)
+    assert lib.fv_linear_backward_workspace(0, 300, 63, 40, y.data_ptr(), 40, x.data_ptr(), 63, 1, w.data_ptr(), 63, 1, 0, C.byref(n)) == 0
+    back = (0, st, y.data_ptr(), 40, x.data_ptr(), 63, 1, w.data_ptr(), 63, 1, 300, 63, 40, 1, None, 0, 0, dx.data_ptr(), dw.data_ptr(), db.data_ptr())
+    assert lib.fv_linear_backward(*back, ws.data_ptr(), n.value - 1) == 1 and b"workspace" in lib.fv_last_error()
+    assert lib.fv_linear_backward(*back, ws.data_ptr(), n.value) == 0
+    s = torch.zeros(300, device="cuda")
+    g = torch.ones(63, device="cuda", dtype=torch.bfloat16)
+    assert lib.fv_layer_norm_backward_workspace(0, 300, 63, 1, C.byref(n)) == 0
+    norm = (0, st, x.data_ptr(), 63, x.data_ptr(), 63, 300, 63, 1, s.data_ptr(), s.data_ptr(), g.data_ptr(), dx.data_ptr(), g.data_ptr(), g.data_ptr())
+    assert lib.fv_layer_norm_backward(*norm, ws.data_ptr(), n.value - 4) == 1 and b"workspace" in lib.fv_last_error()
