@@ -614,11 +614,13 @@ __global__ void __launch_bounds__(128)
   const RowScalars s = finish(p);
   if (lane == 0) write_row(out, row, p, s, xt, t, V, beta);
   if (top == 0) return;
+  // 16-bit elements differ in the leading bits of their keys alone
+  constexpr int DROP = sizeof(T) == 4 ? 0 : std::is_same<T, __half>::value ? 13 : 16;
   unsigned key[E];
 #pragma unroll
-  for (int e = 0; e < E; ++e) key[e] = lane + 32 * e < V ? key_of(x[e]) : 0u;
+  for (int e = 0; e < E; ++e) key[e] = lane + 32 * e < V ? key_of(x[e]) >> DROP : 0u;
   unsigned tau = 0;
-  for (int b = 31; b >= 0; --b) {
+  for (int b = 31 - DROP; b >= 0; --b) {
     const unsigned c = tau | 1u << b;
     unsigned n = 0;
 #pragma unroll
@@ -633,7 +635,7 @@ __global__ void __launch_bounds__(128)
   for (int e = 0; e < E; ++e) {
     const bool take = key[e] > tau;
     const unsigned v = __ballot_sync(FULL, take);
-    if (take) cand[n + __popc(v & below)] = cand_of(key[e], (unsigned)(lane + 32 * e));
+    if (take) cand[n + __popc(v & below)] = cand_of(key_of(x[e]), (unsigned)(lane + 32 * e));
     n += __popc(v);
   }
 #pragma unroll
@@ -641,7 +643,7 @@ __global__ void __launch_bounds__(128)
     const bool take = key[e] == tau;
     const unsigned v = __ballot_sync(FULL, take);
     const int slot = n + __popc(v & below);
-    if (take && slot < top) cand[slot] = cand_of(key[e], (unsigned)(lane + 32 * e));
+    if (take && slot < top) cand[slot] = cand_of(key_of(x[e]), (unsigned)(lane + 32 * e));
     n += __popc(v);
   }
   __syncwarp();
