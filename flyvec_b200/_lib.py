@@ -131,6 +131,7 @@ _PROTOTYPES = {
     "fv_token_log_probs": ([C.c_int, _P, _P, _I, _I, _I, C.c_int, _P, C.c_int, C.c_float, C.c_int, _P, _P, _P, _P, _P, _P], C.c_int),
     "fv_token_log_probs_backward": ([C.c_int, _P, _P, _P, _P, _I, _I, _I, C.c_int, _P, C.c_int, _P, _P, _P, C.c_float, _P], C.c_int),
     "fv_ops_status": ([C.c_int, C.POINTER(C.c_uint32)], C.c_int),
+    "fv_ops_wait_limit": ([_I], C.c_int),
     "fv_device_alloc": ([C.c_int, C.c_size_t, C.POINTER(_P)], C.c_int),
     "fv_device_free": ([C.c_int, _P], C.c_int),
     "fv_host_alloc_pinned": ([C.c_size_t, C.POINTER(_P)], C.c_int),

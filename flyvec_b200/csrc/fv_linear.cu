@@ -31,7 +31,7 @@
 // Roundings to 16 bits: the outputs, and dz before it enters the two products (as tensor-core operands have to be; db
 // is formed from the unrounded dz).
 //
-// Every wait is bounded: a wait that runs out raises a flag (fv_ops_status), the block drains what it has in
+// Every wait is bounded: a wait that runs out raises a flag (fv_ops_status), the block outlasts what it has in
 // flight, frees its TMEM and returns.
 #include <cuda.h>
 
@@ -146,20 +146,18 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-constexpr long long WAIT_CYCLES = 4000000000ll;  // about two seconds
-// Waits for the phase of the given parity; false when the limit ran out here or elsewhere in the block.
-__device__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* stop) {
-  if (mbar_try(bar, parity)) return true;
+// Waits for the phase of the given parity; false when the limit (0: no look at all) ran out here or elsewhere in the block.
+__device__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* stop, long long limit) {
+  if (limit > 0 && mbar_try(bar, parity)) return true;
   const long long t0 = clock64();
-  for (;;) {
+  while (limit > 0) {
     if (mbar_try(bar, parity)) return true;
     if (*stop) return false;
-    if (clock64() - t0 > WAIT_CYCLES) {
-      *stop = 1;
-      atomicOr(&g_status, 1u);
-      return false;
-    }
+    if (clock64() - t0 > limit) break;
   }
+  *stop = 1;
+  atomicOr(&g_status, 1u);
+  return false;
 }
 // One thread of a converged warp, in a form that the compiler knows to be one thread: the loads and products below
 // take their operands from uniform registers, and under a plain lane == 0 each would be wrapped in a loop over lanes
@@ -280,6 +278,7 @@ struct GemmJob {
   int tiles0, tiles;  // of the first product (the one with the longer sums), of both
   int splits;
   int spare;          // tiles of the second product that cost as much as one of the first
+  long long limit;    // cycles of a wait
 };
 // The k-th tile of place c of `places` (blocks, pairs or clusters); -1 after the last.  The first product's tiles go round
 // the places; those that get none in the last round take `spare` tiles of the second product meanwhile, whose other
@@ -572,7 +571,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
     // loads: one thread for A and one for B, because one alone issues a load every 0.09 us
     const bool is_a = warp == 0;
     if (elect_one()) {
-      int s = 0, phase = 0, issued = 0;
+      int s = 0, phase = 0;
       bool ok = true;
       for (int i = 0, t; ok && (t = tile_of(job, first, i, step)) >= 0; ++i) {
         int tm, tn;
@@ -582,7 +581,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
         const bool mn = is_a ? p.a_mn : p.b_mn;
         const int kb1 = last_k(p), row = is_a ? (PAIR ? tm * 2 + side : tm) * BM : tn * BN + side * BROWS;
         for (int kb = first_k(p); kb < kb1; ++kb) {
-          if (!(ok = mbar_wait(empty(s), phase ^ 1, stop))) break;
+          if (!(ok = mbar_wait(empty(s), phase ^ 1, stop, job.limit))) break;
           const uint32_t to = ring + s * STAGE + (is_a ? 0 : A_BYTES);
           const uint32_t bar = PAIR ? cluster_addr(full(s), 0) : full(s);  // a pair's loads report to its first block
           if (is_a && side == 0) mbar_expect(full(s), PAIR ? 2 * STAGE : STAGE);
@@ -592,23 +591,13 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
           } else {
             tma_load<PAIR>(to, map, kb * BK, row, bar);
           }
-          ++issued;
           if (++s == STAGES) {
             s = 0;
             phase ^= 1;
           }
         }
       }
-      if (!ok && side == 0 && is_a) {  // the copies in flight must land before the block (the pair: both meet below) ends
-        volatile int never = 0;
-        for (int k = 0; k < STAGES && k < issued; ++k) {
-          if (--s < 0) {
-            s = STAGES - 1;
-            phase ^= 1;
-          }
-          if (!mbar_wait(full(s), phase, &never)) break;
-        }
-      }
+      if (!ok) outlast_copies();  // of a stage that only one of the two threads has started no phase ends
     }
   } else if (warp == 1) {
     if (side == 0 && elect_one()) {  // products
@@ -621,10 +610,10 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
         const uint32_t a_lead = p.a_mn ? 8192 : 16, b_lead = p.b_mn ? 8192 : 16;
         const uint32_t idesc = p.idesc;
         const int kb0 = first_k(p), kb1 = last_k(p);
-        if (!(ok = mbar_wait(acc_empty(acc), acc_phase ^ 1, stop))) break;
+        if (!(ok = mbar_wait(acc_empty(acc), acc_phase ^ 1, stop, job.limit))) break;
         tc_fence_after();
         for (int kb = kb0; kb < kb1; ++kb) {
-          if (!(ok = mbar_wait(full(s), phase, stop))) break;
+          if (!(ok = mbar_wait(full(s), phase, stop, job.limit))) break;
           tc_fence_after();
           const uint32_t a = ring + s * STAGE, b = a + A_BYTES;
 #pragma unroll
@@ -647,7 +636,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
       if (!ok) {  // products in flight must end before TMEM is freed
         volatile int never = 0;
         mma_commit<PAIR>(drained);
-        mbar_wait(drained, 0, &never);
+        mbar_wait(drained, 0, &never, WAIT_LIMIT);
       }
     }
   } else {
@@ -692,7 +681,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
       for (int j = 0; j < 4; ++j) bias_reg[j] = bias_next[j];
       fetch_ahead(t_next, false);
       bool ahead = false;  // the next tile's first residual slice is on its way
-      if (!mbar_wait(acc_full(acc), acc_phase, stop)) break;
+      if (!__all_sync(FULL, mbar_wait(acc_full(acc), acc_phase, stop, job.limit))) break;  // the warp stays together
       tc_fence_after();
       const uint32_t src = tmem + acc * BN + ((uint32_t)(quarter * 32) << 16);
       if (!PAIR && job.splits > 1) {  // to shared memory (the ring is free: every load was consumed before acc_full)
@@ -1255,6 +1244,7 @@ int gemm(Product* d, int count, int dtype, const Shape& s, int sms, cudaStream_t
   GemmMaps maps{};
   GemmJob job{};
   job.splits = s.splits;
+  job.limit = wait_limit();
   const int rows = s.pair ? 2 * BM : BM;
   int64_t tiles = 0;
   for (int i = 0; i < count; ++i) {
@@ -1357,6 +1347,12 @@ int fv_ops_status(int device, uint32_t* word) {
   uint32_t more = 0;
   FV_CUDA(norm_status(&more));
   *word |= more;
+  return FV_OK;
+}
+
+int fv_ops_wait_limit(int64_t cycles) {
+  FV_REQUIRE(cycles >= -1, FV_ERR_INVALID, "fv_ops_wait_limit: %lld cycles", (long long)cycles);
+  wait_limit(cycles);
   return FV_OK;
 }
 

@@ -24,6 +24,7 @@
 // 16384 x 4096: forward bf16 56 us (4.8 TB/s), float 90 us (5.9 TB/s); backward bf16 82 us (4.9 TB/s), float 132 us (6.1 TB/s).  float
 // is bound by memory; bf16 has twice the elements to a byte and is bound by the issue of their conversions and sums.
 #include <algorithm>
+#include <atomic>
 
 #include "fv_ops.h"
 
@@ -38,6 +39,12 @@ int sm_count(int device) {
     cached[device] = n;
   }
   return cached[device];
+}
+
+long long wait_limit(long long set) {
+  static std::atomic<long long> limit{WAIT_LIMIT};
+  if (set >= -1) limit.store(set == -1 ? WAIT_LIMIT : set, std::memory_order_relaxed);
+  return limit.load(std::memory_order_relaxed);
 }
 
 namespace {
@@ -144,10 +151,12 @@ __device__ __forceinline__ uint32_t ring_bytes(const void* row, int bytes) {
 __device__ __forceinline__ void ring_expect(uint64_t* bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(shared_addr(bar)), "r"(bytes) : "memory");
 }
-// Bounded wait for a stage; false when the copies did not arrive (about two seconds).
-__device__ __forceinline__ bool ring_wait(uint64_t* bar, int parity) {
+// Bounded wait for a stage; false when the copies did not arrive within `limit` cycles (0: gives up without a look).  A
+// thread whose wait ran out goes on without waiting or copying, so that all threads of its group keep meeting at the same
+// barriers, and outlasts the copies in flight before it ends; the results are invalid.
+__device__ __forceinline__ bool ring_wait(uint64_t* bar, int parity, long long limit) {
   long long t0 = 0;
-  for (;;) {
+  while (limit > 0) {
     uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
@@ -159,11 +168,10 @@ __device__ __forceinline__ bool ring_wait(uint64_t* bar, int parity) {
     if (ok) return true;
     const long long now = clock64();
     if (t0 == 0) t0 = now;
-    if (now - t0 > 4000000000ll) {
-      atomicOr(&g_norm_status, 1u);
-      return false;
-    }
+    if (now - t0 > limit) break;
   }
+  atomicOr(&g_norm_status, 1u);
+  return false;
 }
 // A group's place: its threads, its first row and the distance to its next.
 template <bool BLOCK>
@@ -236,15 +244,16 @@ __device__ __forceinline__ void word_pairs(const Columns<VEC, NV>& c, int j, con
 template <typename T, int NV, bool BLOCK, bool EDGE>
 __global__ void __launch_bounds__(BLOCK ? NORM_MAX_THREADS : 32 * NORM_WARPS)
     k_norm(const T* __restrict__ x, int64_t xs, int64_t rows, int D, const T* __restrict__ w, const T* __restrict__ b, float eps,
-           void* __restrict__ y, int ydt, float* __restrict__ mean_out, float* __restrict__ rstd_out, int stages, int pitch) {
+           void* __restrict__ y, int ydt, float* __restrict__ mean_out, float* __restrict__ rstd_out, int stages, int pitch, long long limit) {
   constexpr int VEC = 16 / (int)sizeof(T);
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ __align__(16) float red[2][16][2];
   const Group<BLOCK> g;
   const Ring ring = make_ring<BLOCK>(smem, stages, pitch, 1, g.t);
   const int bytes = D * (int)sizeof(T);
+  bool late = false;
   auto fetch = [&](int64_t r, int s) {
-    if (r < rows) {
+    if (r < rows && !late) {
       const T* row = x + r * xs;
       ring_expect(ring.bars + s, ring_bytes(row, bytes));
       ring_copy(ring.base + (size_t)s * pitch, row, bytes, ring.bars + s);
@@ -269,7 +278,7 @@ __global__ void __launch_bounds__(BLOCK ? NORM_MAX_THREADS : 32 * NORM_WARPS)
   const int pivot_at = EDGE ? (wide ? VEC : off) : 0;
   int s = 0, parity = 0;
   for (int64_t r = g.first; r < rows; r += g.step, out += hop) {
-    if (!ring_wait(ring.bars + s, parity)) break;
+    late = late || !ring_wait(ring.bars + s, parity, limit);
     const T* stage = reinterpret_cast<const T*>(ring.base + (size_t)s * pitch);
     float pivot;
     if (wide) {
@@ -338,6 +347,7 @@ __global__ void __launch_bounds__(BLOCK ? NORM_MAX_THREADS : 32 * NORM_WARPS)
       parity ^= 1;
     }
   }
+  if (late) outlast_copies();
 }
 
 // Rows too long for registers: three passes, the second and third out of L2.
@@ -378,7 +388,7 @@ template <typename T, int NV, bool BLOCK, bool EDGE>
 __global__ void __launch_bounds__(BLOCK ? NORM_MAX_THREADS : 32 * NORM_WARPS)
     k_norm_grad(const T* __restrict__ dy, int64_t gs, const T* __restrict__ x, int64_t xs, int64_t rows, int D,
                 const float* __restrict__ mean, const float* __restrict__ rstd, const T* __restrict__ w, T* __restrict__ dx,
-                float* __restrict__ part, int stages, int pitch) {
+                float* __restrict__ part, int stages, int pitch, long long limit) {
   constexpr int VEC = 16 / (int)sizeof(T);
   constexpr bool KEEP = sizeof(T) == 2 && NV <= 2;
   extern __shared__ __align__(128) unsigned char smem[];
@@ -386,8 +396,9 @@ __global__ void __launch_bounds__(BLOCK ? NORM_MAX_THREADS : 32 * NORM_WARPS)
   const Group<BLOCK> g;
   const Ring ring = make_ring<BLOCK>(smem, stages, pitch, 2, g.t);
   const int bytes = D * (int)sizeof(T);
+  bool late = false;
   auto fetch = [&](int64_t r, int s) {
-    if (r < rows) {
+    if (r < rows && !late) {
       const T *xr = x + r * xs, *gr = dy + r * gs;
       unsigned char* to = ring.base + (size_t)s * 2 * pitch;
       ring_expect(ring.bars + s, ring_bytes(xr, bytes) + ring_bytes(gr, bytes));
@@ -423,7 +434,7 @@ __global__ void __launch_bounds__(BLOCK ? NORM_MAX_THREADS : 32 * NORM_WARPS)
       next_mu = mean[r + g.step];
       next_rs = rstd[r + g.step];
     }
-    if (!ring_wait(ring.bars + s, parity)) break;
+    late = late || !ring_wait(ring.bars + s, parity, limit);
     const T* sx = reinterpret_cast<const T*>(ring.base + (size_t)s * 2 * pitch);
     const T* sg = reinterpret_cast<const T*>(ring.base + (size_t)s * 2 * pitch + pitch);
     // h and dy of word j, 0 outside the row
@@ -490,6 +501,7 @@ __global__ void __launch_bounds__(BLOCK ? NORM_MAX_THREADS : 32 * NORM_WARPS)
       parity ^= 1;
     }
   }
+  if (late) outlast_copies();
   if (!part) return;
   float* out = part + (int64_t)blockIdx.x * 2 * D;
   if (BLOCK) {
@@ -638,7 +650,7 @@ cudaError_t launch_norm(const NormPlan& p, cudaStream_t st, const T* x, int64_t 
   const auto kernel = k_norm<T, NV, BLOCK, EDGE>;
   static size_t given[64] = {0};
   if (cudaError_t e = allow_smem((const void*)kernel, given, p.smem)) return e;
-  kernel<<<(unsigned)p.grid, p.threads, p.smem, st>>>(x, xs, rows, D, w, b, eps, y, ydt, mean, rstd, p.stages, p.pitch);
+  kernel<<<(unsigned)p.grid, p.threads, p.smem, st>>>(x, xs, rows, D, w, b, eps, y, ydt, mean, rstd, p.stages, p.pitch, wait_limit());
   return cudaGetLastError();
 }
 template <typename T, int NV, bool BLOCK, bool EDGE>
@@ -647,7 +659,7 @@ cudaError_t launch_norm_grad(const NormPlan& p, cudaStream_t st, const T* dy, in
   const auto kernel = k_norm_grad<T, NV, BLOCK, EDGE>;
   static size_t given[64] = {0};
   if (cudaError_t e = allow_smem((const void*)kernel, given, p.smem)) return e;
-  kernel<<<(unsigned)p.grid, p.threads, p.smem, st>>>(dy, gs, x, xs, rows, D, mean, rstd, w, dx, part, p.stages, p.pitch);
+  kernel<<<(unsigned)p.grid, p.threads, p.smem, st>>>(dy, gs, x, xs, rows, D, mean, rstd, w, dx, part, p.stages, p.pitch, wait_limit());
   return cudaGetLastError();
 }
 

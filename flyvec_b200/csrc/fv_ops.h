@@ -97,6 +97,12 @@ __device__ __forceinline__ float min_nan(float a, float b) {
   asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
   return y;
 }
+// After a wait that ran out: the asynchronous copies in flight must land before the block's shared memory goes to another.
+// They depend on nothing but memory, which this (some 50 ms) outlasts by far.
+__device__ __forceinline__ void outlast_copies() {
+  const long long t0 = clock64();
+  while (clock64() - t0 < 100000000ll) __nanosleep(10000);
+}
 // two float operations at a time
 __device__ __forceinline__ unsigned long long pack2(float2 v) { return *reinterpret_cast<unsigned long long*>(&v); }
 __device__ __forceinline__ float2 unpack2(unsigned long long v) { return *reinterpret_cast<float2*>(&v); }
@@ -243,6 +249,11 @@ inline cudaError_t allow_smem(const void* kernel, size_t (&done)[64], size_t byt
   if (e == cudaSuccess && device < 64) done[device] = bytes;
   return e;
 }
+
+// Cycles after which a bounded wait inside a kernel gives up, about two seconds; wait_limit answers what the next launches get
+// (and sets it first: -1 the default, 0 waits that give up at once).
+constexpr long long WAIT_LIMIT = 4000000000ll;
+long long wait_limit(long long set = -2);
 
 int sm_count(int device);  // cached per device; 0 after an error
 cudaError_t norm_status(uint32_t* word);  // reads and clears the error bits of fv_norm.cu's kernels
