@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 // the public header: in include/ of the source tree, beside this file in an installed package
 #if __has_include("../../include/flyvec_b200.h")
 #include "../../include/flyvec_b200.h"
@@ -31,6 +33,20 @@ struct DeviceGuard {
     if (prev >= 0) cudaSetDevice(prev);
   }
 };
+
+// Lets a kernel have `bytes` of dynamic shared memory on the current device.  The attribute replaces the limit, it does not
+// raise it: what is asked for is always `most`, the largest size the kernel is ever launched with, so that threads which
+// get here at the same time with different sizes set the same value twice.  `done` is the kernel's own record per device.
+inline cudaError_t allow_smem(const void* kernel, std::atomic<bool> (&done)[64], size_t bytes, size_t most) {
+  if (bytes <= (48u << 10)) return cudaSuccess;
+  if (bytes > most) return cudaErrorInvalidValue;
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess || (device < 64 && done[device].load(std::memory_order_acquire))) return e;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+  if (e == cudaSuccess && device < 64) done[device].store(true, std::memory_order_release);
+  return e;
+}
 
 }  // namespace fv
 

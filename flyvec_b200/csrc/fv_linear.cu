@@ -1216,8 +1216,8 @@ Shape choose_shape(const Size* sizes, int count, int sms, bool narrow, double* t
 
 template <typename T, int BN, bool PAIR>
 int launch_gemm(const GemmMaps& maps, const GemmJob& job, unsigned grid, int splits, cudaStream_t st) {
-  static size_t given[64] = {0};
-  FV_CUDA(allow_smem((const void*)k_gemm<T, BN, PAIR>, given, GEMM_SMEM));
+  static std::atomic<bool> given[64];
+  FV_CUDA(fv::allow_smem((const void*)k_gemm<T, BN, PAIR>, given, GEMM_SMEM, GEMM_SMEM));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(GEMM_THREADS);

@@ -51,6 +51,7 @@ namespace {
 
 constexpr int NORM_WARPS = 4;         // rows a block of the one-warp-per-row form holds
 constexpr int NORM_MAX_THREADS = 512; // of the one-block-per-row form
+constexpr size_t NORM_SMEM = 208 << 10; // what the blocks of an SM share for their rings
 
 // Sum over the group that owns a row: a warp, or a block through `red` ([2][16][2], the two halves used in turn, so
 // that one barrier per sum is enough).
@@ -631,8 +632,8 @@ NormPlan plan_norm(int64_t rows, int64_t D, int dtype, bool grad, bool edge, int
     per_sm = std::max(1, std::min(16, (!grad ? 1024 : dtype == FV_F32 ? 768 : 512) / p.threads));
   }
   const int64_t fixed = (int64_t)groups * RING_MOST * 8, stage = (int64_t)groups * arrays * p.pitch;
-  while (per_sm > 1 && (208 << 10) / per_sm < fixed + 2 * stage) --per_sm;
-  p.stages = (int)std::max<int64_t>(2, std::min<int64_t>(RING_MOST, ((208 << 10) / per_sm - fixed) / stage));
+  while (per_sm > 1 && (int64_t)NORM_SMEM / per_sm < fixed + 2 * stage) --per_sm;
+  p.stages = (int)std::max<int64_t>(2, std::min<int64_t>(RING_MOST, ((int64_t)NORM_SMEM / per_sm - fixed) / stage));
   const int64_t all = (rows + groups - 1) / groups;
   p.grid = std::min<int64_t>(all, (int64_t)sms * per_sm);
   // a block's partial sums cost as much as a row or two: four rows to a block at least
@@ -648,8 +649,8 @@ template <typename T, int NV, bool BLOCK, bool EDGE>
 cudaError_t launch_norm(const NormPlan& p, cudaStream_t st, const T* x, int64_t xs, int64_t rows, int D, const T* w, const T* b, float eps,
                         void* y, int ydt, float* mean, float* rstd) {
   const auto kernel = k_norm<T, NV, BLOCK, EDGE>;
-  static size_t given[64] = {0};
-  if (cudaError_t e = allow_smem((const void*)kernel, given, p.smem)) return e;
+  static std::atomic<bool> given[64];
+  if (cudaError_t e = fv::allow_smem((const void*)kernel, given, p.smem, NORM_SMEM)) return e;
   kernel<<<(unsigned)p.grid, p.threads, p.smem, st>>>(x, xs, rows, D, w, b, eps, y, ydt, mean, rstd, p.stages, p.pitch, wait_limit());
   return cudaGetLastError();
 }
@@ -657,8 +658,8 @@ template <typename T, int NV, bool BLOCK, bool EDGE>
 cudaError_t launch_norm_grad(const NormPlan& p, cudaStream_t st, const T* dy, int64_t gs, const T* x, int64_t xs, int64_t rows, int D,
                              const float* mean, const float* rstd, const T* w, T* dx, float* part) {
   const auto kernel = k_norm_grad<T, NV, BLOCK, EDGE>;
-  static size_t given[64] = {0};
-  if (cudaError_t e = allow_smem((const void*)kernel, given, p.smem)) return e;
+  static std::atomic<bool> given[64];
+  if (cudaError_t e = fv::allow_smem((const void*)kernel, given, p.smem, NORM_SMEM)) return e;
   kernel<<<(unsigned)p.grid, p.threads, p.smem, st>>>(dy, gs, x, xs, rows, D, mean, rstd, w, dx, part, p.stages, p.pitch, wait_limit());
   return cudaGetLastError();
 }

@@ -238,18 +238,6 @@ struct OnDevice {
   OnDevice& operator=(const OnDevice&) = delete;
 };
 
-// Lets a kernel have `bytes` of dynamic shared memory on the current device; `done` is the kernel's own record of what it was
-// given per device (a race between threads repeats a call that does no harm).
-inline cudaError_t allow_smem(const void* kernel, size_t (&done)[64], size_t bytes) {
-  if (bytes <= (48u << 10)) return cudaSuccess;
-  int device = 0;
-  cudaError_t e = cudaGetDevice(&device);
-  if (e != cudaSuccess || (device < 64 && done[device] >= bytes)) return e;
-  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-  if (e == cudaSuccess && device < 64) done[device] = bytes;
-  return e;
-}
-
 // Cycles after which a bounded wait inside a kernel gives up, about two seconds; wait_limit answers what the next launches get
 // (and sets it first: -1 the default, 0 waits that give up at once).
 constexpr long long WAIT_LIMIT = 4000000000ll;

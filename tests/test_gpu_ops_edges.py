@@ -1,5 +1,9 @@
 """The dense operators at their edges: waits that run out, errors and what follows them, threads, streams, far offsets, every
 kernel form of the matrix product.  Helpers and the way tolerances are derived are those of test_gpu_ops."""
+import subprocess
+import sys
+from pathlib import Path
+
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -51,3 +55,44 @@ def test_waits_that_run_out(built_lib, make, sizes):
     got = call()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     assert ops.device_status() == 0
+
+
+FIRST_MEETING = """
+import threading
+import numpy as np
+from flyvec_b200 import ops
+from flyvec_b200.engine import DeviceArray
+
+# two widths that one layer-norm kernel takes with different amounts of shared memory, both beyond 48 KB
+for dtype, widths in (("bfloat16", (16384, 9000)), ("float16", (16384, 9000)), ("float32", (16384, 9000)), ("bfloat16", (16373, 9001)),
+                      ("float16", (16373, 9001)), ("float32", (16381, 9001)), ("float32", (8192, 6000)), ("float32", (8191, 6001))):
+    rng = np.random.default_rng(1)
+    x = [DeviceArray.from_numpy(rng.standard_normal((4, n)), dtype) for n in widths]
+    w = [DeviceArray.from_numpy(np.ones(n), dtype) for n in widths]
+    m = DeviceArray.from_numpy(np.zeros(4, np.float32)), DeviceArray.from_numpy(np.ones(4, np.float32))
+    gate, got, errors = threading.Barrier(2), {}, []
+
+    def both(k):
+        return [a.numpy() for a in (ops.layer_norm(x[k]), *ops.layer_norm_backward(x[k], x[k], *m, w[k]))]
+
+    def work(k):
+        gate.wait()
+        try:
+            got[k] = both(k)
+        except Exception as e:
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in (0, 1)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not errors, (dtype, widths, errors)
+    for k in (0, 1):
+        for a, b in zip(got[k], both(k)):
+            np.testing.assert_array_equal(a, b)
+assert ops.device_status() == 0
+"""
+
+
+def test_threads_that_meet_a_kernel_first_with_different_widths(built_lib):
+    done = subprocess.run([sys.executable, "-c", FIRST_MEETING], cwd=Path(__file__).resolve().parent.parent, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
