@@ -35,8 +35,11 @@ FV_HASH_EXACT = 8
 DTYPES = {"float32": 0, "bfloat16": 1, "float16": 2}
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 
+#: status of a wait inside a kernel that ran out
+FV_ERR_TIMEOUT = 6
+
 STATUS_NAMES = {1: "FV_ERR_INVALID", 2: "FV_ERR_CUDA", 3: "FV_ERR_COMM", 4: "FV_ERR_STATE", 5: "FV_ERR_DATA",
-                6: "FV_ERR_TIMEOUT"}
+                FV_ERR_TIMEOUT: "FV_ERR_TIMEOUT"}
 
 
 class FlyvecError(RuntimeError):

@@ -13,6 +13,7 @@ from typing import Dict, Optional, Union
 
 import numpy as np
 
+from ._lib import FV_ERR_TIMEOUT, FlyvecError
 from .engine import Hasher
 from .tokenizer import GensimTokenizer, VocabTokenizer
 
@@ -223,6 +224,9 @@ class FlyVec:
             scores = ops.linear(x, table, out_dtype="float32")  # K times the correlations
             r = ops.token_log_probs(scores, DeviceArray.from_numpy(words[a:a + chunk], device=self.device), beta=beta / K, top=top)
             parts.append([None if v is None else v.numpy() for v in r])
+        if ops.device_status(self.device):
+            self.__dict__.pop("_word_table", None)  # it may be what failed
+            raise FlyvecError(FV_ERR_TIMEOUT, "a bounded wait inside a kernel ran out: the scores are invalid")
         return ops.TokenLogProbs(*(None if v[0] is None else np.concatenate(v) for v in zip(*parts)))
 
     def similar_words(self, word: str, top: int = 10, beta: float = 20.0):

@@ -36,6 +36,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <mutex>
 
 #include "fv_ops.h"
 
@@ -1339,11 +1340,12 @@ int fv_ops_status(int device, uint32_t* word) {
   FV_REQUIRE(word, FV_ERR_INVALID, "fv_ops_status: NULL argument");
   OnDevice guard(device);
   FV_REQUIRE(guard.ok, FV_ERR_CUDA, "cannot select device %d", device);
-  FV_CUDA(cudaMemcpyFromSymbol(word, g_status, sizeof(uint32_t)));
-  if (*word) {
-    const uint32_t zero = 0;
-    FV_CUDA(cudaMemcpyToSymbol(g_status, &zero, sizeof(zero)));
-  }
+  static std::mutex one;
+  const std::lock_guard<std::mutex> lock(one);
+  FV_CUDA(cudaDeviceSynchronize());  // non-blocking streams too, which the copies below would not wait for
+  void* bits = nullptr;
+  FV_CUDA(cudaGetSymbolAddress(&bits, g_status));
+  FV_CUDA(take_status(static_cast<unsigned*>(bits), word));
   uint32_t more = 0;
   FV_CUDA(norm_status(&more));
   *word |= more;

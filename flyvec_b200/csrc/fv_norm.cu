@@ -702,11 +702,19 @@ bool norm_even(int64_t D, size_t es, std::initializer_list<std::pair<const void*
 }  // namespace fvo
 
 namespace fvo {
+__device__ unsigned g_taken;
+__global__ void k_take_status(unsigned* bits) { g_taken = atomicExch(bits, 0u); }
+cudaError_t take_status(unsigned* bits, uint32_t* word) {
+  cudaError_t e = cudaMemcpy(word, bits, sizeof(uint32_t), cudaMemcpyDeviceToHost);
+  if (e != cudaSuccess || !*word) return e;
+  k_take_status<<<1, 1>>>(bits);
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  return cudaMemcpyFromSymbol(word, g_taken, sizeof(uint32_t));
+}
 cudaError_t norm_status(uint32_t* word) {
-  cudaError_t e = cudaMemcpyFromSymbol(word, g_norm_status, sizeof(uint32_t));
-  const uint32_t zero = 0;
-  if (e == cudaSuccess && *word) e = cudaMemcpyToSymbol(g_norm_status, &zero, sizeof(zero));
-  return e;
+  void* bits = nullptr;
+  const cudaError_t e = cudaGetSymbolAddress(&bits, g_norm_status);
+  return e != cudaSuccess ? e : take_status(static_cast<unsigned*>(bits), word);
 }
 }  // namespace fvo
 

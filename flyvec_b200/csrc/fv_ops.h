@@ -244,7 +244,11 @@ constexpr long long WAIT_LIMIT = 4000000000ll;
 long long wait_limit(long long set = -2);
 
 int sm_count(int device);  // cached per device; 0 after an error
-cudaError_t norm_status(uint32_t* word);  // reads and clears the error bits of fv_norm.cu's kernels
+
+// Reads and clears a word of error bits in device memory in one step, so that a bit raised meanwhile is not lost.  The caller
+// (fv_ops_status) has waited for the device and lets no other thread in.
+cudaError_t take_status(unsigned* bits, uint32_t* word);
+cudaError_t norm_status(uint32_t* word);  // that of fv_norm.cu's kernels
 
 }  // namespace fvo
 

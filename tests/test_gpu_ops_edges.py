@@ -4,6 +4,7 @@ import subprocess
 import sys
 from pathlib import Path
 
+import numpy as np
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -12,6 +13,16 @@ from flyvec_b200 import ops  # noqa: E402
 from tests.test_gpu_ops import made  # noqa: E402
 
 pytestmark = pytest.mark.gpu
+
+
+def word_model(path, K, V, weights=None):
+    """A model of V words w1, w2, ... in K neurons."""
+    from flyvec_b200 import FlyVec, synth
+
+    np.save(path / "syn.npy", synth.make_weights(K, 2 * V, seed=2) if weights is None else weights)
+    (path / "vocab.txt").write_text("\n".join(["<UNK>"] + [f"w{i}" for i in range(1, V)]))
+    (path / "config.yaml").write_text("synapses: syn.npy\ntokenizer: vocab.txt\n")
+    return FlyVec.from_config(path / "config.yaml")
 
 
 def norm_call(rows, cols, dtype):
@@ -96,3 +107,32 @@ assert ops.device_status() == 0
 def test_threads_that_meet_a_kernel_first_with_different_widths(built_lib):
     done = subprocess.run([sys.executable, "-c", FIRST_MEETING], cwd=Path(__file__).resolve().parent.parent, capture_output=True, text=True, timeout=300)
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+def test_the_status_waits_for_side_streams(built_lib):
+    """PyTorch's streams are non-blocking: the default stream does not wait for them."""
+    big = torch.randn(8192, 8192, device="cuda")
+    side, end = torch.cuda.Stream(), torch.cuda.Event()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            big = (big @ big) * 1e-4
+        end.record()
+    assert ops.device_status() == 0
+    assert end.query()
+
+
+def test_word_scores_of_a_wait_that_ran_out_are_an_error(built_lib, tmp_path):
+    from flyvec_b200 import _lib
+
+    m = word_model(tmp_path, 64, 500)
+    idx, words = np.arange(12, dtype=np.int32).reshape(3, 4), [1, 2, 3]
+    m.hasher  # noqa: B018  made beforehand: the waits of the operators alone run out
+    try:
+        assert built_lib.fv_ops_wait_limit(0) == 0
+        with pytest.raises(_lib.FlyvecError, match="FV_ERR_TIMEOUT"):
+            m.word_log_probs(idx, words)
+    finally:
+        assert built_lib.fv_ops_wait_limit(-1) == 0
+    again = word_model(tmp_path, 64, 500)
+    np.testing.assert_array_equal(m.word_log_probs(idx, words).log_prob, again.word_log_probs(idx, words).log_prob)
