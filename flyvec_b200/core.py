@@ -19,6 +19,10 @@ from .tokenizer import GensimTokenizer, VocabTokenizer
 
 __all__ = ["softmax", "normalize_synapses", "FlyVec"]
 
+# Added to a variance before its root so that constant activations standardise to 0.  Normalised synapses have variances of
+# 1e-5 and less over the neurons: anything near that would shrink the correlations.
+_NO_VARIANCE = 1e-30
+
 
 def softmax(x: np.ndarray, beta: float = 1.0):
     """Softmax of a 1-D vector at inverse temperature ``beta`` (flyvec/core.py:17-20)."""
@@ -200,11 +204,11 @@ class FlyVec:
         from . import ops
 
         V = self.hasher.V
-        return ops.layer_norm(self.hasher.activations(np.arange(V, 2 * V, dtype=np.int32)[:, None]), out_dtype="bfloat16")
+        return ops.layer_norm(self.hasher.activations(np.arange(V, 2 * V, dtype=np.int32)[:, None]), eps=_NO_VARIANCE, out_dtype="bfloat16")
 
     def word_log_probs(self, idx, words, beta: float = 20.0, top: int = 0):
         """How well words fit contexts: ``softmax(beta * r)`` over the vocabulary, ``r`` the correlation (over the
-        neurons) of a context's dense activation with a word's dense embedding.
+        neurons) of a context's dense activation with a word's dense embedding (0 where one of them is constant).
 
         ``idx``: int32 ``[n][w]`` input ids of the contexts as in :meth:`hash_windows` (negative: padding); ``words``: ``[n]`` token
         ids, -1 for none.  Returns :class:`flyvec_b200.ops.TokenLogProbs` of host arrays: the words' log probabilities, the
@@ -220,7 +224,7 @@ class FlyVec:
         chunk = max(1, (256 << 20) // (4 * V))  # rows of scores held at once
         parts = []
         for a in range(0, max(len(idx), 1), chunk):
-            x = ops.layer_norm(self.hasher.activations(idx[a:a + chunk]), out_dtype="bfloat16")
+            x = ops.layer_norm(self.hasher.activations(idx[a:a + chunk]), eps=_NO_VARIANCE, out_dtype="bfloat16")
             scores = ops.linear(x, table, out_dtype="float32")  # K times the correlations
             r = ops.token_log_probs(scores, DeviceArray.from_numpy(words[a:a + chunk], device=self.device), beta=beta / K, top=top)
             parts.append([None if v is None else v.numpy() for v in r])

@@ -136,3 +136,30 @@ def test_word_scores_of_a_wait_that_ran_out_are_an_error(built_lib, tmp_path):
         assert built_lib.fv_ops_wait_limit(-1) == 0
     again = word_model(tmp_path, 64, 500)
     np.testing.assert_array_equal(m.word_log_probs(idx, words).log_prob, again.word_log_probs(idx, words).log_prob)
+
+
+def test_word_scores_do_not_depend_on_the_scale_of_the_synapses(built_lib, tmp_path):
+    """Correlations: normalised synapses (elements of 1e-2 and less) answer like large ones, a power of two changes no bit."""
+    from flyvec_b200 import synth
+
+    K, V = 64, 500
+    W = synth.make_weights(K, 2 * V, seed=2)
+    W /= np.linalg.norm(W, axis=1, keepdims=True)
+    rng = np.random.default_rng(5)
+    idx, words = rng.integers(0, V, (40, 4)).astype(np.int32), rng.integers(0, V, 40)
+    W[:, idx[7]] = 0.25  # a context without variance
+    z = lambda a: (a - a.mean(1, keepdims=True)) / np.maximum(a.std(1, keepdims=True), 1e-12)  # noqa: E731
+    s = 12.0 * z(W[:, idx].sum(-1).T.astype(np.float64)) @ z(W[:, V:].T.astype(np.float64)).T / K
+    want = s[np.arange(40), words] - np.log(np.exp(s).sum(1))
+    # as for the test of the words' log probabilities: a standardised value is rounded to bfloat16
+    tol = 2 * 12.0 * 2.0 ** -8 * 1.01
+    answers = []
+    for k, scale in enumerate((1.0, 2.0 ** -14, 2.0 ** 10)):
+        (tmp_path / str(k)).mkdir()
+        r = word_model(tmp_path / str(k), K, V, (W * scale).astype(np.float32)).word_log_probs(idx, words, beta=12.0, top=5)
+        assert np.abs(r.log_prob - want).max() < tol
+        assert abs(r.log_prob[7] + np.log(V)) < 1e-5
+        answers.append(r)
+    for r in answers[1:]:
+        for a, b in zip(r, answers[0]):
+            np.testing.assert_array_equal(a, b)
