@@ -157,6 +157,15 @@ def _vector(x, n: int, what: str, like, types):
     return x if x.is_contiguous() else x.contiguous()
 
 
+def _row_vector(x, lead, rows: int, what: str, like, types):
+    """A dense vector with one element a row, of the rows' own shape or on one axis: of [T, B] for rows [B, T] every element
+    would go to another row."""
+    x = _vector(x, rows, what, like, types)
+    if len(x.shape) != 1:
+        _same_shape(x, lead, what)
+    return x
+
+
 def _same_shape(x, shape, what: str):
     if tuple(x.shape) != tuple(shape):
         raise ValueError(f"{what} must have shape {tuple(shape)}, got {tuple(x.shape)}")
@@ -226,7 +235,7 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, out_dtype: str | No
 
 def layer_norm_backward(dy, x, mean, rstd, weight=None):
     """``(dx, dweight, dbias)`` of :func:`layer_norm` from the gradient ``dy`` of its result and the statistics it
-    returned; without a weight the last two are None.  The weight's gradients are sums over all rows, formed in
+    returned (shaped like ``x`` without its last axis, or flat); without a weight the last two are None.  The weight's gradients are sums over all rows, formed in
     float32 in a fixed order and rounded once."""
     _check(x, "x", DTYPES)
     rows, cols, step = _rows(x, "x")
@@ -236,8 +245,8 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None):
     _check(dy, "dy", (kind,), x)
     _same_shape(dy, x.shape, "dy")
     _, _, gstep = _rows(dy, "dy")
-    mean = _vector(mean, rows, "mean", x, ("float32",))
-    rstd = _vector(rstd, rows, "rstd", x, ("float32",))
+    mean = _row_vector(mean, x.shape[:-1], rows, "mean", x, ("float32",))
+    rstd = _row_vector(rstd, x.shape[:-1], rows, "rstd", x, ("float32",))
     if weight is not None:
         weight = _vector(weight, cols, "weight", x, (kind,))
     dx = _like(x)
@@ -380,7 +389,8 @@ def token_log_probs(logits, targets, beta: float = 1.0, top: int = 0) -> TokenLo
 
 def token_log_probs_backward(grad_log_prob, logits, targets, row_max, log_z, entropy=None, grad_entropy=None, beta: float = 1.0):
     """Gradient by the logits (in their type) of ``sum(grad_log_prob * log_prob) + sum(grad_entropy * entropy)``; ``row_max``,
-    ``log_z`` and, where the entropy has a gradient, ``entropy`` as :func:`token_log_probs` returned them.  Padding
+    ``log_z`` and, where the entropy has a gradient, ``entropy`` as :func:`token_log_probs` returned them, and the gradients, are
+    float32 and shaped like ``targets`` or flat.  Padding
     rows get the entropy's part only, rows of -inf only get zeros."""
     _check(logits, "logits", DTYPES)
     rows, vocab, step = _rows(logits, "logits")
@@ -388,16 +398,16 @@ def token_log_probs_backward(grad_log_prob, logits, targets, row_max, log_z, ent
         raise ValueError("the vocabulary is empty")
     if not (0 < beta < math.inf):
         raise ValueError(f"beta must be positive and finite, got {beta}")
+    lead, f32 = logits.shape[:-1], ("float32",)
     targets = _vector(targets, rows, "targets", logits, _INTS)
-    _same_shape(targets, logits.shape[:-1], "targets")
-    f32 = ("float32",)
-    grad_log_prob = _vector(grad_log_prob, rows, "grad_log_prob", logits, f32)
-    row_max, log_z = _vector(row_max, rows, "row_max", logits, f32), _vector(log_z, rows, "log_z", logits, f32)
+    _same_shape(targets, lead, "targets")
+    grad_log_prob = _row_vector(grad_log_prob, lead, rows, "grad_log_prob", logits, f32)
+    row_max, log_z = _row_vector(row_max, lead, rows, "row_max", logits, f32), _row_vector(log_z, lead, rows, "log_z", logits, f32)
     if grad_entropy is not None:
         if entropy is None:
             raise ValueError("the entropy's gradient needs the entropy")
-        grad_entropy = _vector(grad_entropy, rows, "grad_entropy", logits, f32)
-        entropy = _vector(entropy, rows, "entropy", logits, f32)
+        grad_entropy = _row_vector(grad_entropy, lead, rows, "grad_entropy", logits, f32)
+        entropy = _row_vector(entropy, lead, rows, "entropy", logits, f32)
     else:
         entropy = None
     dx, dev = _like(logits), logits.get_device()

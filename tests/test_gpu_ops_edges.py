@@ -163,3 +163,19 @@ def test_word_scores_do_not_depend_on_the_scale_of_the_synapses(built_lib, tmp_p
     for r in answers[1:]:
         for a, b in zip(r, answers[0]):
             np.testing.assert_array_equal(a, b)
+
+
+def test_row_vectors_on_one_axis(built_lib):
+    """[B, T] rows and their values flat; as many values in [T, B] are refused."""
+    x, t = made((2, 3, 500), "float32", 1), torch.randint(0, 500, (2, 3), device="cuda")
+    g = made((2, 3), "float32", 2)
+    r = ops.token_log_probs(x, t)
+    want = ops.token_log_probs_backward(g, x, t, r.row_max, r.log_z)
+    assert torch.equal(ops.token_log_probs_backward(g.reshape(-1), x, t, r.row_max.reshape(-1), r.log_z), want)
+    with pytest.raises(ValueError, match="grad_log_prob must have shape"):
+        ops.token_log_probs_backward(g.t(), x, t, r.row_max, r.log_z)
+    _, mean, rstd = ops.layer_norm(x, return_stats=True)
+    want = ops.layer_norm_backward(x, x, mean, rstd)[0]
+    assert torch.equal(ops.layer_norm_backward(x, x, mean.reshape(-1), rstd)[0], want)
+    with pytest.raises(ValueError, match="rstd must have shape"):
+        ops.layer_norm_backward(x, x, mean, rstd.t())

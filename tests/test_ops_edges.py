@@ -5,6 +5,9 @@ from pathlib import Path
 
 import pytest
 
+from flyvec_b200 import ops
+from tests.test_ops_refusals import Fake
+
 ROOT = Path(__file__).resolve().parent.parent
 
 
@@ -21,3 +24,24 @@ def test_threads_that_ask_for_different_shared_memory(tmp_path):
                     "-o", str(exe)], check=True)
     done = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
     assert done.returncode == 0, done.stdout
+
+
+def test_row_vectors_of_another_shape_are_refused(built_lib):
+    """As many elements in another order: [T, B] for rows [B, T].  One axis for all rows has the rows' order."""
+    rows, flat = Fake((2, 3)), Fake((6,))
+    x, t, w = Fake((2, 3, 8)), Fake((2, 3), "int64"), Fake((8,))
+    for wrong in (Fake((3, 2)), Fake((1, 6)), Fake((2, 3, 1))):
+        for args, kw, what in [((x, x, wrong, rows, w), {}, "mean"), ((x, x, rows, wrong, w), {}, "rstd"), ((x, x, rows, wrong), {}, "rstd")]:
+            with pytest.raises(ValueError, match=what + " must have shape"):
+                ops.layer_norm_backward(*args, **kw)
+        with pytest.raises(ValueError, match="targets must have shape"):
+            ops.token_log_probs(x, Fake(wrong.shape, "int32"))
+        for args, kw, what in [((wrong, x, t, rows, rows), {}, "grad_log_prob"), ((rows, x, t, wrong, rows), {}, "row_max"),
+                               ((rows, x, Fake(wrong.shape, "int64"), rows, rows), {}, "targets"), ((rows, x, t, rows, wrong), {}, "log_z"),
+                               ((rows, x, t, rows, rows, wrong), {"grad_entropy": rows}, "entropy"),
+                               ((rows, x, t, rows, rows, rows), {"grad_entropy": wrong}, "grad_entropy")]:
+            with pytest.raises(ValueError, match=what + " must have shape"):
+                ops.token_log_probs_backward(*args, **kw)
+    for call in (lambda: ops.layer_norm_backward(x, x, flat, flat, w), lambda: ops.token_log_probs_backward(flat, x, t, flat, flat)):
+        with pytest.raises(AssertionError, match="too late"):  # it got past the checks
+            call()
