@@ -9,7 +9,7 @@ enqueued on the current stream of the tensors' device (the default stream for ``
 return at once; they may be captured into a CUDA graph.
 
 Nothing here records a graph for automatic differentiation: tensors that require a gradient are refused
-while gradients are enabled (pass ``x.detach()``), and the ``*_backward`` functions are called by hand or from
+while gradients are enabled, and tensors with a forward-mode tangent always (pass ``x.detach()``); and the ``*_backward`` functions are called by hand or from
 a ``torch.autograd.Function``.
 
 The last axis of every array is contiguous (``linear`` also takes a transposed ``x`` or ``weight``); leading axes
@@ -36,6 +36,7 @@ MAX_TOP = 64
 _names: dict = {}  # dtype object -> name
 _torch_types: dict = {}  # name -> torch dtype
 _raw_stream = None  # (device) -> handle of the current stream
+_forward_ad = None  # torch.autograd.forward_ad
 
 
 def _type(x) -> str:
@@ -43,6 +44,15 @@ def _type(x) -> str:
     if name is None:
         name = _names[x.dtype] = str(x.dtype).replace("torch.", "")
     return name
+
+
+def _has_tangent(x) -> bool:
+    """Whether a tensor is one of forward-mode differentiation.  Outside of a level of it there are none: the question is
+    asked of every argument, so that is looked at first (0.1 instead of 0.7 us)."""
+    global _forward_ad
+    if _forward_ad is None:
+        _forward_ad = sys.modules["torch"].autograd.forward_ad
+    return getattr(_forward_ad, "_current_level", 0) >= 0 and _forward_ad.unpack_dual(x).tangent is not None
 
 
 def _refuse(x, what: str, types, like):
@@ -54,6 +64,8 @@ def _refuse(x, what: str, types, like):
             raise ValueError(f"{what} must be on a GPU, got a tensor on {x.device}")
         if x.requires_grad and sys.modules["torch"].is_grad_enabled():
             raise ValueError(f"{what} requires a gradient, which these operators do not record: pass {what}.detach()")
+        if _has_tangent(x):
+            raise ValueError(f"{what} has a forward-mode tangent, which these operators do not carry on: pass {what}.detach()")
         if x.is_neg():
             raise ValueError(f"{what} is a lazily negated view: pass {what}.resolve_neg()")
     if _type(x) not in types:
@@ -69,7 +81,8 @@ def _check(x, what: str, types, like=None):
     """One argument: a device array, of one of ``types``, on the device and of the kind of ``like``."""
     try:
         if x.is_cuda and not x.requires_grad and not x.is_neg() and _names.get(x.dtype) in types and (
-                like is None or (type(x) is type(like) and x.get_device() == like.get_device())):
+                like is None or (type(x) is type(like) and x.get_device() == like.get_device())) and (
+                isinstance(x, DeviceArray) or not _has_tangent(x)):
             return
     except AttributeError:
         pass

@@ -179,3 +179,13 @@ def test_row_vectors_on_one_axis(built_lib):
     assert torch.equal(ops.layer_norm_backward(x, x, mean.reshape(-1), rstd)[0], want)
     with pytest.raises(ValueError, match="rstd must have shape"):
         ops.layer_norm_backward(x, x, mean, rstd.t())
+
+
+def test_forward_mode_tensors(built_lib):
+    ad = torch.autograd.forward_ad
+    x = made((3, 8), "float32", 1)
+    with ad.dual_level():
+        with pytest.raises(ValueError, match="x has a forward-mode tangent"):
+            ops.layer_norm(ad.make_dual(x, x))
+        plain = ops.layer_norm(ad.make_dual(x, x).detach())
+    assert torch.equal(plain, ops.layer_norm(x))

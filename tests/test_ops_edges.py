@@ -45,3 +45,33 @@ def test_row_vectors_of_another_shape_are_refused(built_lib):
     for call in (lambda: ops.layer_norm_backward(x, x, flat, flat, w), lambda: ops.token_log_probs_backward(flat, x, t, flat, flat)):
         with pytest.raises(AssertionError, match="too late"):  # it got past the checks
             call()
+
+
+def test_forward_mode_tensors_are_refused(built_lib):
+    """A dual tensor does not require a gradient, yet its tangent would be lost."""
+    torch = pytest.importorskip("torch")
+    ad = torch.autograd.forward_ad
+
+    class OnGpu(torch.Tensor):
+        """A tensor that says it lies on a GPU; nothing may ask where."""
+
+        is_cuda = True
+
+        def get_device(self):
+            return 0
+
+        def data_ptr(self):
+            raise AssertionError("the refusal came too late")
+
+    made = lambda *shape: torch.randn(*shape).as_subclass(OnGpu)  # noqa: E731
+    with ad.dual_level():
+        dual = lambda *shape: ad.make_dual(made(*shape), made(*shape))  # noqa: E731
+        t = torch.zeros(3, dtype=torch.int64).as_subclass(OnGpu)
+        half = lambda x: x.bfloat16()  # noqa: E731
+        for call, what in [(lambda: ops.layer_norm(dual(3, 8)), "x"), (lambda: ops.layer_norm(made(3, 8), dual(8)), "weight"),
+                           (lambda: ops.layer_norm_backward(dual(3, 8), made(3, 8), made(3), made(3)), "dy"),
+                           (lambda: ops.linear(half(dual(3, 8)), half(made(5, 8))), "x"), (lambda: ops.linear(half(made(3, 8)), half(dual(5, 8))), "weight"),
+                           (lambda: ops.token_log_probs(dual(3, 8), t), "logits"),
+                           (lambda: ops.token_log_probs_backward(dual(3), made(3, 8), t, made(3), made(3)), "grad_log_prob")]:
+            with pytest.raises(ValueError, match=f"{what} has a forward-mode tangent"):
+                call()
