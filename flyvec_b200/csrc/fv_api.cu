@@ -21,6 +21,9 @@ int fail(int code, const char* fmt, ...) {
   vsnprintf(buf, sizeof(buf), fmt, ap);
   va_end(ap);
   g_last_error = buf;
+  // The runtime keeps a failed call's error until someone asks, and a later launch, here or in a library that shares the
+  // runtime (PyTorch), would be taken for the one that failed.
+  if (code == FV_ERR_CUDA) (void)cudaGetLastError();
   return code;
 }
 

@@ -189,3 +189,28 @@ def test_forward_mode_tensors(built_lib):
             ops.layer_norm(ad.make_dual(x, x))
         plain = ops.layer_norm(ad.make_dual(x, x).detach())
     assert torch.equal(plain, ops.layer_norm(x))
+
+
+def test_calls_after_a_failed_one(built_lib):
+    """The runtime's record of a failure reported here does not fail the next launch, neither here nor in PyTorch."""
+    from flyvec_b200 import _lib
+    from flyvec_b200.engine import DeviceArray
+
+    x = made((4, 8), "float32", 1)
+    want, y = ops.layer_norm(x), torch.empty_like(x)
+
+    def call(device):
+        return built_lib.fv_layer_norm(device, None, x.data_ptr(), 8, 4, 8, 0, None, None, 1e-5, y.data_ptr(), 0, None, None)
+
+    assert call(99) == 2 and b"device 99" in built_lib.fv_last_error()
+    assert call(0) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(y, want)
+    assert call(99) == 2
+    assert (x + 1).sum().item() == pytest.approx((x.cpu() + 1).sum().item(), rel=1e-4)
+    with pytest.raises(_lib.FlyvecError, match="memory"):
+        DeviceArray((1 << 40,), "float32")
+    assert torch.equal(ops.layer_norm(x), want)
+    with pytest.raises(_lib.FlyvecError, match="memory"):
+        DeviceArray((1 << 40,), "float32")
+    assert torch.equal((x + 1).cpu(), x.cpu() + 1)
