@@ -25,7 +25,6 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
-#include <cmath>
 #include <type_traits>
 
 #include "fv_ops.h"
@@ -41,6 +40,7 @@ constexpr int LP_SMALL = 1024;     // rows up to here: one warp
 constexpr int LP_THREADS = 256;    // largest block, and that of every cluster
 constexpr int LP_SLOTS = 16;       // batches of a thread whose maxima are kept apart
 constexpr int LP_LIST = 256;       // batches that can be listed for their candidates
+constexpr float LP_MAX_BETA = 0x1p127f; // its product with log2(e) is still a float
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 
@@ -797,7 +797,7 @@ int fv_token_log_probs(int device, void* stream, const void* logits, int64_t str
   FV_CHECK_DTYPE(dtype, "fv_token_log_probs");
   FV_REQUIRE(rows >= 0 && rows < (1ll << 28) && vocab >= 1 && vocab < (1ll << 31) && stride >= 0, FV_ERR_INVALID,
              "fv_token_log_probs: bad shape [%lld][%lld], stride %lld", (long long)rows, (long long)vocab, (long long)stride);
-  FV_REQUIRE(beta > 0.f && std::isfinite(beta), FV_ERR_INVALID, "fv_token_log_probs: beta must be positive and finite");
+  FV_REQUIRE(beta > 0.f && beta <= LP_MAX_BETA, FV_ERR_INVALID, "fv_token_log_probs: beta must be positive and at most 2^127");
   FV_REQUIRE(top >= 0 && top <= LP_MAX_TOP && top <= vocab, FV_ERR_INVALID,
              "fv_token_log_probs: top must be in [0, min(%d, vocabulary size)], got %d", LP_MAX_TOP, top);
   if (rows == 0) return FV_OK;
@@ -842,7 +842,7 @@ int fv_token_log_probs_backward(int device, void* stream, const float* grad_log_
   FV_CHECK_DTYPE(dtype, "fv_token_log_probs_backward");
   FV_REQUIRE(rows >= 0 && rows < (1ll << 28) && vocab >= 1 && vocab < (1ll << 31) && stride >= 0, FV_ERR_INVALID,
              "fv_token_log_probs_backward: bad shape [%lld][%lld], stride %lld", (long long)rows, (long long)vocab, (long long)stride);
-  FV_REQUIRE(beta > 0.f && std::isfinite(beta), FV_ERR_INVALID, "fv_token_log_probs_backward: beta must be positive and finite");
+  FV_REQUIRE(beta > 0.f && beta <= LP_MAX_BETA, FV_ERR_INVALID, "fv_token_log_probs_backward: beta must be positive and at most 2^127");
   if (rows == 0) return FV_OK;
   FV_REQUIRE(grad_log_prob && logits && targets && row_max && log_z && (!grad_entropy || entropy) && dlogits, FV_ERR_INVALID,
              "fv_token_log_probs_backward: NULL argument");

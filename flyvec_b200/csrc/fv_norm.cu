@@ -25,6 +25,7 @@
 // is bound by memory; bf16 has twice the elements to a byte and is bound by the issue of their conversions and sums.
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include "fv_ops.h"
 
@@ -729,7 +730,7 @@ int fv_layer_norm(int device, void* stream, const void* x, int64_t x_stride, int
   FV_REQUIRE(rows >= 0 && cols >= 1 && cols < (1ll << 31), FV_ERR_INVALID, "fv_layer_norm: bad shape [%lld][%lld]", (long long)rows,
              (long long)cols);
   FV_REQUIRE(x_stride >= 0, FV_ERR_INVALID, "fv_layer_norm: negative row stride");
-  FV_REQUIRE(eps >= 0.f, FV_ERR_INVALID, "fv_layer_norm: eps must not be negative");
+  FV_REQUIRE(eps >= 0.f && std::isfinite(eps), FV_ERR_INVALID, "fv_layer_norm: eps must be finite and not negative");
   FV_REQUIRE(!bias || weight, FV_ERR_INVALID, "fv_layer_norm: a bias needs a weight");
   if (rows == 0) return FV_OK;
   FV_REQUIRE(x && y, FV_ERR_INVALID, "fv_layer_norm: NULL argument");

@@ -18,7 +18,6 @@ are taken together as rows and must lie at one common distance from one another.
 from __future__ import annotations
 
 import ctypes as C
-import math
 import sys
 from functools import lru_cache
 from typing import Any, NamedTuple
@@ -32,6 +31,10 @@ __all__ = ["layer_norm", "layer_norm_backward", "linear", "linear_backward", "to
 
 #: largest number of alternatives ``token_log_probs`` returns
 MAX_TOP = 64
+
+_FLOAT_MAX = (2 - 2.0 ** -23) * 2.0 ** 127
+#: a beta has to be a positive float32 whose product with log2(e) is one too
+_BETAS = 2.0 ** -149, 2.0 ** 127
 
 _names: dict = {}  # dtype object -> name
 _torch_types: dict = {}  # name -> torch dtype
@@ -229,8 +232,8 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, out_dtype: str | No
         raise TypeError(f"out_dtype must be one of {', '.join(DTYPES)}, got {out_dtype!r}")
     if cols == 0:
         raise ValueError("x has no columns")
-    if not 0 <= eps < math.inf:
-        raise ValueError(f"eps must be finite and not negative, got {eps}")
+    if not 0 <= eps <= _FLOAT_MAX:
+        raise ValueError(f"eps must be a finite float32 and not negative, got {eps}")
     if bias is not None and weight is None:
         raise ValueError("a bias needs a weight")
     if weight is not None:
@@ -383,8 +386,8 @@ def token_log_probs(logits, targets, beta: float = 1.0, top: int = 0) -> TokenLo
     rows, vocab, step = _rows(logits, "logits")
     if vocab == 0:
         raise ValueError("the vocabulary is empty")
-    if not (0 < beta < math.inf):
-        raise ValueError(f"beta must be positive and finite, got {beta}")
+    if not _BETAS[0] <= beta <= _BETAS[1]:
+        raise ValueError(f"beta must be between 2^-149 and 2^127, got {beta}")
     if not 0 <= top <= min(MAX_TOP, vocab):
         raise ValueError(f"top must be between 0 and min({MAX_TOP}, {vocab}), got {top}")
     lead = tuple(logits.shape[:-1])
@@ -409,8 +412,8 @@ def token_log_probs_backward(grad_log_prob, logits, targets, row_max, log_z, ent
     rows, vocab, step = _rows(logits, "logits")
     if vocab == 0:
         raise ValueError("the vocabulary is empty")
-    if not (0 < beta < math.inf):
-        raise ValueError(f"beta must be positive and finite, got {beta}")
+    if not _BETAS[0] <= beta <= _BETAS[1]:
+        raise ValueError(f"beta must be between 2^-149 and 2^127, got {beta}")
     lead, f32 = logits.shape[:-1], ("float32",)
     targets = _vector(targets, rows, "targets", logits, _INTS)
     _same_shape(targets, lead, "targets")

@@ -341,7 +341,7 @@ int fv_linear_backward(int device, void* stream, const void* dy, int64_t dy_stri
 /* Of every row of logits: log probability of its target under softmax(beta * logits), entropy, maximum logit, log of the
  * sum of exp(beta * (logit - maximum)), and the `top` (0..64) most probable tokens (larger logit first, then the lower id)
  * with their log probabilities.  targets are int32 or int64; -1 marks padding (log probability 0, no gradient), any other
- * id outside [0, vocab) gives NaN.  A row of -inf only: log probabilities -inf, entropy 0, log_z -inf, gradient 0.  A row
+ * id outside [0, vocab) gives NaN; beta is positive and at most 2^127.  A row of -inf only: log probabilities -inf, entropy 0, log_z -inf, gradient 0.  A row
  * with a NaN or +inf: NaN everywhere but in top_ids (NaN first). */
 int fv_token_log_probs(int device, void* stream, const void* logits, int64_t stride, int64_t rows, int64_t vocab, int dtype,
                        const void* targets, int targets_int64, float beta, int top, float* log_prob, float* entropy, float* row_max,

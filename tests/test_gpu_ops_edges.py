@@ -214,3 +214,18 @@ def test_calls_after_a_failed_one(built_lib):
     with pytest.raises(_lib.FlyvecError, match="memory"):
         DeviceArray((1 << 40,), "float32")
     assert torch.equal((x + 1).cpu(), x.cpu() + 1)
+
+
+def test_log_probs_at_the_ends_of_beta(built_lib):
+    """As a maximum (the largest beta) and as an average (the smallest)."""
+    x = made((4, 3000), "float32", 1)
+    x[1, 7] = x[1].max()
+    t = x.argmax(1)
+    for v in (x, x[:, :700].contiguous()):
+        t = v.argmax(1)
+        r = ops.token_log_probs(v, t, beta=2.0 ** 127, top=3)
+        ties = (v == v.amax(1, keepdim=True)).sum(1).float()
+        assert torch.allclose(r.log_prob, -ties.log(), atol=1e-6) and torch.allclose(r.entropy, ties.log(), atol=1e-6)
+        r = ops.token_log_probs(v, t, beta=2.0 ** -149, top=3)
+        n = torch.full((4,), float(v.shape[1]), device="cuda").log()
+        assert torch.allclose(r.log_prob, -n, atol=1e-5) and torch.allclose(r.entropy, n, atol=1e-5)

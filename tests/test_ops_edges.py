@@ -1,4 +1,6 @@
 """The dense operators at their edges, as far as no GPU is needed."""
+import ctypes as C
+import math
 import os
 import subprocess
 from pathlib import Path
@@ -75,3 +77,20 @@ def test_forward_mode_tensors_are_refused(built_lib):
                            (lambda: ops.token_log_probs_backward(dual(3), made(3, 8), t, made(3), made(3)), "grad_log_prob")]:
             with pytest.raises(ValueError, match=f"{what} has a forward-mode tangent"):
                 call()
+
+
+def test_numbers_that_no_float_holds_are_refused(built_lib):
+    """Python's floats reach further than the kernels': a beta that becomes 0, or infinite with log2(e), and an infinite eps."""
+    x, t, f = Fake((3, 50)), Fake((3,), "int64"), Fake((3,))
+    for beta in (3e38, 1e39, 1e-46, 0.0, -1.0, math.nan, math.inf):
+        with pytest.raises(ValueError, match="beta"):
+            ops.token_log_probs(x, t, beta=beta)
+        with pytest.raises(ValueError, match="beta"):
+            ops.token_log_probs_backward(f, x, t, f, f, beta=beta)
+    for eps in (1e39, math.inf, -1e-5, math.nan):
+        with pytest.raises(ValueError, match="eps"):
+            ops.layer_norm(x, eps=eps)
+    lib, p = built_lib, C.c_void_p(4096)
+    assert lib.fv_token_log_probs(0, None, p, 50, 3, 50, 0, p, 1, 3e38, 0, p, p, p, p, None, None) == 1 and b"beta" in lib.fv_last_error()
+    assert lib.fv_token_log_probs_backward(0, None, p, None, p, 50, 3, 50, 0, p, 1, p, p, None, 3e38, p) == 1 and b"beta" in lib.fv_last_error()
+    assert lib.fv_layer_norm(0, None, p, 8, 3, 8, 0, None, None, math.inf, p, 0, None, None) == 1 and b"eps" in lib.fv_last_error()
