@@ -220,7 +220,10 @@ class FlyVec:
         words = np.ascontiguousarray(words, np.int64).reshape(-1)
         if idx.ndim != 2 or len(words) != len(idx):
             raise ValueError(f"idx must have shape [n][w] and words [n], got {idx.shape} and {words.shape}")
-        K, V, table = self.hasher.K, self.hasher.V, self._word_table
+        K, V = self.hasher.K, self.hasher.V
+        if not 0 <= top <= min(ops.MAX_TOP, V):
+            raise ValueError(f"top must be between 0 and min({ops.MAX_TOP}, {V}), got {top}")
+        table = self._word_table
         chunk = max(1, (256 << 20) // (4 * V))  # rows of scores held at once
         parts = []
         for a in range(0, max(len(idx), 1), chunk):
@@ -234,9 +237,14 @@ class FlyVec:
         return ops.TokenLogProbs(*(None if v[0] is None else np.concatenate(v) for v in zip(*parts)))
 
     def similar_words(self, word: str, top: int = 10, beta: float = 20.0):
-        """The ``top`` words whose dense embeddings correlate best with that of the first token of ``word``, itself left
-        out: a list of ``(token, log probability)`` under :meth:`word_log_probs`; empty for an unknown word."""
-        if self.is_unknown_token(word):
+        """The ``top`` (at most 63, fewer in a smaller vocabulary) words whose dense embeddings correlate best with that of the
+        first token of ``word``, itself left out: a list of ``(token, log probability)`` under :meth:`word_log_probs`; empty for an
+        unknown word."""
+        from .ops import MAX_TOP
+
+        if not 0 <= top < MAX_TOP:  # the word itself is asked for too
+            raise ValueError(f"top must be between 0 and {MAX_TOP - 1}, got {top}")
+        if top == 0 or self.is_unknown_token(word):
             return []
         tok_id = self.tokenizer.token2id(self.tokenizer.tokenize(word)[0])
         V = self.hasher.V

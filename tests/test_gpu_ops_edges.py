@@ -229,3 +229,15 @@ def test_log_probs_at_the_ends_of_beta(built_lib):
         r = ops.token_log_probs(v, t, beta=2.0 ** -149, top=3)
         n = torch.full((4,), float(v.shape[1]), device="cuda").log()
         assert torch.allclose(r.log_prob, -n, atol=1e-5) and torch.allclose(r.entropy, n, atol=1e-5)
+
+
+def test_similar_words_counts(built_lib, tmp_path):
+    m = word_model(tmp_path, 64, 500)
+    most = m.similar_words("w7", top=63)
+    assert len(most) == 63 and "w7" not in dict(most) and m.similar_words("w7", top=5) == most[:5]
+    for top in (65, -1):
+        with pytest.raises(ValueError, match=f"got {top}"):
+            m.word_log_probs([[1]], [2], top=top)
+    (tmp_path / "few").mkdir()
+    few = word_model(tmp_path / "few", 64, 12)
+    assert len(few.similar_words("w7", top=63)) == 11

@@ -94,3 +94,15 @@ def test_numbers_that_no_float_holds_are_refused(built_lib):
     assert lib.fv_token_log_probs(0, None, p, 50, 3, 50, 0, p, 1, 3e38, 0, p, p, p, p, None, None) == 1 and b"beta" in lib.fv_last_error()
     assert lib.fv_token_log_probs_backward(0, None, p, None, p, 50, 3, 50, 0, p, 1, p, p, None, 3e38, p) == 1 and b"beta" in lib.fv_last_error()
     assert lib.fv_layer_norm(0, None, p, 8, 3, 8, 0, None, None, math.inf, p, 0, None, None) == 1 and b"eps" in lib.fv_last_error()
+
+
+def test_similar_words_refuses(tmp_path):
+    """Before anything is loaded, with the number the caller gave."""
+    from flyvec_b200 import FlyVec
+
+    (tmp_path / "vocab.txt").write_text("<UNK>\nw1\nw2")
+    m = FlyVec(tmp_path / "nothing.npy", tmp_path / "vocab.txt")
+    for top in (64, 65, 1000, -1, -2):
+        with pytest.raises(ValueError, match=f"between 0 and 63, got {top}"):
+            m.similar_words("w1", top=top)
+    assert m.similar_words("w1", top=0) == [] and m.similar_words("nothere") == []
