@@ -929,13 +929,15 @@ struct PackJob {
   } one[2];
   int count;
   int64_t rows, cols;  // the most of either
+  unsigned across;     // blocks along x that take the columns; as many again take further rows
 };
 __device__ __forceinline__ void pack_rows(const PackJob& job, int which) {
   const auto& j = job.one[which];
-  const int64_t c0 = ((int64_t)blockIdx.x * 32 + (threadIdx.x & 31)) * 8;
-  if (c0 >= j.cols) return;
+  const unsigned times = gridDim.x / job.across, turn = blockIdx.x / job.across;
+  const int64_t c0 = ((int64_t)(blockIdx.x - turn * job.across) * 32 + (threadIdx.x & 31)) * 8;
+  if (c0 >= j.cols || turn >= times) return;
 #pragma unroll 2
-  for (int64_t r = (int64_t)blockIdx.y * 8 + (threadIdx.x >> 5); r < j.rows; r += (int64_t)gridDim.y * 8) {
+  for (int64_t r = ((int64_t)turn * gridDim.y + blockIdx.y) * 8 + (threadIdx.x >> 5); r < j.rows; r += (int64_t)times * gridDim.y * 8) {
     uint16_t v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = c0 + i < j.cols ? __ldg(j.src + r * j.ld + c0 + i) : (uint16_t)0;
@@ -1034,7 +1036,9 @@ __global__ void __launch_bounds__(256)
 template <typename T, int VEC>
 cudaError_t launch_act_grad(cudaStream_t st, const T* dy, int64_t ldg, const T* z, int64_t ldz, int64_t rows, int64_t outer, int act, T* dz,
                             int64_t pitch, float* part, T* db, int64_t chunks, const PackJob& job) {
-  const unsigned gx = (unsigned)((outer + 32 * VEC - 1) / (32 * VEC)), px = job.count ? (unsigned)((job.cols + 255) / 256) : 0u;
+  const unsigned gx = (unsigned)((outer + 32 * VEC - 1) / (32 * VEC));
+  // the rows to copy may be many more than dy's, by which y goes: blocks along x take them, up to four rows to a warp
+  const unsigned px = job.count ? job.across * (unsigned)((job.rows + 32 * chunks - 1) / (32 * chunks)) : 0u;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(std::max(gx, px), (unsigned)chunks, 1u + (unsigned)job.count);
   cfg.blockDim = dim3(256);
@@ -1109,6 +1113,7 @@ int plan_pack(Operand& a, Operand& b, Workspace& ws, PackJob* job) {
     job->one[job->count++] = {static_cast<const uint16_t*>(o->p), dst, o->ld, o->outer(), o->inner(), pitch};
     job->rows = std::max(job->rows, o->outer());
     job->cols = std::max(job->cols, o->inner());
+    job->across = (unsigned)((job->cols + 255) / 256);
     o->p = dst;
     o->ld = pitch;
   }
@@ -1118,7 +1123,7 @@ int plan_pack(Operand& a, Operand& b, Workspace& ws, PackJob* job) {
 }
 int pack_operands(const PackJob& job, cudaStream_t st) {
   if (!job.count) return FV_OK;
-  k_pack<<<dim3((unsigned)((job.cols + 255) / 256), (unsigned)std::min<int64_t>((job.rows + 7) / 8, 4096), (unsigned)job.count), 256, 0, st>>>(job);
+  k_pack<<<dim3(job.across, (unsigned)std::min<int64_t>((job.rows + 7) / 8, 4096), (unsigned)job.count), 256, 0, st>>>(job);
   FV_CUDA(cudaGetLastError());
   return FV_OK;
 }
