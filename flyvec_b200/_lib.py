@@ -125,6 +125,7 @@ _PROTOTYPES = {
     "fv_layer_norm": ([C.c_int, _P, _P, _I, _I, _I, C.c_int, _P, _P, C.c_float, _P, C.c_int, _P, _P], C.c_int),
     "fv_layer_norm_backward_workspace": ([C.c_int, _I, _I, C.c_int, C.POINTER(C.c_size_t)], C.c_int),
     "fv_layer_norm_backward": ([C.c_int, _P, _P, _I, _P, _I, _I, _I, C.c_int, _P, _P, _P, _P, _P, _P, _P, C.c_size_t], C.c_int),
+    "fv_linear_shapes": ([C.c_int, _I, _I, _I, C.c_int, C.POINTER(C.c_int32)], C.c_int),
     "fv_linear_workspace": ([_I, _I, _I, _P, _I, _I, _P, _I, _I, C.POINTER(C.c_size_t)], C.c_int),
     "fv_linear": ([C.c_int, _P, _P, _I, _I, _P, _I, _I, _I, _I, _I, C.c_int, _P, C.c_int, _P, _I, _P, C.c_int, _P, _P, C.c_size_t],
                   C.c_int),

@@ -1220,6 +1220,16 @@ Shape choose_shape(const Size* sizes, int count, int sms, bool narrow, double* t
   return best;
 }
 
+// The two products of a backward pass: in one launch of one shape (answers 1) or in two.
+int choose_backward(const Size* sizes, int sms, Shape* shapes) {
+  double one = 0, two[2] = {0, 0};
+  const Shape joint = choose_shape(sizes, 2, sms, false, &one);
+  for (int i = 0; i < 2; ++i) shapes[i] = choose_shape(&sizes[i], 1, sms, false, &two[i]);
+  if (one > two[0] + two[1]) return 2;
+  shapes[0] = joint;
+  return 1;
+}
+
 template <typename T, int BN, bool PAIR>
 int launch_gemm(const GemmMaps& maps, const GemmJob& job, unsigned grid, int splits, cudaStream_t st) {
   static std::atomic<bool> given[64];
@@ -1360,6 +1370,29 @@ int fv_ops_status(int device, uint32_t* word) {
 int fv_ops_wait_limit(int64_t cycles) {
   FV_REQUIRE(cycles >= -1, FV_ERR_INVALID, "fv_ops_wait_limit: %lld cycles", (long long)cycles);
   wait_limit(cycles);
+  return FV_OK;
+}
+
+int fv_linear_shapes(int sms, int64_t rows, int64_t inner, int64_t outer, int backward, int32_t* shapes) {
+  FV_REQUIRE(shapes && sms >= 2 && sms <= 1024 && rows >= 1 && sizes_ok(rows, inner, outer), FV_ERR_INVALID, "fv_linear_shapes: bad argument");
+  auto blocks = [](int64_t n) { return (n + BK - 1) / BK; };
+  Shape s[2];
+  int count = 1;
+  if (backward) {
+    Size sizes[2] = {{rows, inner, blocks(outer)}, {outer, inner, blocks(rows)}};
+    if (rows > outer) std::swap(sizes[0], sizes[1]);
+    count = choose_backward(sizes, sms, s);
+  } else {
+    const bool narrow = rows <= NARROW_ROWS;
+    const Size size{narrow ? outer : rows, narrow ? rows : outer, blocks(inner)};
+    s[0] = choose_shape(&size, 1, sms, narrow, nullptr);
+  }
+  *shapes++ = count;
+  for (int i = 0; i < count; ++i) {
+    *shapes++ = s[i].bn;
+    *shapes++ = s[i].splits;
+    *shapes++ = s[i].pair;
+  }
   return FV_OK;
 }
 
@@ -1538,12 +1571,10 @@ int fv_linear_backward(int device, void* stream, const void* dy, int64_t dy_stri
   Product d[2] = {{od, transposed(ow), px}, {transposed(od), transposed(ox), pw}};
   if (rows > outer) std::swap(d[0], d[1]);  // the one with the longer sums first
   const Size sizes[2] = {size_of(d[0]), size_of(d[1])};
-  double one = 0, two[2] = {0, 0};
-  const Shape joint = choose_shape(sizes, 2, sms, false, &one);
-  const Shape each[2] = {choose_shape(&sizes[0], 1, sms, false, &two[0]), choose_shape(&sizes[1], 1, sms, false, &two[1])};
-  if (one <= two[0] + two[1]) return gemm(d, 2, dtype, joint, sms, st);
+  Shape shapes[2];
+  if (choose_backward(sizes, sms, shapes) == 1) return gemm(d, 2, dtype, shapes[0], sms, st);
   for (int i = 0; i < 2; ++i)
-    if (int rc = gemm(&d[i], 1, dtype, each[i], sms, st)) return rc;
+    if (int rc = gemm(&d[i], 1, dtype, shapes[i], sms, st)) return rc;
   return FV_OK;
 }
 

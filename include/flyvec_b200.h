@@ -331,6 +331,10 @@ int fv_linear_workspace(int64_t rows, int64_t inner, int64_t outer, const void* 
 int fv_linear(int device, void* stream, const void* x, int64_t x_rs, int64_t x_cs, const void* w, int64_t w_rs, int64_t w_cs, int64_t rows,
               int64_t inner, int64_t outer, int dtype, const void* bias, int act, const void* residual, int64_t residual_stride, void* y,
               int y_dtype, void* z, void* workspace, size_t workspace_bytes);
+/* How the tensor-core kernel divides a product (backward: the two of a backward pass) on a GPU of `sms` multiprocessors: int32
+ * [7] receives the number of launches and for each the tile width, the blocks that share a tile's sums, and whether pairs of
+ * blocks share tiles.  (One or two rows are done without it.) */
+int fv_linear_shapes(int sms, int64_t rows, int64_t inner, int64_t outer, int backward, int32_t* shapes);
 /* dz = dy act'(z), dx = dz w, dw = dz^T x (dense [outer][inner]), db = column sums of dz; the residual's gradient is dy. */
 int fv_linear_backward_workspace(int device, int64_t rows, int64_t inner, int64_t outer, const void* dy, int64_t dy_stride, const void* x,
                                  int64_t x_rs, int64_t x_cs, const void* w, int64_t w_rs, int64_t w_cs, int act, size_t* bytes);

@@ -8,6 +8,7 @@ from pathlib import Path
 import pytest
 
 from flyvec_b200 import ops
+from tests import product_shapes
 from tests.test_ops_refusals import Fake
 
 ROOT = Path(__file__).resolve().parent.parent
@@ -106,3 +107,14 @@ def test_similar_words_refuses(tmp_path):
         with pytest.raises(ValueError, match=f"between 0 and 63, got {top}"):
             m.similar_words("w1", top=top)
     assert m.similar_words("w1", top=0) == [] and m.similar_words("nothere") == []
+
+
+def test_the_products_sizes_reach_every_form(built_lib):
+    """The sizes at which the products are compared with 64 bits take the forms they are listed for."""
+    for size, want in product_shapes.FORWARD.items():
+        assert product_shapes.shapes(built_lib, product_shapes.SMS, size, False) == [want], size
+    for size, want in product_shapes.BACKWARD.items():
+        assert product_shapes.shapes(built_lib, product_shapes.SMS, size, True) == want, size
+    bad = (C.c_int32 * 7)()
+    assert built_lib.fv_linear_shapes(148, 0, 8, 8, 0, bad) == 1 and built_lib.fv_linear_shapes(1, 8, 8, 8, 0, bad) == 1
+    assert built_lib.fv_linear_shapes(148, 8, 8, 8, 0, None) == 1
