@@ -10,6 +10,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 from flyvec_b200 import ops  # noqa: E402
+from tests import product_shapes  # noqa: E402
 from tests import test_gpu_ops as base  # noqa: E402
 from tests.test_gpu_ops import made  # noqa: E402
 
@@ -276,3 +277,24 @@ def test_copies_do_not_go_by_the_rows_of_the_gradient(built_lib):
         return lambda: ops.linear_backward(dy, x, w)
 
     assert graph_time(call(16)) < 1.5 * graph_time(call(777))
+
+
+# ---- every form of the product kernel --------------------------------------------------------------------
+@pytest.mark.parametrize("size", list(product_shapes.FORWARD), ids=lambda s: "x".join(map(str, s)))
+def test_linear_in_every_form(built_lib, size):
+    """With bias, activation, residual and pre-activation, in both types of result; the sums in the order of each form."""
+    base.test_linear(built_lib, *size, "float16" if size[0] % 3 == 0 else "bfloat16")
+
+
+@pytest.mark.parametrize("size", list(product_shapes.BACKWARD), ids=lambda s: "x".join(map(str, s)))
+def test_linear_backward_in_every_form(built_lib, size):
+    base.test_linear_backward(built_lib, *size, "float16" if size[0] % 3 == 0 else "bfloat16")
+
+
+def test_the_forms_on_this_gpu(built_lib):
+    """With another number of multiprocessors than the sizes were chosen for, some forms may not have run."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    got = {f for size in product_shapes.FORWARD for f in product_shapes.shapes(built_lib, sms, size, False)}
+    if sms != product_shapes.SMS:
+        pytest.skip(f"{sms} multiprocessors: forms {sorted(got)}")
+    assert got == set(product_shapes.FORWARD.values())
