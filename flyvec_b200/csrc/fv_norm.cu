@@ -595,7 +595,7 @@ __global__ void __launch_bounds__(512)
 
 struct NormPlan {
   bool is_long, block, edge;
-  int words;           // 16-byte words per thread: 1, 2, 4 or 8
+  int words;           // 16-byte words per thread
   int threads, stages, pitch;
   int64_t grid;
   size_t smem;
@@ -665,26 +665,28 @@ cudaError_t launch_norm_grad(const NormPlan& p, cudaStream_t st, const T* dy, in
   return cudaGetLastError();
 }
 
-// eight words a thread: the float forward pass alone
-template <typename T, int NV, bool BLOCK, bool EDGE, typename... A>
-cudaError_t launch_norm_widest(const NormPlan& p, A... a) {
-  if constexpr (sizeof(T) == 4) return launch_norm<T, NV, BLOCK, EDGE>(p, a...);
-  return cudaErrorInvalidValue;
+// The forms that plan_norm chooses: a warp's threads hold one, two or four words; a block's two or four of a gradient, four of a
+// 16-bit forward row, two, four or eight of a float one.
+template <typename T, bool EDGE, typename... A>
+cudaError_t launch_norm_form(const NormPlan& p, A... a) {
+  if (!p.block)
+    return p.words == 1   ? launch_norm<T, 1, false, EDGE>(p, a...)
+           : p.words == 2 ? launch_norm<T, 2, false, EDGE>(p, a...)
+                          : launch_norm<T, 4, false, EDGE>(p, a...);
+  if constexpr (sizeof(T) == 4) {
+    if (p.words == 2) return launch_norm<T, 2, true, EDGE>(p, a...);
+    if (p.words == 8) return launch_norm<T, 8, true, EDGE>(p, a...);
+  }
+  return launch_norm<T, 4, true, EDGE>(p, a...);
 }
-template <typename T, int NV, bool BLOCK, bool EDGE, typename... A>
-cudaError_t launch_norm_grad_widest(const NormPlan&, A...) {
-  return cudaErrorInvalidValue;
+template <typename T, bool EDGE, typename... A>
+cudaError_t launch_norm_grad_form(const NormPlan& p, A... a) {
+  if (!p.block)
+    return p.words == 1   ? launch_norm_grad<T, 1, false, EDGE>(p, a...)
+           : p.words == 2 ? launch_norm_grad<T, 2, false, EDGE>(p, a...)
+                          : launch_norm_grad<T, 4, false, EDGE>(p, a...);
+  return p.words == 2 ? launch_norm_grad<T, 2, true, EDGE>(p, a...) : launch_norm_grad<T, 4, true, EDGE>(p, a...);
 }
-
-#define NORM_EDGE(p, FN, T, NV, BLOCK, ...) ((p).edge ? FN<T, NV, BLOCK, true>(p, __VA_ARGS__) : FN<T, NV, BLOCK, false>(p, __VA_ARGS__))
-#define NORM_LAUNCH(p, FN, T, ...)                                                                                   \
-  (!(p).block ? ((p).words == 1   ? NORM_EDGE(p, FN, T, 1, false, __VA_ARGS__)                                       \
-                 : (p).words == 2 ? NORM_EDGE(p, FN, T, 2, false, __VA_ARGS__)                                       \
-                                  : NORM_EDGE(p, FN, T, 4, false, __VA_ARGS__))                                      \
-              : ((p).words == 1   ? NORM_EDGE(p, FN, T, 1, true, __VA_ARGS__)                                        \
-                 : (p).words == 2 ? NORM_EDGE(p, FN, T, 2, true, __VA_ARGS__)                                        \
-                 : (p).words == 4 ? NORM_EDGE(p, FN, T, 4, true, __VA_ARGS__)                                        \
-                                  : NORM_EDGE(p, FN##_widest, T, 8, true, __VA_ARGS__)))
 
 int64_t grad_parts(const NormPlan& p, int64_t rows, int64_t D, int sms) {
   if (!p.is_long) return p.grid;
@@ -749,7 +751,8 @@ int fv_layer_norm(int device, void* stream, const void* x, int64_t x_stride, int
       k_norm_long<T><<<(unsigned)p.grid, p.threads, 0, st>>>(px, x_stride, rows, cols, pw, pb, eps, y, y_dtype, mean, rstd);
       e = cudaGetLastError();
     } else {
-      e = NORM_LAUNCH(p, launch_norm, T, st, px, x_stride, rows, (int)cols, pw, pb, eps, y, y_dtype, mean, rstd);
+      e = p.edge ? launch_norm_form<T, true>(p, st, px, x_stride, rows, (int)cols, pw, pb, eps, y, y_dtype, mean, rstd)
+                 : launch_norm_form<T, false>(p, st, px, x_stride, rows, (int)cols, pw, pb, eps, y, y_dtype, mean, rstd);
     }
   });
   FV_CUDA(e);
@@ -814,7 +817,8 @@ int fv_layer_norm_backward(int device, void* stream, const void* dy, int64_t dy_
         k_norm_grad_cols<T><<<dim3((unsigned)((cols + 255) / 256), (unsigned)parts), 256, 0, st>>>(pg, dy_stride, px, x_stride, rows, cols,
                                                                                                   mean, rstd, part);
     } else {
-      e = NORM_LAUNCH(p, launch_norm_grad, T, st, pg, dy_stride, px, x_stride, rows, (int)cols, mean, rstd, pw, pd, part);
+      e = p.edge ? launch_norm_grad_form<T, true>(p, st, pg, dy_stride, px, x_stride, rows, (int)cols, mean, rstd, pw, pd, part)
+                 : launch_norm_grad_form<T, false>(p, st, pg, dy_stride, px, x_stride, rows, (int)cols, mean, rstd, pw, pd, part);
     }
     if (part)
       k_norm_grad_reduce<T><<<(unsigned)((2 * cols + 31) / 32), 512, 0, st>>>(part, parts, cols, static_cast<T*>(dweight),
