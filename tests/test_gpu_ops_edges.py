@@ -298,3 +298,69 @@ def test_the_forms_on_this_gpu(built_lib):
     if sms != product_shapes.SMS:
         pytest.skip(f"{sms} multiprocessors: forms {sorted(got)}")
     assert got == set(product_shapes.FORWARD.values())
+
+
+# ---- offsets past 2^31 elements --------------------------------------------------------------------------
+def far_rows(n, at):
+    """Rows at the front, around the one in which element 2^31 lies, at the end."""
+    return [slice(0, 700), slice(at - 350, at + 350), slice(n - 700, n)]
+
+
+def test_layer_norm_of_far_rows(built_lib):
+    """A row's result is the same wherever the row lies; 700 rows take the form of all."""
+    n, d = 560000, 4096
+    x = made((n, d), "bfloat16", 1)
+    w = made((d,), "bfloat16", 2, 0, 0.2, 1.0)
+    y, mean, rstd = ops.layer_norm(x, w, return_stats=True)
+    dx, dw, db = ops.layer_norm_backward(x, y, mean, rstd, w)
+    want_b = torch.zeros(d, dtype=torch.float64, device="cuda")
+    for a in range(0, n, 40000):
+        want_b += x[a:a + 40000].double().sum(0)
+    for s in far_rows(n, 2 ** 31 // d):
+        part = ops.layer_norm(x[s].clone(), w, return_stats=True)
+        assert torch.equal(y[s], part[0]) and torch.equal(mean[s], part[1]) and torch.equal(rstd[s], part[2])
+        assert torch.equal(dx[s], ops.layer_norm_backward(x[s].clone(), y[s].clone(), part[1], part[2], w)[0])
+    # sums of n normal values (of size sqrt(n)): a block's n / 296 rows one after the other, then a tree, each addition off by
+    # 2^-24 of a partial sum of the size of the whole at most, and the rounding to bfloat16
+    tol = (n / 296 + 20) * base.U * 4 * n ** 0.5 + want_b.abs() * base.half_step("bfloat16")
+    assert ((db.double() - want_b).abs() <= tol).all()
+
+
+def test_linear_of_far_rows(built_lib):
+    def check(x, w, rows):
+        y = ops.linear(x, w)
+        for s in rows:
+            want = x[s].double() @ w.double().t()
+            base.close(y[s], want, base.rounded(want, "bfloat16", base.product_slack(x[s], w.t(), x.shape[1])))
+        return y
+
+    x, w = made((560000, 4096), "bfloat16", 1), base.weight(72, 4096, "bfloat16", 2, False)
+    check(x, w, far_rows(560000, 2 ** 31 // 4096))
+    x, w = x[:120000, :64], base.weight(20000, 64, "bfloat16", 3, False)
+    y = check(x, w, far_rows(120000, 2 ** 31 // 20000))
+    dx, dw, db = ops.linear_backward(y, x, w)
+    for s in far_rows(120000, 2 ** 31 // 20000):
+        want = y[s].double() @ w.double()
+        base.close(dx[s], want, base.rounded(want, "bfloat16", base.product_slack(y[s], w, 20000)))
+    del y, dx
+    wide = torch.zeros(60, 40_000_000, device="cuda", dtype=torch.bfloat16)  # rows far apart
+    wide[:, :136] = made((60, 136), "bfloat16", 4)
+    for k in (0, 1):  # read where they lie, and copied
+        x = wide[:, k:k + 128]
+        for rows in (2, 60):
+            for w in (base.weight(72, 128, "bfloat16", 5, False), x):
+                assert torch.equal(ops.linear(x[:rows], w), ops.linear(x[:rows].contiguous(), w.contiguous()))
+
+
+def test_token_log_probs_of_far_rows(built_lib):
+    n, v = 120000, 20000
+    x = made((n, v), "bfloat16", 1)
+    t = torch.arange(n, device="cuda") * 7 % v
+    g = made((n,), "float32", 2)
+    r = ops.token_log_probs(x, t, top=5)
+    d = ops.token_log_probs_backward(g, x, t, r.row_max, r.log_z)
+    for s in far_rows(n, 2 ** 31 // v):
+        part = ops.token_log_probs(x[s].clone(), t[s], top=5)
+        for a, b in zip(r, part):
+            assert torch.equal(a[s], b)
+        assert torch.equal(d[s], ops.token_log_probs_backward(g[s], x[s].clone(), t[s], part.row_max, part.log_z))
