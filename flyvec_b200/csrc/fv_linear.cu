@@ -147,18 +147,19 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-// Waits for the phase of the given parity; false when the limit (0: no look at all) ran out here or elsewhere in the block.
+// Waits for the phase of the given parity; false when the limit ran out here or elsewhere in the block.
 __device__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* stop, long long limit) {
-  if (limit > 0 && mbar_try(bar, parity)) return true;
+  if (mbar_try(bar, parity)) return true;
   const long long t0 = clock64();
-  while (limit > 0) {
+  for (;;) {
     if (mbar_try(bar, parity)) return true;
     if (*stop) return false;
-    if (clock64() - t0 > limit) break;
+    if (clock64() - t0 > limit) {
+      *stop = 1;
+      atomicOr(&g_status, 1u);
+      return false;
+    }
   }
-  *stop = 1;
-  atomicOr(&g_status, 1u);
-  return false;
 }
 // One thread of a converged warp, in a form that the compiler knows to be one thread: the loads and products below
 // take their operands from uniform registers, and under a plain lane == 0 each would be wrapped in a loop over lanes
@@ -536,7 +537,8 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
       mbar_init(acc_empty(a), PAIR ? 2 * EPI_WARPS : EPI_WARPS);
     }
     mbar_init(drained, 1);
-    *stop = 0;
+    *stop = job.limit == 0;  // waits that last no longer than a look
+    if (*stop) atomicOr(&g_status, 1u);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -682,7 +684,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
       for (int j = 0; j < 4; ++j) bias_reg[j] = bias_next[j];
       fetch_ahead(t_next, false);
       bool ahead = false;  // the next tile's first residual slice is on its way
-      if (!__all_sync(FULL, mbar_wait(acc_full(acc), acc_phase, stop, job.limit))) break;  // the warp stays together
+      mbar_wait(acc_full(acc), acc_phase, stop, job.limit);  // if it runs out the warp goes on, together, with what there is
       tc_fence_after();
       const uint32_t src = tmem + acc * BN + ((uint32_t)(quarter * 32) << 16);
       if (!PAIR && job.splits > 1) {  // to shared memory (the ring is free: every load was consumed before acc_full)

@@ -153,12 +153,11 @@ __device__ __forceinline__ uint32_t ring_bytes(const void* row, int bytes) {
 __device__ __forceinline__ void ring_expect(uint64_t* bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(shared_addr(bar)), "r"(bytes) : "memory");
 }
-// Bounded wait for a stage; false when the copies did not arrive within `limit` cycles (0: gives up without a look).  A
-// thread whose wait ran out goes on without waiting or copying, so that all threads of its group keep meeting at the same
-// barriers, and outlasts the copies in flight before it ends; the results are invalid.
-__device__ __forceinline__ bool ring_wait(uint64_t* bar, int parity, long long limit) {
-  long long t0 = 0;
-  while (limit > 0) {
+// Bounded wait for a stage.  A thread whose wait ran out is `late`: it goes on without waiting or copying, so that all
+// threads of its group keep meeting at the same barriers, and outlasts the copies in flight before it ends; the results
+// are invalid.  A limit of 0 cycles makes every thread late from the start.
+__device__ __forceinline__ void ring_wait(uint64_t* bar, int parity, long long limit, bool& late) {
+  for (long long t0 = 0;;) {
     uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
@@ -167,13 +166,14 @@ __device__ __forceinline__ bool ring_wait(uint64_t* bar, int parity, long long l
         : "=r"(ok)
         : "r"(shared_addr(bar)), "r"(parity)
         : "memory");
-    if (ok) return true;
+    if (ok || late) return;
     const long long now = clock64();
     if (t0 == 0) t0 = now;
-    if (now - t0 > limit) break;
+    if (now - t0 > limit) {
+      atomicOr(&g_norm_status, 1u);
+      late = true;
+    }
   }
-  atomicOr(&g_norm_status, 1u);
-  return false;
 }
 // A group's place: its threads, its first row and the distance to its next.
 template <bool BLOCK>
@@ -263,6 +263,10 @@ __global__ void __launch_bounds__(BLOCK ? NORM_MAX_THREADS : 32 * NORM_WARPS)
   };
   if (g.t == 0)
     for (int s = 0; s < stages; ++s) fetch(g.first + s * g.step, s);
+  if (limit == 0) {
+    late = true;
+    atomicOr(&g_norm_status, 1u);
+  }
   const int off = EDGE ? (int)(((uintptr_t)(x + g.first * xs) & 15) / sizeof(T)) : 0;
   const Columns<VEC, NV> col{off, D, g.t, g.size};
   int turn = 0;
@@ -280,7 +284,7 @@ __global__ void __launch_bounds__(BLOCK ? NORM_MAX_THREADS : 32 * NORM_WARPS)
   const int pivot_at = EDGE ? (wide ? VEC : off) : 0;
   int s = 0, parity = 0;
   for (int64_t r = g.first; r < rows; r += g.step, out += hop) {
-    late = late || !ring_wait(ring.bars + s, parity, limit);
+    ring_wait(ring.bars + s, parity, limit, late);
     const T* stage = reinterpret_cast<const T*>(ring.base + (size_t)s * pitch);
     float pivot;
     if (wide) {
@@ -410,6 +414,10 @@ __global__ void __launch_bounds__(BLOCK ? NORM_MAX_THREADS : 32 * NORM_WARPS)
   };
   if (g.t == 0)
     for (int s = 0; s < stages; ++s) fetch(g.first + s * g.step, s);
+  if (limit == 0) {
+    late = true;
+    atomicOr(&g_norm_status, 1u);
+  }
   const int off = EDGE ? (int)(((uintptr_t)(x + g.first * xs) & 15) / sizeof(T)) : 0;
   const int goff = EDGE ? (int)(((uintptr_t)(dy + g.first * gs) & 15) / sizeof(T)) : 0;
   const Columns<VEC, NV> col{off, D, g.t, g.size};
@@ -436,7 +444,7 @@ __global__ void __launch_bounds__(BLOCK ? NORM_MAX_THREADS : 32 * NORM_WARPS)
       next_mu = mean[r + g.step];
       next_rs = rstd[r + g.step];
     }
-    late = late || !ring_wait(ring.bars + s, parity, limit);
+    ring_wait(ring.bars + s, parity, limit, late);
     const T* sx = reinterpret_cast<const T*>(ring.base + (size_t)s * 2 * pitch);
     const T* sg = reinterpret_cast<const T*>(ring.base + (size_t)s * 2 * pitch + pitch);
     // h and dy of word j, 0 outside the row

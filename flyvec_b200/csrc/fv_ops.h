@@ -239,7 +239,7 @@ struct OnDevice {
 };
 
 // Cycles after which a bounded wait inside a kernel gives up, about two seconds; wait_limit answers what the next launches get
-// (and sets it first: -1 the default, 0 waits that give up at once).
+// (and sets it first: -1 the default, 0 waits that last no longer than a look).
 constexpr long long WAIT_LIMIT = 4000000000ll;
 long long wait_limit(long long set = -2);
 

@@ -360,7 +360,8 @@ int fv_token_log_probs_backward(int device, void* stream, const float* grad_log_
  * call's outputs are invalid); waits for the device and clears them. */
 int fv_ops_status(int device, uint32_t* word);
 /* Clock cycles after which the waits of kernels launched from now on give up, in this process: -1 the default (about two
- * seconds), 0 waits that give up at once.  For trying out what a caller does about fv_ops_status. */
+ * seconds), 0 waits that last no longer than a look and calls that count as run out.  For trying out what a caller does about
+ * fv_ops_status. */
 int fv_ops_wait_limit(int64_t cycles);
 
 /* ---- raw buffers (cuda_helpers.cu:8-29 do_gpu_cudaHostAlloc & co.) ------- */
