@@ -21,7 +21,7 @@
 //
 // 10000 x 20000 bf16: 73 us (5.5 TB/s) without alternatives, bound by the issue of ex2 and the arithmetic around it; 97 us with
 // ten, whose search (two more barriers, a second trip to L2) hides only in part behind the other blocks' rows.  4096 x 50000
-// float: 131 us (6.2 TB/s) and 155 us.  1280 threads per SM: 1024 are 5 % slower, 1536 spill.
+// float: 131 us (6.2 TB/s) and 158 us with twenty.  1280 threads per SM: 1024 are 5 % slower, 1536 spill.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -694,7 +694,8 @@ __device__ __forceinline__ GradRow grad_row(int64_t row, long long t, int64_t V,
   return r;
 }
 // A block takes some 1024 words of one row, four to a thread; they are aligned to the gradient, which is dense.  Bound by
-// memory: 4096 x 50000, bf16 132 us (6.2 TB/s read and written), float 259 us (6.3 TB/s); half as many words a block 170 us.
+// memory: 4096 x 50000, bf16 130 us (6.3 TB/s read and written), float 258 us (6.4 TB/s); half as many words a block 170 us.  float16
+// costs more instructions to convert, and the issue slots are 86 % full with bf16: 10000 x 20000 157 us where bf16 takes 133.
 template <typename T>
 __global__ void __launch_bounds__(256)
     k_log_probs_grad(const T* __restrict__ logits, int64_t xs, int64_t V, int chunks, const void* __restrict__ targets, int t64,

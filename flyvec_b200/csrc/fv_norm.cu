@@ -21,8 +21,10 @@
 // atomics: the same inputs give the same bits).  Rows of more than 32 KB (64 KB in the float forward pass) are read
 // again from L2 instead of being held.
 //
-// 16384 x 4096: forward bf16 56 us (4.8 TB/s), float 90 us (5.9 TB/s); backward bf16 82 us (4.9 TB/s), float 132 us (6.1 TB/s).  float
-// is bound by memory; bf16 has twice the elements to a byte and is bound by the issue of their conversions and sums.
+// 16384 x 4096: forward 16-bit 55 us (4.9 TB/s), float 90 us (6.0 TB/s); backward bf16 82 us and float16 85 us (4.9 and 4.7 TB/s), float
+// 132 us (6.1 TB/s).  float is bound by memory.  16-bit rows have twice the elements to a byte, and neither memory nor the issue
+// slots are full (55 and 52 % of them issue): the 16 warps an SM that the registers allow wait on fixed latencies, on reads
+// of shared memory and, backward, at the barrier of the row's sums.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
