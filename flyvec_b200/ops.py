@@ -9,8 +9,8 @@ enqueued on the current stream of the tensors' device (the default stream for ``
 return at once; they may be captured into a CUDA graph.
 
 Nothing here records a graph for automatic differentiation: tensors that require a gradient are refused
-while gradients are enabled, and tensors with a forward-mode tangent always (pass ``x.detach()``); and the ``*_backward`` functions are called by hand or from
-a ``torch.autograd.Function``.
+while gradients are enabled, and tensors with a forward-mode tangent always (pass ``x.detach()``).  The ``*_backward``
+functions are called by hand or from a ``torch.autograd.Function``.
 
 The last axis of every array is contiguous (``linear`` also takes a transposed ``x`` or ``weight``); leading axes
 are taken together as rows and must lie at one common distance from one another.
@@ -251,8 +251,8 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, out_dtype: str | No
 
 def layer_norm_backward(dy, x, mean, rstd, weight=None):
     """``(dx, dweight, dbias)`` of :func:`layer_norm` from the gradient ``dy`` of its result and the statistics it
-    returned (shaped like ``x`` without its last axis, or flat); without a weight the last two are None.  The weight's gradients are sums over all rows, formed in
-    float32 in a fixed order and rounded once."""
+    returned (shaped like ``x`` without its last axis, or flat); without a weight the last two are None.  The weight's
+    gradients are sums over all rows, formed in float32 in a fixed order and rounded once."""
     _check(x, "x", DTYPES)
     rows, cols, step = _rows(x, "x")
     kind = _type(x)
